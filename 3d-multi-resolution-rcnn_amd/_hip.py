@@ -45,8 +45,20 @@ def lib():
         L.mr3d_status_string.argtypes = [ctypes.c_int]
         L.mr3d_nms3d_workspace_bytes.restype = ctypes.c_size_t
         L.mr3d_nms3d_workspace_bytes.argtypes = [ctypes.c_int]
+        _declare(L)
         _lib = L
     return _lib
+
+
+def _declare(L):
+    """argument types of the calls whose cost at the smallest sizes is the binding's: converted without a look at each value"""
+    p, i, ll, f, z = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_size_t
+    for name, res, args in (
+            ('mr3d_layer_norm_workspace_bytes', z, [ll, i, i]),
+            ('mr3d_layer_norm_forward', i, [p, ll, p, p, p, p, p, ll, i, f, i, i, p]),
+            ('mr3d_layer_norm_backward', i, [p, ll, p, ll, p, p, p, p, p, p, ll, i, i, i, p, z, p])):
+        fn = getattr(L, name)
+        fn.restype, fn.argtypes = res, args
 
 
 def check(status, what):
@@ -1348,3 +1360,43 @@ def mask_bce(pred, target, labels, valid_rows=None, want_grad=True):
                                  ptr(_loss_workspace(pred.device)), stream_ptr(pred.device))
     check(st, 'mr3d_mask_bce')
     return loss, grad
+
+
+# --------------------------------------------------------------------------------------------
+STORAGE_DTYPES = {torch.float32: 0, torch.bfloat16: 1}                   # MR3D_DTYPE_F32 / _BF16
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def layer_norm_forward(x, weight, bias, eps, want_stats):
+    """x [rows, cols] (last axis contiguous) -> y, mean, rstd (None without want_stats)"""
+    rows, cols = x.shape
+    y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if want_stats else None
+    param = weight if weight is not None else bias
+    pd = STORAGE_DTYPES[param.dtype if param is not None else x.dtype]
+    sp = None if stats is None else stats.data_ptr()
+    with torch.cuda.device(x.device):
+        check(lib().mr3d_layer_norm_forward(x.data_ptr(), x.stride(0), _addr(weight), _addr(bias), y.data_ptr(), sp,
+                                            None if sp is None else sp + 4 * rows, rows, cols, eps, STORAGE_DTYPES[x.dtype], pd,
+                                            torch.cuda.current_stream(x.device).cuda_stream), 'mr3d_layer_norm_forward')
+    return y, stats
+
+
+def layer_norm_backward(x, dy, weight, stats, param_dtype, want_dx, want_dw, want_db):
+    rows, cols = x.shape
+    dev = x.device
+    dx = torch.empty((rows, cols), dtype=x.dtype, device=dev) if want_dx else None
+    dw = torch.empty((cols,), dtype=param_dtype, device=dev) if want_dw else None
+    db = torch.empty((cols,), dtype=param_dtype, device=dev) if want_db else None
+    dt = STORAGE_DTYPES[x.dtype]
+    with torch.cuda.device(dev):
+        need = lib().mr3d_layer_norm_workspace_bytes(rows, cols, dt) if want_dw or want_db else 0
+        ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+        check(lib().mr3d_layer_norm_backward(x.data_ptr(), x.stride(0), dy.data_ptr(), dy.stride(0), _addr(weight), stats.data_ptr(),
+                                             stats.data_ptr() + 4 * rows, _addr(dx), _addr(dw), _addr(db), rows, cols, dt,
+                                             STORAGE_DTYPES[param_dtype], _addr(ws), need,
+                                             torch.cuda.current_stream(dev).cuda_stream), 'mr3d_layer_norm_backward')
+    return dx, dw, db

@@ -513,6 +513,22 @@ int mr3d_linear_wgrad(const float *dy, const float *x, float *dw, int rows, int 
                       float *workspace, long long workspace_bytes, mr3d_stream_t s);
 
 /* ------------------------------------------------------------------------------------------------
+ * Layer norm over the last axis of [rows][cols] (csrc/norm.hip); not part of the reference, which normalises with frozen BatchNorm.
+ *   y = (x - mean) / sqrt(var + eps) * weight + bias        var: the biased variance
+ * x / dy rows are x_stride / dy_stride elements apart (0: one row for all; the last axis is contiguous), y and dx are packed.  dtype of x, y, dy, dx:
+ * MR3D_DTYPE_F32 or MR3D_DTYPE_BF16; param_dtype of weight, bias and their gradients: MR3D_DTYPE_F32 or dtype.  weight / bias may be
+ * NULL (1 / 0).  mean / rstd [rows] (fp32): both NULL or both written by forward, read by backward.  dx, dweight, dbias: any may be
+ * NULL; with dweight or dbias, workspace (device memory, 4-byte aligned) of mr3d_layer_norm_workspace_bytes is needed.  cols <= 16384 (a row
+ * lives in one workgroup's registers), else MR3D_ERR_UNSUPPORTED.  Sums in fp32, over rows in double at the end; bits do not vary between runs.
+ * ---------------------------------------------------------------------------------------------- */
+size_t mr3d_layer_norm_workspace_bytes(long long rows, int cols, int dtype);
+int mr3d_layer_norm_forward(const void *x, long long x_stride, const void *weight, const void *bias, void *y, float *mean, float *rstd,
+                            long long rows, int cols, float eps, int dtype, int param_dtype, mr3d_stream_t s);
+int mr3d_layer_norm_backward(const void *x, long long x_stride, const void *dy, long long dy_stride, const void *weight, const float *mean,
+                             const float *rstd, void *dx, void *dweight, void *dbias, long long rows, int cols, int dtype,
+                             int param_dtype, void *workspace, size_t workspace_bytes, mr3d_stream_t s);
+
+/* ------------------------------------------------------------------------------------------------
  * DeformConv3d (v1) / modulated (v2): the sampling halves of the operator; the GEMM halves are
  * mr3d_conv3d_forward / mr3d_conv3d_wgrad over the column matrix (see csrc/deform_conv3d.hip).
  * Extends the reference's 2D operator (mmdet/ops/dcn/src/deform_conv_cuda_kernel.cu:83-435,569-766 and
