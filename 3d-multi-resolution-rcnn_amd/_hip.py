@@ -57,8 +57,9 @@ def _declare(L):
             ('mr3d_layer_norm_workspace_bytes', z, [ll, i, i]),
             ('mr3d_layer_norm_forward', i, [p, ll, p, p, p, p, p, ll, i, f, i, i, p]),
             ('mr3d_layer_norm_backward', i, [p, ll, p, ll, p, p, p, p, p, p, ll, i, i, i, p, z, p])):
-        fn = getattr(L, name)
-        fn.restype, fn.argtypes = res, args
+        fn = getattr(L, name, None)          # MR3D_LIB may name an older build
+        if fn is not None:
+            fn.restype, fn.argtypes = res, args
 
 
 def check(status, what):
