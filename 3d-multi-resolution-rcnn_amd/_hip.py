@@ -54,6 +54,8 @@ def _declare(L):
     """argument types of the calls whose cost at the smallest sizes is the binding's: converted without a look at each value"""
     p, i, ll, f, z = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_size_t
     for name, res, args in (
+            ('mr3d_orthogonalize_workspace_bytes', z, [p, i]),
+            ('mr3d_orthogonalize', i, [p, i, i, f, f, f, f, p, z, p]),
             ('mr3d_layer_norm_workspace_bytes', z, [ll, i, i]),
             ('mr3d_layer_norm_forward', i, [p, ll, p, p, p, p, p, ll, i, f, i, i, p]),
             ('mr3d_layer_norm_backward', i, [p, ll, p, ll, p, p, p, p, p, p, ll, i, i, i, p, z, p])):
@@ -1401,3 +1403,22 @@ def layer_norm_backward(x, dy, weight, stats, param_dtype, want_dx, want_dw, wan
                                              STORAGE_DTYPES[param_dtype], _addr(ws), need,
                                              torch.cuda.current_stream(dev).cuda_stream), 'mr3d_layer_norm_backward')
     return dx, dw, db
+
+
+class Matrix(ctypes.Structure):
+    """mr3d_matrix (include/mr3d.h)"""
+    _fields_ = [('in_', ctypes.c_void_p), ('out', ctypes.c_void_p), ('rows', ctypes.c_longlong), ('cols', ctypes.c_longlong),
+                ('in_row_stride', ctypes.c_longlong), ('in_col_stride', ctypes.c_longlong), ('dtype', ctypes.c_int), ('reserved', ctypes.c_int)]
+
+
+def orthogonalize(mats, outs, steps, coefficients, eps):
+    """mats: 2-D tensors of one device, none of them empty; outs: packed tensors of the same types and sizes (may be mats themselves)"""
+    dev = mats[0].device
+    table = (Matrix * len(mats))(*[(m.data_ptr(), o.data_ptr(), m.shape[0], m.shape[1], *m.stride(), STORAGE_DTYPES[m.dtype], 0)
+                                   for m, o in zip(mats, outs)])
+    a, b, c = coefficients
+    with torch.cuda.device(dev):
+        need = lib().mr3d_orthogonalize_workspace_bytes(table, len(mats))
+        ws = torch.empty((max(need, 256),), dtype=torch.uint8, device=dev)
+        check(lib().mr3d_orthogonalize(table, len(mats), steps, a, b, c, eps, ws.data_ptr(), need, torch.cuda.current_stream(dev).cuda_stream),
+              'mr3d_orthogonalize')

@@ -529,6 +529,26 @@ int mr3d_layer_norm_backward(const void *x, long long x_stride, const void *dy, 
                              int param_dtype, void *workspace, size_t workspace_bytes, mr3d_stream_t s);
 
 /* ------------------------------------------------------------------------------------------------
+ * Orthogonalised updates of a list of matrices by Newton-Schulz products (csrc/ortho.hip); not part of the reference, whose optimiser is SGD.
+ *   X = G / (|G|_F + eps), transposed when rows > cols;   steps times:  A = X X^T,  X = a X + (b A + c A A) X;   out = X (transposed back)
+ * in: element (r, c) at in[r * in_row_stride + c * in_col_stride]; out: packed row-major [rows][cols], of the same dtype (MR3D_DTYPE_F32 / _BF16);
+ * out may be in itself (packed), no other overlap.  The whole list runs in one launch per stage.  Products carry 22 bits of each
+ * factor with fp32 accumulation; bits do not vary between runs.  1 <= steps <= 100, |a|, |b|, |c| <= 16, rows and cols up to 2^20; singular values that
+ * the polynomial drives beyond about 4 overflow to infinity or NaN, and an input with NaN or infinity gives NaN in its own matrix.
+ * workspace: 256-byte aligned device memory of mr3d_orthogonalize_workspace_bytes(the same list; 0 = the list is refused); mats_host is read
+ * before the call returns.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct {
+  const void *in;
+  void *out;
+  long long rows, cols, in_row_stride, in_col_stride;
+  int dtype, reserved;
+} mr3d_matrix;
+size_t mr3d_orthogonalize_workspace_bytes(const mr3d_matrix *mats_host, int count);
+int mr3d_orthogonalize(const mr3d_matrix *mats_host, int count, int steps, float a, float b, float c, float eps, void *workspace,
+                       size_t workspace_bytes, mr3d_stream_t s);
+
+/* ------------------------------------------------------------------------------------------------
  * DeformConv3d (v1) / modulated (v2): the sampling halves of the operator; the GEMM halves are
  * mr3d_conv3d_forward / mr3d_conv3d_wgrad over the column matrix (see csrc/deform_conv3d.hip).
  * Extends the reference's 2D operator (mmdet/ops/dcn/src/deform_conv_cuda_kernel.cu:83-435,569-766 and
