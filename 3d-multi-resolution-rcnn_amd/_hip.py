@@ -54,6 +54,9 @@ def _declare(L):
     """argument types of the calls whose cost at the smallest sizes is the binding's: converted without a look at each value"""
     p, i, ll, f, z = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_size_t
     for name, res, args in (
+            ('mr3d_linear_cross_entropy_workspace_bytes', z, [p]),
+            ('mr3d_linear_cross_entropy', i, [p, p, z, p]),
+            ('mr3d_scale_by', i, [p, ll, i, p, p]),
             ('mr3d_orthogonalize_workspace_bytes', z, [p, i]),
             ('mr3d_orthogonalize', i, [p, i, i, f, f, f, f, p, z, p]),
             ('mr3d_layer_norm_workspace_bytes', z, [ll, i, i]),
@@ -1422,3 +1425,42 @@ def orthogonalize(mats, outs, steps, coefficients, eps):
         ws = torch.empty((max(need, 256),), dtype=torch.uint8, device=dev)
         check(lib().mr3d_orthogonalize(table, len(mats), steps, a, b, c, eps, ws.data_ptr(), need, torch.cuda.current_stream(dev).cuda_stream),
               'mr3d_orthogonalize')
+
+
+class LinearCe(ctypes.Structure):
+    """mr3d_linear_ce (include/mr3d.h)"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ('x', 'weight', 'bias', 'labels', 'row_weight', 'avg_factor_dev', 'valid_rows_dev', 'loss', 'dx',
+                                               'dweight', 'dbias')] + \
+               [(n, ctypes.c_longlong) for n in ('x_stride', 'weight_stride', 'ignore_index')] + [('avg_factor', ctypes.c_float)] + \
+               [(n, ctypes.c_int) for n in ('rows', 'hidden', 'classes', 'dtype', 'param_dtype', 'want_dx', 'want_dweight', 'want_dbias')]
+
+
+def linear_cross_entropy(x, weight, bias, labels, row_weight, avg_factor, valid_rows, ignore_index, want_dx, want_dw, want_db):
+    """x [rows, hidden], weight [classes, hidden] (last axes contiguous) -> loss [1], dx, dweight, dbias (None where not wanted)"""
+    dev = x.device
+    rows, hidden = x.shape
+    classes = weight.shape[0]
+    loss = torch.empty((1,), dtype=torch.float32, device=dev)
+    dx = torch.empty((rows, hidden), dtype=x.dtype, device=dev) if want_dx else None
+    dw = torch.empty((classes, hidden), dtype=x.dtype, device=dev) if want_dw else None
+    db = torch.empty((classes,), dtype=bias.dtype, device=dev) if want_db else None
+    on_dev = torch.is_tensor(avg_factor)
+    a = LinearCe(x.data_ptr(), weight.data_ptr(), _addr(bias), labels.data_ptr(), _addr(row_weight), avg_factor.data_ptr() if on_dev else None,
+                 _addr(valid_rows), loss.data_ptr(), _addr(dx), _addr(dw), _addr(db), x.stride(0), weight.stride(0), ignore_index,
+                 0.0 if on_dev or avg_factor is None else avg_factor, rows, hidden, classes, STORAGE_DTYPES[x.dtype],
+                 STORAGE_DTYPES[x.dtype if bias is None else bias.dtype], want_dx, want_dw, want_db)
+    ref = ctypes.byref(a)
+    with torch.cuda.device(dev):
+        need = lib().mr3d_linear_cross_entropy_workspace_bytes(ref)
+        ws = torch.empty((need + 1024,), dtype=torch.uint8, device=dev)
+        check(lib().mr3d_linear_cross_entropy(ref, ws.data_ptr() + -ws.data_ptr() % 1024, need, torch.cuda.current_stream(dev).cuda_stream),
+              'mr3d_linear_cross_entropy')
+    return loss, dx, dw, db
+
+
+def scale_by(t, factor):
+    """t *= factor (a device scalar) in place; free when the factor is 1"""
+    with torch.cuda.device(t.device):
+        check(lib().mr3d_scale_by(t.data_ptr(), t.numel(), STORAGE_DTYPES[t.dtype], factor.data_ptr(),
+                                  torch.cuda.current_stream(t.device).cuda_stream), 'mr3d_scale_by')
+    return t

@@ -1,0 +1,689 @@
+// Softmax cross entropy of a linear classifier over many classes, with its gradients, without the [rows][classes] logits:
+//   z = x W^T + b      loss = sum_i w_i (lse(z_i) - z_i[label_i]) / avg
+//   g = (softmax(z) - onehot(label)) w / avg      dx = g W      dW = g^T x      db = sum_i g
+// 6 R V K operations with gradients; the loss and the gradients leave the same call (the caller scales them by the incoming gradient).
+//   rows     live rows (weight not 0, label not ignored, row < valid_rows) are numbered; the others cost nothing further, take no part
+//            in any product (NaN in them stays there) and get a zero row of dx
+//   pack     live rows of x (and W, where its storage is not what the products read) into gemm16.h's operand form
+//   logits   z tile by tile; a wave holds 128 classes of a row: it leaves exp(z - max of the 128) and (max, sum).  The exponentials take the place
+//            of the logits: 2 bytes a value (bf16: relative to their own maximum they lose what g's own rounding loses anyway), 4 for fp32
+//   grad     per row: lse from the (max, sum) pairs, the label's logit once more as a dot product, loss; exponentials -> g in place
+//   dx, dw   g W (split over the classes, parts added in a fixed order) and g^T x
+// The exponentials of at most kPiece bytes of rows exist at a time; dW accumulates over such pieces in fp32.
+// Recomputing z for the gradient instead (no such buffer at all) costs 2 R V K more: 1.7 ps a logit at 1024 features against 0.8 ps for the
+// buffer's extra trip through memory.
+#include "gemm16.h"
+
+using namespace gemm16;
+
+namespace {
+
+typedef __bf16 bf16;
+constexpr float kSG = 16384.f;                               // fp32: g without its weight, in [-1, 1], times this
+constexpr long long kPiece = 1ll << 31;
+constexpr int kStatCols = 128;                               // classes per (max, sum) pair
+
+struct Ce {
+  const char *x, *w, *bias;
+  const long long *labels;
+  const float *row_weight, *avg_dev;
+  const int *valid_rows;
+  float avg_host;
+  long long x_stride, w_stride, ignore;                      // strides in elements
+  int rows, hidden, classes, bias_f32;
+  // workspace
+  int *head;                                                 // [0] live rows  [1] avg (float)  [2] max |W|  [3] max |x w| (float bits)
+  int *index, *pos;                                          // live row -> row, row -> live row or -1
+  float *xmax;                                               // fp32: max |x| of a live row
+  char *xp, *xwp, *wp;                                       // packed operands (wp may be the caller's W)
+  long long ldx, ldw, ldg;                                   // bytes
+  char *g;
+  float2 *stats;
+  float *part;
+  double *row_loss;
+  float *dwacc, *dbpart;
+  int cap, pieces, z;                                        // rows of a piece, (max, sum) pairs of a row, parts of dx
+  char *dx, *dw, *db;
+  float *loss;
+  int db_f32;
+};
+
+template <bool F32> __device__ __forceinline__ float elem(const char *p, long long i) {
+  return F32 ? ((const float *)p)[i] : (float)((const bf16 *)p)[i];
+}
+
+// largest power of two that keeps |v| <= max below 2^14
+__device__ __forceinline__ float scale_for(float max) {
+  if (!(max > 0.f) || !(max < 3.0e38f)) return 1.f;
+  int e = 14 - (ilogbf(max) + 1);
+  e = e > 120 ? 120 : e;
+  return ldexpf(1.f, e);
+}
+__device__ __forceinline__ float scale_of(const Ce &c, int slot) { return scale_for(__int_as_float(c.head[slot])); }
+
+// live rows in order: a prefix sum over 1024 rows at a time by one workgroup
+__global__ __launch_bounds__(1024) void ce_rows_kernel(Ce c) {
+  __shared__ int wsum[16], wpos[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int base = 0, positive = 0;
+  const int valid = c.valid_rows ? min(max(*c.valid_rows, 0), c.rows) : c.rows;
+  for (int r0 = 0; r0 < c.rows; r0 += 1024) {
+    const int r = r0 + threadIdx.x;
+    bool live = false, pos = false;
+    if (r < valid) {
+      const float w = c.row_weight ? c.row_weight[r] : 1.f;
+      live = w != 0.f && c.labels[r] != c.ignore;
+      pos = live && w > 0.f;
+    }
+    const unsigned long long bl = __ballot(live), bp = __ballot(pos);
+    if (lane == 0) {
+      wsum[wave] = __popcll(bl);
+      wpos[wave] = __popcll(bp);
+    }
+    __syncthreads();
+    int before = base;
+    for (int k = 0; k < 16; ++k) {
+      if (k < wave) before += wsum[k];
+      base += wsum[k];
+      positive += wpos[k];
+    }
+    const int at = before + __popcll(bl & ((1ull << lane) - 1));
+    if (live) c.index[at] = r;
+    if (r < c.rows) c.pos[r] = live ? at : -1;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    c.head[0] = base;
+    ((float *)c.head)[1] = c.avg_dev ? *c.avg_dev : (c.avg_host > 0.f ? c.avg_host : (float)max(positive, 1));
+    c.head[2] = c.head[3] = 0;
+  }
+}
+
+__device__ __forceinline__ float block_max(float v, float *lds) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
+}
+
+// fp32: the largest |x| of each live row and |x w| of all, the largest |W| (the first `rows` workgroups take x, the rest W).  The maximum of
+// positive floats is the maximum of their bits: an integer atomic, whose order does not matter
+__global__ __launch_bounds__(256) void ce_max_kernel(Ce c, int wblocks) {
+  __shared__ float lds[4];
+  float m = 0.f;
+  if ((int)blockIdx.x < c.rows) {
+    if ((int)blockIdx.x >= c.head[0]) return;
+    const int r = c.index[blockIdx.x];
+    const float *x = (const float *)c.x + r * c.x_stride;
+    for (int k = threadIdx.x; k < c.hidden; k += 256) m = fmaxf(m, fabsf(x[k]));
+    m = block_max(m, lds);
+    if (threadIdx.x == 0) {
+      c.xmax[blockIdx.x] = m;
+      const float w = m * fabsf(c.row_weight ? c.row_weight[r] : 1.f);
+      if (w < 3.0e38f) atomicMax(&c.head[3], __float_as_int(w));
+      else atomicMax(&c.head[3], 0x7f800000);
+    }
+  } else {
+    for (int v = blockIdx.x - c.rows; v < c.classes; v += wblocks) {
+      const float *w = (const float *)c.w + v * c.w_stride;
+      for (int k = threadIdx.x; k < c.hidden; k += 256) m = fmaxf(m, fabsf(w[k]));
+    }
+    m = block_max(m, lds);
+    if (threadIdx.x == 0) atomicMax(&c.head[2], __float_as_int(m));
+  }
+}
+
+// one stored row of an operand: bf16 copied, fp32 split; zeros behind the last column
+template <bool F32> __device__ __forceinline__ void pack_row(const char *src, char *dst, long long ld, int cols, float scale, float factor) {
+  if constexpr (F32) {
+    const float *s = (const float *)src;
+    for (int k = threadIdx.x * 4; k < ld / 4; k += 1024) {
+      _Float16 h[4], l[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) split16(k + e < cols ? s[k + e] * factor * scale : 0.f, h[e], l[e]);
+      char *d = dst + (k >> 5) * 128 + (k & 31) * 2;
+      *reinterpret_cast<uint2 *>(d) = *reinterpret_cast<uint2 *>(h);
+      *reinterpret_cast<uint2 *>(d + 64) = *reinterpret_cast<uint2 *>(l);
+    }
+  } else {
+    const bf16 *s = (const bf16 *)src;
+    const bool vec = (((uintptr_t)src) & 15) == 0;
+    for (int k = threadIdx.x * 8; k < ld / 2; k += 2048) {
+      bf16 t[8];
+      if (vec && k + 8 <= cols) *reinterpret_cast<uint4 *>(t) = *reinterpret_cast<const uint4 *>(s + k);
+      else
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] = k + e < cols ? s[k + e] : (bf16)0.f;
+      *reinterpret_cast<uint4 *>(dst + 2 * k) = *reinterpret_cast<uint4 *>(t);
+    }
+  }
+}
+
+template <bool F32>
+__global__ __launch_bounds__(256) void ce_pack_kernel(Ce c, int want_xw) {
+  const int b = blockIdx.x;
+  if (b < c.rows) {
+    if (b >= c.head[0]) return;
+    const int r = c.index[b];
+    const char *src = c.x + r * c.x_stride * (F32 ? 4 : 2);
+    pack_row<F32>(src, c.xp + b * c.ldx, c.ldx, c.hidden, F32 ? scale_for(c.xmax[b]) : 1.f, 1.f);
+    if (F32 && want_xw) pack_row<F32>(src, c.xwp + b * c.ldx, c.ldx, c.hidden, scale_of(c, 3), c.row_weight ? c.row_weight[r] : 1.f);
+  } else {
+    const int v = b - c.rows;
+    pack_row<F32>(c.w + v * c.w_stride * (F32 ? 4 : 2), c.wp + v * c.ldw, c.ldw, c.hidden, F32 ? scale_of(c, 2) : 1.f, 1.f);
+  }
+}
+
+// z of one tile (classes x live rows) -> exponentials and (max, sum)
+template <class T, bool TRAIN>
+__global__ __launch_bounds__(T::THREADS, 2) void ce_logits_kernel(Ce c, int row0) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int live = min(c.head[0] - row0, c.cap);
+  if (live <= 0) return;
+  const int nti = (c.classes + T::BI - 1) / T::BI, ntj = (live + T::BJ - 1) / T::BJ;
+  if ((int)blockIdx.x >= nti * ntj) return;
+  int ti, tj;
+  tile_of(blockIdx.x, nti * ntj, nti, ntj, ti, tj);
+  f32x16 acc[T::TI][T::TJ];
+  run<T>(lds, side_kc(c.wp, c.ldw, c.classes, c.ldx, ti * T::BI, 0), side_kc(c.xp + row0 * c.ldx, c.ldx, live, c.ldx, tj * T::BJ, 0),
+         (int)(c.ldx / 128), acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave % T::NWI, wj = wave / T::NWI;
+  const float rsw = T::SPLIT ? 1.f / scale_of(c, 2) : 1.f;
+  const int vpad = (int)(c.ldg / (T::SPLIT ? 4 : 2));
+  constexpr int WI = T::TI * 32;
+  static_assert(WI <= kStatCols && kStatCols % WI == 0, "a wave's classes lie in one pair or its own part of it");
+#pragma unroll
+  for (int b = 0; b < T::TJ; ++b) {
+    const int j = tj * T::BJ + (wj * T::TJ + b) * 32 + (lane & 31);
+    const float rs = T::SPLIT ? rsw / scale_for(j < live ? c.xmax[row0 + j] : 0.f) : 1.f;
+    const int iw = ti * T::BI + wi * WI + (lane >> 5) * 4;
+    float m = -INFINITY;
+#pragma unroll
+    for (int a = 0; a < T::TI; ++a)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int i = iw + a * 32 + (e / 4) * 8 + (e & 3);
+        float z = acc[a][b][e];
+        if constexpr (T::SPLIT) z *= rs;
+        if (c.bias) z += i < c.classes ? (c.bias_f32 ? ((const float *)c.bias)[i] : (float)((const bf16 *)c.bias)[i]) : 0.f;
+        if (i >= c.classes) z = -INFINITY;
+        acc[a][b][e] = z;
+        m = fmaxf(m, z);
+      }
+    m = fmaxf(m, __shfl_xor(m, 32));
+    const float ms = m == -INFINITY ? 0.f : m;
+    float s = 0.f;
+#pragma unroll
+    for (int a = 0; a < T::TI; ++a)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float p = __expf(acc[a][b][e] - ms);
+        s += p;
+        acc[a][b][e] = p;
+      }
+    s += __shfl_xor(s, 32);
+    if (j >= live) continue;
+    if (lane < 32) c.stats[(long long)j * c.pieces + (ti * T::BI + wi * WI) / WI] = make_float2(m, s);
+    if constexpr (TRAIN) {
+      char *row = c.g + j * c.ldg;
+#pragma unroll
+      for (int a = 0; a < T::TI; ++a)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int i = iw + a * 32 + q * 8;
+          if (i >= vpad) continue;
+          if constexpr (T::SPLIT) {
+            *reinterpret_cast<float4 *>(row + i * 4) = make_float4(acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]);
+          } else {
+            bf16 t[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[e] = (bf16)acc[a][b][4 * q + e];
+            *reinterpret_cast<uint2 *>(row + i * 2) = *reinterpret_cast<uint2 *>(t);
+          }
+        }
+    }
+  }
+}
+
+__device__ __forceinline__ double block_sum(double v, double *lds) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return lds[0] + lds[1] + lds[2] + lds[3];
+}
+
+// one live row: log-sum-exp, loss, and (TRAIN) the exponentials become g.  `wcols`: classes of a (max, sum) pair
+template <bool F32, bool TRAIN>
+__global__ __launch_bounds__(256) void ce_grad_kernel(Ce c, int row0, int wcols) {
+  __shared__ double lds[4];
+  __shared__ float ldm[4];
+  const int j = blockIdx.x;
+  if (j >= min(c.head[0] - row0, c.cap)) return;
+  const int r = c.index[row0 + j];
+  const float2 *st = c.stats + (long long)j * c.pieces;
+  float m = -INFINITY;
+  bool nan = false;
+  for (int k = threadIdx.x; k < c.pieces; k += 256) {
+    const float v = st[k].x;
+    nan |= v != v || st[k].y != st[k].y;                     // fmaxf drops a NaN
+    m = fmaxf(m, v);
+  }
+  m = block_max(m, ldm);
+  nan = __syncthreads_or(nan);
+  const float ms = m == -INFINITY ? 0.f : m;
+  double s = 0;
+  for (int k = threadIdx.x; k < c.pieces; k += 256) s += (double)st[k].y * (double)expf(st[k].x - ms);
+  s = block_sum(s, lds);
+  const long long label = c.labels[r];
+  const bool known = label >= 0 && label < c.classes;        // else: the loss and this row's gradient are NaN
+  double dot = 0;
+  if (known)
+    for (int k = threadIdx.x; k < c.hidden; k += 256)
+      dot += (double)elem<F32>(c.x, r * c.x_stride + k) * (double)elem<F32>(c.w, label * c.w_stride + k);
+  dot = block_sum(dot, lds);
+  if (known && c.bias) dot += c.bias_f32 ? (double)((const float *)c.bias)[label] : (double)(float)((const bf16 *)c.bias)[label];
+  const double lse = known && !nan ? (double)m + log(s) : (double)NAN;
+  const float w = c.row_weight ? c.row_weight[r] : 1.f;
+  if (threadIdx.x == 0) c.row_loss[row0 + j] = (lse - dot) * (double)w;
+  if constexpr (TRAIN) {
+    const float l = (float)lse, avg = ((const float *)c.head)[1];
+    const float f = F32 ? kSG : w / avg;
+    const float at = (float)expm1(dot - lse);                // p - 1 of the label, without the cancellation
+    char *row = c.g + j * c.ldg;
+    if constexpr (F32) {
+      for (long long k = threadIdx.x * 4; k < c.ldg / 4; k += 1024) {
+        float4 p = *reinterpret_cast<const float4 *>(row + k * 4);
+        const float e = __expf(st[k / wcols].x - l) * f;
+        float v[4] = {p.x * e, p.y * e, p.z * e, p.w * e};
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (k + q == label) v[q] = at * f;
+        _Float16 hi[4], lo[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) split16(v[q], hi[q], lo[q]);
+        // 32 values a group, 8 lanes of one wave: all of its loads have returned before any of its stores leaves
+        char *d = row + (k >> 5) * 128 + (k & 31) * 2;
+        *reinterpret_cast<uint2 *>(d) = *reinterpret_cast<uint2 *>(hi);
+        *reinterpret_cast<uint2 *>(d + 64) = *reinterpret_cast<uint2 *>(lo);
+      }
+    } else {
+      for (long long k = threadIdx.x * 8; k < c.ldg / 2; k += 2048) {
+        bf16 t[8];
+        *reinterpret_cast<uint4 *>(t) = *reinterpret_cast<const uint4 *>(row + k * 2);
+        const float e = __expf(st[k / wcols].x - l) * f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) t[q] = (bf16)(k + q == label ? at * f : (float)t[q] * e);
+        *reinterpret_cast<uint4 *>(row + k * 2) = *reinterpret_cast<uint4 *>(t);
+      }
+    }
+  }
+}
+
+// part z of dx: live rows x hidden, summed over the z-th share of the classes
+template <class T>
+__global__ __launch_bounds__(T::THREADS, 2) void ce_dx_kernel(Ce c, int row0) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int live = min(c.head[0] - row0, c.cap);
+  if (live <= 0) return;
+  const int nti = (c.hidden + T::BI - 1) / T::BI, ntj = (live + T::BJ - 1) / T::BJ;
+  if ((int)blockIdx.x >= nti * ntj * c.z) return;
+  const int zi = blockIdx.x % c.z;
+  const int ti = blockIdx.x / c.z % nti, tj = blockIdx.x / c.z / nti;
+  const int total = (c.classes + T::KK - 1) / T::KK;
+  const int s0 = (int)((long long)total * zi / c.z), s1 = (int)((long long)total * (zi + 1) / c.z);
+  f32x16 acc[T::TI][T::TJ];
+  run<T>(lds, side_ks<T::SPLIT>(c.wp, c.ldw, c.classes, c.ldx, ti * T::BI * (T::SPLIT ? 4 : 2), s0), side_kc(c.g, c.ldg, live, c.ldg, tj * T::BJ, s0),
+         s1 - s0, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave % T::NWI, wj = wave / T::NWI;
+  const int hp = (c.hidden + 3) / 4 * 4;
+#pragma unroll
+  for (int b = 0; b < T::TJ; ++b) {
+    const int j = tj * T::BJ + (wj * T::TJ + b) * 32 + (lane & 31);
+    if (j >= live) continue;
+    float *row = c.part + ((long long)zi * c.cap + j) * hp;
+#pragma unroll
+    for (int a = 0; a < T::TI; ++a)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int i = ti * T::BI + (wi * T::TI + a) * 32 + q * 8 + (lane >> 5) * 4;
+        if (i < hp) *reinterpret_cast<float4 *>(row + i) = make_float4(acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]);
+      }
+  }
+}
+
+// dx rows of the caller: the parts of a live row added up, zeros for the others
+template <bool F32>
+__global__ __launch_bounds__(256) void ce_dx_rows_kernel(Ce c, int row0) {
+  const int live = min(c.head[0] - row0, c.cap);
+  const int hp = (c.hidden + 3) / 4 * 4;
+  const float avg = ((const float *)c.head)[1], rsw = F32 ? 1.f / scale_of(c, 2) : 1.f;
+  const int r = blockIdx.x, p = c.pos[r];
+  if (p < 0 ? row0 != 0 : (p < row0 || p >= row0 + live)) return;            // another piece's row
+  const float f = F32 ? (c.row_weight ? c.row_weight[r] : 1.f) / avg * (rsw / kSG) : 1.f;
+  for (int k = threadIdx.x * 4; k < c.hidden; k += 1024) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (p >= 0) {
+      for (int z = 0; z < c.z; ++z) {
+        const float4 t = *reinterpret_cast<const float4 *>(c.part + ((long long)z * c.cap + p - row0) * hp + k);
+        v.x += t.x; v.y += t.y; v.z += t.z; v.w += t.w;
+      }
+      if constexpr (F32) { v.x *= f; v.y *= f; v.z *= f; v.w *= f; }
+    }
+    const float o[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (k + e < c.hidden) {
+        if (F32) ((float *)c.dx)[(long long)r * c.hidden + k + e] = o[e];
+        else ((bf16 *)c.dx)[(long long)r * c.hidden + k + e] = (bf16)o[e];
+      }
+  }
+}
+
+// dW tile: classes x hidden, summed over the piece's live rows.  mode 0: store in the caller's type, 1: store to / 2: add to an fp32 accumulator
+template <class T>
+__global__ __launch_bounds__(T::THREADS, 2) void ce_dw_kernel(Ce c, int row0, int mode) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int live = max(min(c.head[0] - row0, c.cap), 0);
+  if (live == 0 && row0) return;
+  const int nti = (c.hidden + T::BI - 1) / T::BI, ntj = (c.classes + T::BJ - 1) / T::BJ;
+  int ti, tj;
+  tile_of(blockIdx.x, nti * ntj, nti, ntj, ti, tj);
+  constexpr int E = T::SPLIT ? 4 : 2;
+  f32x16 acc[T::TI][T::TJ];
+  const char *x = (T::SPLIT ? c.xwp : c.xp) + row0 * c.ldx;
+  run<T>(lds, side_ks<T::SPLIT>(x, c.ldx, live, c.ldx, ti * T::BI * E, 0), side_ks<T::SPLIT>(c.g, c.ldg, live, c.ldg, (long long)tj * T::BJ * E, 0),
+         (live + T::KK - 1) / T::KK, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave % T::NWI, wj = wave / T::NWI;
+  const float f = T::SPLIT ? 1.f / (kSG * ((const float *)c.head)[1] * scale_of(c, 3)) : 1.f;
+#pragma unroll
+  for (int b = 0; b < T::TJ; ++b) {
+    const int j = tj * T::BJ + (wj * T::TJ + b) * 32 + (lane & 31);
+    if (j >= c.classes) continue;
+#pragma unroll
+    for (int a = 0; a < T::TI; ++a)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int i = ti * T::BI + (wi * T::TI + a) * 32 + q * 8 + (lane >> 5) * 4;
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = T::SPLIT ? acc[a][b][4 * q + e] * f : acc[a][b][4 * q + e];
+        const long long at = (long long)j * c.hidden + i;
+        const bool whole = i + 4 <= c.hidden && (c.hidden & 3) == 0;
+        if (T::SPLIT || mode) {
+          float *d = (T::SPLIT ? (float *)c.dw : c.dwacc) + at;
+          if (whole) {
+            float4 t = make_float4(v[0], v[1], v[2], v[3]);
+            if (mode == 2) {
+              const float4 o = *reinterpret_cast<const float4 *>(d);
+              t = make_float4(o.x + t.x, o.y + t.y, o.z + t.z, o.w + t.w);
+            }
+            *reinterpret_cast<float4 *>(d) = t;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (i + e < c.hidden) d[e] = mode == 2 ? d[e] + v[e] : v[e];
+          }
+        } else {
+          bf16 *d = (bf16 *)c.dw + at;
+          bf16 t[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) t[e] = (bf16)v[e];
+          if (whole) *reinterpret_cast<uint2 *>(d) = *reinterpret_cast<uint2 *>(t);
+          else
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (i + e < c.hidden) d[e] = t[e];
+        }
+      }
+  }
+}
+
+__global__ __launch_bounds__(256) void ce_dw_round_kernel(const float *__restrict__ acc, bf16 *__restrict__ dw, long long n) {
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) dw[i] = (bf16)acc[i];
+}
+
+// db: column sums of g, a workgroup adds kDbRows rows of 512 columns; the parts are added in order afterwards
+constexpr int kDbRows = 256;
+template <bool F32>
+__global__ __launch_bounds__(256) void ce_db_kernel(Ce c, int row0) {
+  const int live = min(c.head[0] - row0, c.cap);
+  const int slice = blockIdx.y, j0 = slice * kDbRows, j1 = min(j0 + kDbRows, live);
+  const int i = (blockIdx.x * 256 + threadIdx.x) * 2;
+  if (i >= c.classes) return;
+  float s0 = 0.f, s1 = 0.f;
+  const float f = F32 ? 1.f / (kSG * ((const float *)c.head)[1]) : 1.f;
+  for (int j = j0; j < j1; ++j) {
+    const char *row = c.g + j * c.ldg;
+    if constexpr (F32) {
+      const char *d = row + (i >> 5) * 128 + (i & 31) * 2;
+      const _Float16 *h = (const _Float16 *)d, *l = (const _Float16 *)(d + 64);
+      const int r = c.index[row0 + j];
+      const float w = c.row_weight ? c.row_weight[r] : 1.f;
+      s0 += ((float)h[0] + (float)l[0]) * w;
+      s1 += ((float)h[1] + (float)l[1]) * w;
+    } else {
+      const bf16 *d = (const bf16 *)row + i;
+      s0 += (float)d[0];
+      s1 += (float)d[1];
+    }
+  }
+  float *o = c.dbpart + (long long)(row0 / kDbRows + slice) * c.classes + i;
+  o[0] = s0 * f;
+  if (i + 1 < c.classes) o[1] = s1 * f;
+}
+__global__ __launch_bounds__(256) void ce_db_sum_kernel(Ce c, int slices) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= c.classes) return;
+  double s = 0;
+  for (int k = 0; k < slices; ++k) s += (double)c.dbpart[(long long)k * c.classes + i];
+  if (c.db_f32) ((float *)c.db)[i] = (float)s;
+  else ((bf16 *)c.db)[i] = (bf16)(float)s;
+}
+
+__global__ __launch_bounds__(256) void ce_loss_kernel(Ce c) {
+  __shared__ double lds[4];
+  double s = 0;
+  const int live = c.head[0];
+  for (int j = threadIdx.x; j < live; j += 256) s += c.row_loss[j];
+  s = block_sum(s, lds);
+  if (threadIdx.x == 0) c.loss[0] = (float)(s / (double)((const float *)c.head)[1]);
+}
+
+// grad *= *factor, unless the factor is 1 (the usual root of a backward pass): then nothing is read or written
+__global__ __launch_bounds__(256) void ce_scale_kernel(char *p, long long n, int f32, const float *__restrict__ factor) {
+  const float f = *factor;
+  if (f == 1.f) return;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    if (f32) ((float *)p)[i] *= f;
+    else ((bf16 *)p)[i] = (bf16)((float)((bf16 *)p)[i] * f);
+  }
+}
+
+// Tiles.  256 x 256 (8 waves of 128 x 64, one workgroup a CU) has the fewest LDS bytes per product; it needs enough tiles to fill 256 CUs.
+// 128 x 128 (4 waves of 64 x 64, two workgroups a CU) below that.
+template <bool IKS, bool JKS, bool SPLIT> struct Tiles {
+  typedef Tile<256, 256, 2, 4, IKS, JKS, SPLIT> Large;
+  typedef Tile<128, 128, 2, 2, IKS, JKS, SPLIT> Small;
+};
+bool large_tiles(long long i, long long j, long long z) { return ((i + 255) / 256) * ((j + 255) / 256) * z >= 192; }
+
+long long up(long long v, long long a) { return (v + a - 1) / a * a; }
+
+struct Layout {
+  size_t bytes, head, index, pos, xmax, xp, xwp, wp, g, stats, part, row_loss, dwacc, dbpart;
+  long long ldx, ldw, ldg;
+  int cap, chunks, pieces, z, wcols, db_slices;
+  bool pack_w, big_logits;
+};
+
+size_t take(size_t &at, size_t bytes) {
+  const size_t here = at;
+  at = mr3d_align_up(at + bytes, 1024);
+  return here;
+}
+
+int layout_of(const mr3d_linear_ce *a, Layout &l) {
+  if (!a || a->rows <= 0 || a->hidden <= 0 || a->classes <= 0) return MR3D_ERR_INVALID_ARG;
+  if (a->dtype != MR3D_DTYPE_F32 && a->dtype != MR3D_DTYPE_BF16) return MR3D_ERR_UNSUPPORTED;
+  if (a->param_dtype != MR3D_DTYPE_F32 && a->param_dtype != a->dtype) return MR3D_ERR_UNSUPPORTED;
+  if (a->rows > (1 << 22) || a->hidden > (1 << 16) || a->classes > (1 << 20)) return MR3D_ERR_UNSUPPORTED;
+  if (a->x_stride < a->hidden || a->weight_stride < a->hidden) return MR3D_ERR_INVALID_ARG;
+  const bool f32 = a->dtype == MR3D_DTYPE_F32, train = a->want_dx || a->want_dweight || a->want_dbias;
+  l = Layout{};
+  size_t at = 0;
+  l.ldx = up(a->hidden, f32 ? 32 : 64) * (f32 ? 4 : 2);
+  l.ldg = up(a->classes, f32 ? 32 : 64) * (f32 ? 4 : 2);
+  // bf16 weights are read where they are when a row is whole 128-byte k-steps on 16-byte boundaries
+  l.pack_w = f32 || a->hidden % 64 || a->weight_stride % 8 || ((uintptr_t)a->weight & 15);
+  l.ldw = l.pack_w ? l.ldx : a->weight_stride * 2;
+  l.chunks = 1;
+  long long cap = a->rows;
+  if (train && cap * l.ldg > kPiece) {
+    cap = kPiece / l.ldg / 256 * 256;
+    if (cap < 256) cap = 256;
+    l.chunks = (int)((a->rows + cap - 1) / cap);
+  }
+  l.cap = (int)cap;
+  l.big_logits = large_tiles(a->classes, cap, 1);
+  l.wcols = l.big_logits ? 128 : 64;
+  l.pieces = (int)(up(a->classes, l.big_logits ? 256 : 128) / l.wcols);
+  l.head = take(at, 64);
+  l.index = take(at, (size_t)a->rows * 4);
+  l.pos = take(at, (size_t)a->rows * 4);
+  l.row_loss = take(at, (size_t)a->rows * 8);
+  l.xmax = take(at, (size_t)a->rows * 4);
+  l.xp = take(at, (size_t)(a->rows * l.ldx));
+  if (f32 && a->want_dweight) l.xwp = take(at, (size_t)(a->rows * l.ldx));
+  if (l.pack_w) l.wp = take(at, (size_t)(a->classes * l.ldx));
+  l.stats = take(at, (size_t)cap * l.pieces * 8);
+  if (train) l.g = take(at, (size_t)(cap * l.ldg));
+  if (a->want_dx) {
+    // parts over the classes until two workgroups a CU have work; a part keeps 16 k-steps
+    const long long tiles = ((a->hidden + 127) / 128) * ((cap + 127) / 128), steps = l.ldg / 128;
+    long long z = tiles >= 512 ? 1 : 512 / tiles;
+    if (large_tiles(a->hidden, cap, 1)) z = 1;
+    if (z > steps / 16) z = steps / 16;
+    l.z = (int)(z < 1 ? 1 : z);
+    l.part = take(at, (size_t)l.z * cap * up(a->hidden, 4) * 4);
+  }
+  if (a->want_dweight && !f32 && l.chunks > 1) l.dwacc = take(at, (size_t)a->classes * a->hidden * 4);
+  if (a->want_dbias) {
+    l.db_slices = (int)(l.chunks * ((cap + kDbRows - 1) / kDbRows));
+    l.dbpart = take(at, (size_t)l.db_slices * a->classes * 4);
+  }
+  l.bytes = at;
+  return MR3D_OK;
+}
+
+template <class K> int allow_lds(K kernel, int bytes) {
+  return hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess ? MR3D_OK : MR3D_ERR_LAUNCH;
+}
+
+template <class T, bool TRAIN> int launch_logits(const Ce &c, int row0, hipStream_t q) {
+  if (T::LDS_BYTES > 65536)
+    if (const int e = allow_lds(ce_logits_kernel<T, TRAIN>, T::LDS_BYTES)) return e;
+  const long long n = (long long)((c.classes + T::BI - 1) / T::BI) * ((c.cap + T::BJ - 1) / T::BJ);
+  ce_logits_kernel<T, TRAIN><<<(unsigned)n, T::THREADS, T::LDS_BYTES, q>>>(c, row0);
+  return MR3D_OK;
+}
+template <class T> int launch_dx(const Ce &c, int row0, hipStream_t q) {
+  if (T::LDS_BYTES > 65536)
+    if (const int e = allow_lds(ce_dx_kernel<T>, T::LDS_BYTES)) return e;
+  const long long n = (long long)((c.hidden + T::BI - 1) / T::BI) * ((c.cap + T::BJ - 1) / T::BJ) * c.z;
+  ce_dx_kernel<T><<<(unsigned)n, T::THREADS, T::LDS_BYTES, q>>>(c, row0);
+  return MR3D_OK;
+}
+template <class T> int launch_dw(const Ce &c, int row0, int mode, hipStream_t q) {
+  if (T::LDS_BYTES > 65536)
+    if (const int e = allow_lds(ce_dw_kernel<T>, T::LDS_BYTES)) return e;
+  const long long n = (long long)((c.hidden + T::BI - 1) / T::BI) * ((c.classes + T::BJ - 1) / T::BJ);
+  ce_dw_kernel<T><<<(unsigned)n, T::THREADS, T::LDS_BYTES, q>>>(c, row0, mode);
+  return MR3D_OK;
+}
+
+template <bool F32> int run_ce(const mr3d_linear_ce *a, const Layout &l, Ce &c, hipStream_t q) {
+  const bool train = a->want_dx || a->want_dweight || a->want_dbias;
+  typedef Tiles<false, false, F32> TL;
+  typedef Tiles<true, false, F32> TX;
+  typedef Tiles<true, true, F32> TW;
+  ce_rows_kernel<<<1, 1024, 0, q>>>(c);
+  if (F32) {
+    const int wb = a->classes < 1024 ? a->classes : 1024;
+    ce_max_kernel<<<a->rows + wb, 256, 0, q>>>(c, wb);
+  }
+  ce_pack_kernel<F32><<<a->rows + (l.pack_w ? a->classes : 0), 256, 0, q>>>(c, a->want_dweight);
+  for (int k = 0; k < l.chunks; ++k) {
+    const int row0 = k * l.cap;
+    int e = MR3D_OK;
+    if (train) {
+      e = l.big_logits ? launch_logits<typename TL::Large, true>(c, row0, q) : launch_logits<typename TL::Small, true>(c, row0, q);
+      ce_grad_kernel<F32, true><<<l.cap, 256, 0, q>>>(c, row0, l.wcols);
+    } else {
+      e = l.big_logits ? launch_logits<typename TL::Large, false>(c, row0, q) : launch_logits<typename TL::Small, false>(c, row0, q);
+      ce_grad_kernel<F32, false><<<l.cap, 256, 0, q>>>(c, row0, l.wcols);
+    }
+    if (e) return e;
+    if (a->want_dx) {
+      e = large_tiles(a->hidden, l.cap, l.z) && l.z == 1 ? launch_dx<typename TX::Large>(c, row0, q) : launch_dx<typename TX::Small>(c, row0, q);
+      if (e) return e;
+      ce_dx_rows_kernel<F32><<<a->rows, 256, 0, q>>>(c, row0);
+    }
+    if (a->want_dweight) {
+      const int mode = k ? 2 : (l.chunks > 1 ? 1 : 0);
+      e = large_tiles(a->hidden, a->classes, 1) ? launch_dw<typename TW::Large>(c, row0, mode, q) : launch_dw<typename TW::Small>(c, row0, mode, q);
+      if (e) return e;
+    }
+    if (a->want_dbias) ce_db_kernel<F32><<<dim3((a->classes + 511) / 512, (l.cap + kDbRows - 1) / kDbRows), 256, 0, q>>>(c, row0);
+  }
+  if (a->want_dweight && l.dwacc) ce_dw_round_kernel<<<2048, 256, 0, q>>>(c.dwacc, (bf16 *)c.dw, (long long)a->classes * a->hidden);
+  if (a->want_dbias) ce_db_sum_kernel<<<(a->classes + 255) / 256, 256, 0, q>>>(c, l.db_slices);
+  ce_loss_kernel<<<1, 256, 0, q>>>(c);
+  return mr3d_launch_status();
+}
+
+}  // namespace
+
+extern "C" size_t mr3d_linear_cross_entropy_workspace_bytes(const mr3d_linear_ce *args_host) {
+  Layout l;
+  return layout_of(args_host, l) == MR3D_OK ? l.bytes : 0;
+}
+
+extern "C" int mr3d_linear_cross_entropy(const mr3d_linear_ce *a, void *workspace, size_t workspace_bytes, mr3d_stream_t s) {
+  Layout l;
+  if (const int e = layout_of(a, l)) return e;
+  if (!a->x || !a->weight || !a->labels || !a->loss) return MR3D_ERR_INVALID_ARG;
+  if ((a->want_dx && !a->dx) || (a->want_dweight && !a->dweight) || (a->want_dbias && (!a->dbias || !a->bias))) return MR3D_ERR_INVALID_ARG;
+  if (!(a->avg_factor >= 0.f)) return MR3D_ERR_INVALID_ARG;
+  if (!workspace || ((uintptr_t)workspace & 1023) || workspace_bytes < l.bytes) return MR3D_ERR_WORKSPACE;
+  char *b = (char *)workspace;
+  Ce c{};
+  c.x = (const char *)a->x; c.w = (const char *)a->weight; c.bias = (const char *)a->bias;
+  c.labels = a->labels; c.row_weight = a->row_weight; c.avg_dev = a->avg_factor_dev; c.valid_rows = a->valid_rows_dev;
+  c.avg_host = a->avg_factor;
+  c.x_stride = a->x_stride; c.w_stride = a->weight_stride; c.ignore = a->ignore_index;
+  c.rows = a->rows; c.hidden = a->hidden; c.classes = a->classes;
+  c.bias_f32 = c.db_f32 = a->param_dtype == MR3D_DTYPE_F32;
+  c.head = (int *)(b + l.head); c.index = (int *)(b + l.index); c.pos = (int *)(b + l.pos);
+  c.xmax = (float *)(b + l.xmax);
+  c.xp = b + l.xp; c.xwp = b + l.xwp;
+  c.wp = l.pack_w ? b + l.wp : (char *)const_cast<void *>(a->weight);
+  c.ldx = l.ldx; c.ldw = l.ldw; c.ldg = l.ldg;
+  c.g = b + l.g; c.stats = (float2 *)(b + l.stats); c.part = (float *)(b + l.part);
+  c.row_loss = (double *)(b + l.row_loss);
+  c.dwacc = (float *)(b + l.dwacc); c.dbpart = (float *)(b + l.dbpart);
+  c.cap = l.cap; c.pieces = l.pieces; c.z = l.z;
+  c.dx = (char *)a->dx; c.dw = (char *)a->dweight; c.db = (char *)a->dbias; c.loss = a->loss;
+  return a->dtype == MR3D_DTYPE_F32 ? run_ce<true>(a, l, c, mr3d_stream(s)) : run_ce<false>(a, l, c, mr3d_stream(s));
+}
+
+extern "C" int mr3d_scale_by(void *data, long long count, int dtype, const float *factor_dev, mr3d_stream_t s) {
+  if (!data || count < 0 || !factor_dev) return MR3D_ERR_INVALID_ARG;
+  if (dtype != MR3D_DTYPE_F32 && dtype != MR3D_DTYPE_BF16) return MR3D_ERR_UNSUPPORTED;
+  if (!count) return MR3D_OK;
+  const long long blocks = (count + 2047) / 2048;
+  ce_scale_kernel<<<(unsigned)(blocks > 2048 ? 2048 : blocks), 256, 0, mr3d_stream(s)>>>((char *)data, count, dtype == MR3D_DTYPE_F32, factor_dev);
+  return mr3d_launch_status();
+}

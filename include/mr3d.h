@@ -529,6 +529,35 @@ int mr3d_layer_norm_backward(const void *x, long long x_stride, const void *dy, 
                              int param_dtype, void *workspace, size_t workspace_bytes, mr3d_stream_t s);
 
 /* ------------------------------------------------------------------------------------------------
+ * Softmax cross entropy of a linear classifier, loss and gradients in one call, without the [rows][classes] logits (csrc/linear_ce.hip): what
+ * mr3d_linear_forward + mr3d_weighted_softmax_ce + mr3d_linear_dgrad / _wgrad compute, for large label sets.
+ *   z = x weight^T + bias;  loss = sum_i row_weight_i (lse(z_i) - z_i[label_i]) / avg;  dx, dweight, dbias: its gradients
+ * x [rows][hidden] and weight [classes][hidden] with x_stride / weight_stride elements between rows (>= hidden), dx and dweight packed, all of
+ * dtype MR3D_DTYPE_F32 or _BF16; bias / dbias [classes] of param_dtype (MR3D_DTYPE_F32 or dtype).  row_weight (fp32), bias, valid_rows_dev may be
+ * NULL.  A row counts when its weight is not 0, its label is not ignore_index and it lies before *valid_rows_dev; the others take no part whatever
+ * they hold and get zeros in dx.  avg: *avg_factor_dev, else avg_factor when it is > 0, else max(number of counted rows with a positive weight, 1).
+ * A counted row whose label is outside [0, classes) makes the loss, its dx row and dweight NaN.  want_*: which gradients are written.
+ * fp32 products carry 22 bits of each factor, bf16 gradients of the logits are rounded to bf16 once more; sums are fp32 or wider, in a
+ * fixed order.  hidden <= 65536, classes <= 2^20, rows <= 2^22.  workspace: 1024-byte aligned device memory of
+ * mr3d_linear_cross_entropy_workspace_bytes (0 = refused; the exponentials in it are bounded by 2 GiB, rows go through in pieces).
+ * mr3d_scale_by: data *= *factor_dev in place; nothing is touched when the factor is 1.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct {
+  const void *x, *weight, *bias;
+  const long long *labels;
+  const float *row_weight, *avg_factor_dev;
+  const int *valid_rows_dev;
+  float *loss;
+  void *dx, *dweight, *dbias;
+  long long x_stride, weight_stride, ignore_index;
+  float avg_factor;
+  int rows, hidden, classes, dtype, param_dtype, want_dx, want_dweight, want_dbias;
+} mr3d_linear_ce;
+size_t mr3d_linear_cross_entropy_workspace_bytes(const mr3d_linear_ce *args_host);
+int mr3d_linear_cross_entropy(const mr3d_linear_ce *args_host, void *workspace, size_t workspace_bytes, mr3d_stream_t s);
+int mr3d_scale_by(void *data, long long count, int dtype, const float *factor_dev, mr3d_stream_t s);
+
+/* ------------------------------------------------------------------------------------------------
  * Orthogonalised updates of a list of matrices by Newton-Schulz products (csrc/ortho.hip); not part of the reference, whose optimiser is SGD.
  *   X = G / (|G|_F + eps), transposed when rows > cols;   steps times:  A = X X^T,  X = a X + (b A + c A A) X;   out = X (transposed back)
  * in: element (r, c) at in[r * in_row_stride + c * in_col_stride]; out: packed row-major [rows][cols], of the same dtype (MR3D_DTYPE_F32 / _BF16);

@@ -1,0 +1,356 @@
+"""linear_cross_entropy (csrc/linear_ce.hip) against the formulas in 64 bits.
+
+Tolerances, norm-wise per row or matrix.  u = 2^-24.
+  logits   fp32: each factor carries 22 bits (error 2^-23 of the value at most), lo * lo (2^-22 of a term) is dropped, and the K products are
+           summed in fp32 with at most K / 16 + 16 roundings (16 products an instruction): |dz| <= (2^-21 + (K / 16 + 16) u) |x| |W_c|.
+           bf16: factors are exact, |dz| <= (K / 16 + 16) u |x| |W_c|.  Adding the bias and subtracting the maximum: 2 u |z| more.  Call the row's
+           largest Z.  Exponential and sums: 2^-20 relative in all (the hardware exponential is good to a few u; sums are short).
+  loss     |d ce_i| <= 2 Z + 2^-20, and the weighted mean over rows; stored in fp32.
+  g        relative to softmax: E = 2 Z + 2^-19; the label's entry is computed apart, absolute error E.  fp32: two planes of 14 + 22 bits
+           (2^-21 of the value and 2^-38 absolute); bf16: 2^-8 for the stored exponential and 2^-8 for g.
+           So |dg_i| <= (E + r) |g_i| + E p_label w with r = 2^-20 (fp32), 2^-7 (bf16), taken entry by entry below.
+  dx, dW   the error of g through |W| and |x|, entry by entry, plus (2^-20 + (n / 16 + 20) u) sum |g| |W| for the product (n its length), plus
+           half a step of the stored type."""
+import pytest
+import torch
+
+U = 2.0 ** -24
+
+
+def _reference(x, w, b, label, rw, ignore=-100, valid=None, avg=None):
+    f32 = x.dtype == torch.float32
+    x, w = x.double(), w.double()
+    n, k = x.shape
+    v = w.shape[0]
+    live = label != ignore
+    rw = torch.ones(n, dtype=torch.float64) if rw is None else rw.double()
+    if valid is not None:
+        live = live & (torch.arange(n) < valid)
+    live = live & (rw != 0)
+    if avg is None:
+        avg = max(int((live & (rw > 0)).sum()), 1)
+    rows = live.nonzero().squeeze(1)
+    xl, rl, ll = x[rows], rw[rows], label[rows]
+    z = xl @ w.t() + (0 if b is None else b.double())
+    lse = torch.logsumexp(z, 1)
+    at = torch.arange(len(rows))
+    ce = lse - z[at, ll]
+    p = torch.exp(z - lse[:, None])
+    g = p.clone()
+    g[at, ll] -= 1
+    s = (rl / avg)[:, None]
+    zerr = ((2.0 ** -21 if f32 else 0) + (k / 16 + 16) * U) * xl.norm(dim=1, keepdim=True) * w.norm(dim=1).max() + 2 * U * z.abs().amax(1, keepdim=True)
+    e = 2 * zerr + 2.0 ** -19
+    eg = (e + (2.0 ** -20 if f32 else 2.0 ** -7)) * g.abs() + (2.0 ** -36 if f32 else 0)
+    eg[at, ll] += e.squeeze(1) * torch.ones(len(rows))
+    g, eg = g * s, eg * s.abs()
+    prod = lambda m: (2.0 ** -20 if f32 else 0) + (m / 16 + 20) * U
+    dx, ex = torch.zeros_like(x), torch.zeros_like(x)
+    dx[rows] = g @ w
+    ex[rows] = eg @ w.abs() + prod(v) * (g.abs() @ w.abs())
+    out = dict(loss=((ce * rl).sum() / avg).reshape(1), dx=dx, dw=g.t() @ xl, db=g.sum(0))
+    bound = dict(loss=((2 * zerr.squeeze(1) + 2.0 ** -20 + 4 * U * ce) * rl.abs()).sum().reshape(1) / abs(avg) + 2 * U * out['loss'].abs(), dx=ex,
+                 dw=eg.t() @ xl.abs() + prod(n) * (g.abs().t() @ xl.abs()), db=eg.sum(0) + 300 * U * g.abs().sum(0))
+    return out, bound
+
+
+def _check(got, ref, bound, what):
+    assert torch.isfinite(got).all(), what
+    half = 0.0 if got.dtype == torch.float32 else torch.finfo(got.dtype).eps / 2
+    tol = bound * (1 + half) + (half + 2 * U) * ref.abs() + 1e-30
+    over = float(((got.detach().double().cpu() - ref).abs() / tol).max()) if ref.numel() else 0.0
+    assert over <= 1, f'{what}: {over:.3g} times the bound'
+
+
+def _inputs(n, k, v, dtype, seed=0, bias=True, dead=0.3, scale=2.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(n, k, generator=g).to(dtype)
+    w = (torch.randn(v, k, generator=g) * scale / k ** 0.5).to(dtype)
+    b = (0.5 * torch.randn(v, generator=g)).to(dtype) if bias else None
+    label = torch.randint(0, v, (n,), generator=g)
+    label[torch.rand(n, generator=g) < dead] = -100
+    rw = 0.25 + torch.rand(n, generator=g)
+    return x, w, b, label, rw
+
+
+def _run(x, w, b, label, rw, scale=None, **kw):
+    from mr3d_amd.core import linear_cross_entropy
+    leaves = [None if t is None else t.detach().cuda().requires_grad_(True) for t in (x, w, b)]
+    loss = linear_cross_entropy(leaves[0], leaves[1], label.cuda(), None if rw is None else rw.cuda(), bias=leaves[2], **kw)
+    g = torch.autograd.grad(loss if scale is None else loss * scale, [t for t in leaves if t is not None])
+    return dict(zip(('loss', 'dx', 'dw', 'db'), (loss.detach(),) + g))
+
+
+def _compare(x, w, b, label, rw, what, ref_kw={}, **kw):
+    ref, bound = _reference(x, w, b, label, rw, **ref_kw)
+    got = _run(x, w, b, label, rw, **kw)
+    for name, t in got.items():
+        _check(t, ref[name], bound[name], (name,) + what)
+    return got
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('n,k,v', [(1, 1, 1), (1, 1, 2), (2, 3, 5), (1, 64, 1000), (5, 64, 64), (64, 31, 127), (63, 33, 129), (130, 65, 257), (33, 128, 128),
+                                   (300, 100, 500), (257, 515, 1204), (1000, 64, 300), (100, 1024, 2000), (700, 200, 8001)])
+def test_loss_and_gradients(n, k, v, dtype):
+    x, w, b, label, rw = _inputs(n, k, v, dtype, seed=n + k + v)
+    label[0] = v - 1
+    _compare(x, w, b, label, rw, (n, k, v, dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_large_tiles(dtype):
+    """enough rows, classes and features for the 256 x 256 tiles of all three products"""
+    x, w, b, label, rw = _inputs(3500, 3700, 3600, dtype, seed=4)
+    _compare(x, w, b, label, rw, (dtype,))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_forward_alone_and_single_gradients(dtype):
+    from mr3d_amd.core import linear_cross_entropy
+    x, w, b, label, rw = _inputs(90, 96, 700, dtype)
+    ref, bound = _reference(x, w, b, label, rw)
+    full = _run(x, w, b, label, rw)
+    t = [a.cuda() for a in (x, w, b, label, rw)]
+    with torch.no_grad():
+        _check(linear_cross_entropy(t[0], t[1], t[3], t[4], bias=t[2]), ref['loss'], bound['loss'], ('loss',))
+    for i, name in ((0, 'dx'), (1, 'dw'), (2, 'db')):
+        leaves = [a.clone().requires_grad_(q == i) for q, a in enumerate(t[:3])]
+        (g,) = torch.autograd.grad(linear_cross_entropy(leaves[0], leaves[1], t[3], t[4], bias=leaves[2]), [leaves[i]])
+        assert torch.equal(g, full[name]), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_rows_in_pieces(dtype, monkeypatch):
+    """more exponentials than fit one piece: 2 GiB is 1100 rows of 2^20 - 13 bf16 classes, half of that in fp32"""
+    v = (1 << 20) - 13
+    x, w, _, label, rw = _inputs(1100, 8, v, dtype, seed=2, bias=False, dead=0.0, scale=1.0)
+    label[:20] = -100
+    got = _run(x, w, None, label, rw)
+    half = 600                                               # the rows of the first piece alone, and the others alone
+    parts = []
+    for sl in (slice(0, half), slice(half, None)):
+        lab = torch.full_like(label, -100)
+        lab[sl] = label[sl]
+        parts.append(_run(x, w, None, lab, rw, avg_factor=1080.0))
+    tol = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -22
+    s = parts[0]['dw'].double() + parts[1]['dw'].double()
+    assert float((got['dw'].double() - s).norm()) <= 3 * tol * float(s.norm())
+    assert torch.equal(got['dx'][:half], parts[0]['dx'][:half]) and torch.equal(got['dx'][half:], parts[1]['dx'][half:])
+    want = float(parts[0]['loss']) + float(parts[1]['loss'])
+    assert abs(float(got['loss']) - want) <= 4 * U * abs(want)
+    assert float(got['dx'][:20].abs().max()) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_rows_that_do_not_count_may_hold_anything(dtype):
+    x, w, b, label, rw = _inputs(150, 64, 400, dtype)
+    rw[5], rw[6], label[9] = 0.0, -0.0, -7
+    valid = 140
+    label = torch.where(label == -100, torch.full_like(label, -7), label)
+    vr = torch.tensor([valid], dtype=torch.int32).cuda()
+    ref, bound = _reference(x, w, b, label, rw, ignore=-7, valid=valid)
+    x2, rw2, label2 = x.clone(), rw.clone(), label.clone()
+    dead = (label == -7) | (rw == 0) | (torch.arange(150) >= valid)
+    x2[dead.nonzero().squeeze(1)[::2]] = float('nan')
+    x2[dead.nonzero().squeeze(1)[1::2]] = float('inf')
+    rw2[valid:] = float('nan')
+    label2[valid:] = 1 << 40
+    rw2[label == -7] = float('inf')
+    got = _run(x2, w, b, label2, rw2, ignore_index=-7, valid_rows=vr)
+    for name, t in got.items():
+        _check(t, ref[name], bound[name], (name,))
+    assert float(got['dx'][dead.cuda()].abs().max()) == 0
+    # nothing counts at all
+    for kw in (dict(valid_rows=torch.zeros(1, dtype=torch.int32).cuda()), dict(ignore_index=3)):
+        lab = torch.full_like(label, 3)
+        none = _run(x2, w, b, lab, rw, **kw)
+        assert all(float(t.abs().max()) == 0 for t in none.values())
+
+
+@pytest.mark.gpu
+def test_masked_classes_and_extreme_logits():
+    """a bias of -infinity takes a class out; the type's lowest value too; logits of +-3e4 neither overflow nor lose the label's gradient"""
+    x, w, b, label, rw = _inputs(40, 32, 300, torch.float32, dead=0.0)
+    keep = torch.ones(300, dtype=torch.bool)
+    keep[::3] = False
+    label = keep.nonzero().squeeze(1)[label % 200]
+    bk = b.clone()
+    small, bound = _reference(x, w[keep], b[keep], (torch.cumsum(keep, 0) - 1)[label], rw)
+    for low in (float('-inf'), torch.finfo(torch.float32).min):
+        bk[~keep] = low
+        got = _run(x, w, bk, label, rw)
+        _check(got['loss'], small['loss'], bound['loss'], ('loss',))
+        _check(got['dx'], small['dx'], bound['dx'], ('dx',))
+        _check(got['dw'][keep.cuda()], small['dw'], bound['dw'], ('dw',))
+        assert float(got['dw'][~keep.cuda()].abs().max()) == 0 and float(got['db'][~keep.cuda()].abs().max()) == 0
+    _compare(x * 300, w * 20, b, label, rw, ('extreme',))
+    _compare(x * 2.0 ** -40, w * 2.0 ** 30, b, label, rw, ('small rows, large weights',))
+    xs = x * torch.logspace(-12, 3, 40)[:, None]
+    _compare(xs, w * torch.logspace(0, -8, 300)[:, None], b, label, rw * torch.logspace(-3, 3, 40), ('mixed scales',))
+
+
+@pytest.mark.gpu
+def test_nan_rows_and_labels_out_of_range():
+    x, w, b, label, rw = _inputs(30, 32, 200, torch.float32, dead=0.0)
+    ref, bound = _reference(x, w, b, label, rw)
+    for bad in (200, 1 << 40, -1, -(1 << 50)):
+        lab = label.clone()
+        lab[4] = bad
+        got = _run(x, w, b, lab, rw)
+        assert torch.isnan(got['loss']).all() and torch.isnan(got['dx'][4]).all() and torch.isnan(got['dw']).all()
+        rest = torch.arange(30) != 4
+        _check(got['dx'][rest.cuda()], ref['dx'][rest], bound['dx'][rest], ('dx',))
+    for value in (float('nan'), float('inf')):
+        x2 = x.clone()
+        x2[7, 3] = value
+        got = _run(x2, w, b, label, rw)
+        rest = torch.arange(30) != 7
+        assert torch.isnan(got['loss']).all() and torch.isnan(got['dx'][7]).all()
+        _check(got['dx'][rest.cuda()], ref['dx'][rest], bound['dx'][rest], ('dx',))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_strides_shapes_factors_and_incoming_gradient(dtype):
+    from mr3d_amd.core import linear_cross_entropy
+    x, w, b, label, rw = _inputs(60, 200, 150, dtype)
+    for cx, cw in ((slice(0, 128), slice(0, 128)), (slice(3, 67), slice(8, 72)), (slice(1, 50), slice(64, 113))):
+        ref, bound = _reference(x[:, cx], w[:, cw], None, label, None, avg=7.5)
+        xd, wd = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+        loss = linear_cross_entropy(xd[:, cx].reshape(3, 20, -1), wd[:, cw], label.cuda().reshape(3, 20), avg_factor=torch.tensor(7.5).cuda())
+        (loss * -3.0).sum().backward()
+        _check(loss, ref['loss'], bound['loss'], ('loss',))
+        _check(xd.grad[:, cx], -3 * ref['dx'], 3 * bound['dx'], ('dx',))
+        _check(wd.grad[:, cw], -3 * ref['dw'], 3 * bound['dw'], ('dw',))
+    # a transposed weight has no contiguous rows, a broadcast row no stride
+    wt = w.t().contiguous().cuda().t()
+    _check(linear_cross_entropy(x.cuda()[:1].expand(60, 200), wt, label.cuda(), avg_factor=2.0),
+           *[d['loss'] for d in _reference(x[:1].expand(60, 200), w, None, label, None, avg=2.0)], ('loss',))
+    # fp32 bias beside bf16
+    _compare(x, w, b.float(), label, rw, ('fp32 bias', dtype))
+    # one backward
+    xd = x.cuda().requires_grad_(True)
+    loss = linear_cross_entropy(xd, w.cuda(), label.cuda())
+    loss.backward(retain_graph=True)
+    with pytest.raises(RuntimeError, match='second backward'):
+        loss.backward()
+
+
+@pytest.mark.gpu
+def test_gradient_against_differences():
+    """central differences along random directions of unit norm.  With logits of size 2 the third derivative along such a direction of x or W
+    is below 10 |W|^3 or 10 |x|^3 (|W_c| about 2, |x_i| about 6): step 2^-6 leaves 10 * 216 * 2^-12 / 6 < 0.1 of the mean over rows
+    in the worst case and 1e-3 in a typical one; the loss itself is good to 2^-20 of 6, over the step 4e-4.  2e-3 covers both."""
+    from mr3d_amd.core import linear_cross_entropy
+    x, w, b, label, rw = _inputs(40, 36, 90, torch.float32, seed=11)
+    got = _run(x, w, b, label, rw)
+    g = torch.Generator().manual_seed(1)
+    f = lambda p: float(linear_cross_entropy(p[0].cuda(), p[1].cuda(), label.cuda(), rw.cuda(), bias=p[2].cuda()).double())
+    e = 2.0 ** -6
+    for i, name in enumerate(('dx', 'dw', 'db')):
+        p = [x, w, b]
+        d = torch.randn(p[i].shape, generator=g)
+        d = d / d.norm()
+        hi, lo = list(p), list(p)
+        hi[i], lo[i] = p[i] + e * d, p[i] - e * d
+        assert abs((f(hi) - f(lo)) / (2 * e) - float((got[name].double().cpu() * d.double()).sum())) <= 2e-3, name
+
+
+@pytest.mark.gpu
+def test_same_bits_every_run_on_another_stream_and_in_a_graph():
+    from mr3d_amd import _hip
+    for dtype in (torch.float32, torch.bfloat16):
+        x, w, b, label, rw = (t.cuda() for t in _inputs(300, 256, 900, dtype))
+        both = lambda: _hip.linear_cross_entropy(x, w, b, label, rw, None, None, -100, True, True, True)
+        first = both()
+        assert all(torch.equal(p, q) for p, q in zip(first, both()))
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = both()
+        torch.cuda.current_stream().wait_stream(side)
+        assert all(torch.equal(p, q) for p, q in zip(first, other))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = both()
+        for k in range(3):
+            g = torch.Generator().manual_seed(k)
+            x.copy_(torch.randn(x.shape, generator=g).to(dtype))
+            label.copy_(torch.randint(0, 900, (300,), generator=g))
+            label[torch.rand(300, generator=g).cuda() < 0.2 * k] = -100
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(held, both())), k
+
+
+@pytest.mark.gpu
+def test_agrees_with_the_layer_and_the_loss_it_joins():
+    """layers.linear + weighted_cross_entropy on the same inputs: both are within their bounds of the 64-bit value"""
+    from mr3d_amd.core import weighted_cross_entropy
+    from mr3d_amd.detector import layers
+    x, w, b, label, rw = _inputs(128, 256, 81, torch.float32, dead=0.0)
+    rw[::5] = 0
+    ref, bound = _reference(x, w, b, label, rw)
+    got = _run(x, w, b, label, rw)
+    leaves = [t.cuda().requires_grad_(True) for t in (x, w, b)]
+    loss = weighted_cross_entropy(layers.linear(*leaves), label.cuda(), rw.cuda())
+    loss.sum().backward()
+    assert abs(float(loss) - float(got['loss'])) <= 2 * float(bound['loss']) + 2e-5 * float(loss)
+    for name, t in zip(('dx', 'dw', 'db'), leaves):
+        _check(got[name], ref[name], bound[name], (name,))
+        assert float((t.grad - got[name]).norm()) <= 1e-4 * float(got[name].norm()), name
+
+
+@pytest.mark.gpu
+def test_no_rows():
+    from mr3d_amd.core import linear_cross_entropy
+    x = torch.zeros(0, 16, device='cuda', requires_grad=True)
+    w = torch.ones(10, 16, device='cuda', requires_grad=True)
+    loss = linear_cross_entropy(x, w, torch.zeros(0, dtype=torch.int64, device='cuda'))
+    loss.backward()
+    assert float(loss) == 0 and x.grad.shape == (0, 16) and float(w.grad.abs().max()) == 0
+
+
+def test_refusals_need_no_gpu():
+    import ctypes
+    import mr3d_amd
+    from mr3d_amd import _hip
+    from mr3d_amd.core import linear_cross_entropy as ce
+    x, w, lab = torch.zeros(4, 8), torch.zeros(10, 8), torch.zeros(4, dtype=torch.int64)
+    with pytest.raises(NotImplementedError):
+        ce(x, w, lab)
+    for args, kw in (((x, torch.zeros(10, 7), lab), {}), ((x, w, lab[:3]), {}), ((x, w, lab.int()), {}), ((x, w, lab, torch.ones(5)), {}),
+                     ((x, w, lab), dict(bias=torch.zeros(9))), ((x, w, lab), dict(bias=torch.zeros(10).half())), ((x, w, lab), dict(avg_factor=0.0)),
+                     ((x, w, lab), dict(avg_factor=float('nan'))), ((x, w, lab), dict(avg_factor=torch.ones(2))),
+                     ((x, w, lab), dict(valid_rows=torch.zeros(1, dtype=torch.int64)))):
+        with pytest.raises(ValueError):
+            ce(*args, **kw)
+    for a, b in ((x.half(), w.half()), (x, w.bfloat16()), (x.bfloat16(), w)):
+        with pytest.raises(TypeError):
+            ce(a, b, lab)
+    with pytest.raises(NotImplementedError):
+        ce(x, torch.zeros(1, 8).expand((1 << 20) + 1, 8), lab)
+    with pytest.raises(NotImplementedError):
+        ce(x, w, lab, torch.ones(4, requires_grad=True))
+    L = mr3d_amd._hip.lib()
+    base = dict(x=1024, weight=1024, bias=1024, labels=1024, loss=1024, dx=1024, dweight=1024, dbias=1024, x_stride=8, weight_stride=8, ignore_index=-100,
+                rows=4, hidden=8, classes=10, dtype=0, param_dtype=0, want_dx=1, want_dweight=1, want_dbias=1)
+    mk = lambda **kw: ctypes.byref(_hip.LinearCe(**{**base, **kw}))
+    need = L.mr3d_linear_cross_entropy_workspace_bytes(mk())
+    call = lambda ws=1024, by=need, **kw: L.mr3d_linear_cross_entropy(mk(**kw), ws, by, None)
+    assert need > 0
+    for kw in (dict(x=None), dict(weight=None), dict(labels=None), dict(loss=None), dict(dx=None), dict(dweight=None), dict(dbias=None), dict(bias=None),
+               dict(rows=0), dict(hidden=0), dict(classes=0), dict(x_stride=7), dict(weight_stride=7), dict(avg_factor=-1.0), dict(avg_factor=float('nan'))):
+        assert call(**kw) == 1, kw
+    for kw in (dict(dtype=2), dict(param_dtype=1), dict(classes=(1 << 20) + 1), dict(hidden=(1 << 16) + 1, x_stride=1 << 20, weight_stride=1 << 20),
+               dict(rows=(1 << 22) + 1)):
+        assert call(**kw) == 4, kw
+    assert call(ws=None) == 2 and call(ws=1032) == 2 and call(by=need - 1) == 2
+    assert L.mr3d_scale_by(None, 4, 0, 1024, None) == 1 and L.mr3d_scale_by(1024, 4, 0, None, None) == 1 and L.mr3d_scale_by(1024, 4, 2, 1024, None) == 4
+    assert L.mr3d_scale_by(1024, 0, 0, 1024, None) == 0
