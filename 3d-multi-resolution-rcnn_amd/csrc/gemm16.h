@@ -149,11 +149,11 @@ __device__ __forceinline__ void run(char *lds, Side si, Side sj, int nsteps, f32
       for (int a = 0; a < T::TI; ++a)
 #pragma unroll
         for (int b = 0; b < T::TJ; ++b) {
-          acc[a][b] = mfma<T::SPLIT>(fi[a][0], fj[b][0], acc[a][b]);
-          if constexpr (T::SPLIT) {
+          if constexpr (T::SPLIT) {                        // small terms first: one rounding at the size of the result instead of three
             acc[a][b] = mfma<true>(fi[a][0], fj[b][1], acc[a][b]);
             acc[a][b] = mfma<true>(fi[a][1], fj[b][0], acc[a][b]);
           }
+          acc[a][b] = mfma<T::SPLIT>(fi[a][0], fj[b][0], acc[a][b]);
         }
     }
   }

@@ -6,7 +6,7 @@
 //            in any product (NaN in them stays there) and get a zero row of dx
 //   pack     live rows of x (and W, where its storage is not what the products read) into gemm16.h's operand form
 //   logits   z tile by tile; a wave holds 128 classes of a row: it leaves exp(z - max of the 128) and (max, sum).  The exponentials take the place
-//            of the logits: 2 bytes a value (bf16: relative to their own maximum they lose what g's own rounding loses anyway), 4 for fp32
+//            of the logits: for bf16 in fp16 (in [0, 1]; 2^-12 of the value, an eighth of what g's rounding to bf16 loses), else fp32
 //   grad     per row: lse from the (max, sum) pairs, the label's logit once more as a dot product, loss; exponentials -> g in place
 //   dx, dw   g W (split over the classes, parts added in a fixed order) and g^T x
 // The exponentials of at most kPiece bytes of rows exist at a time; dW accumulates over such pieces in fp32.
@@ -107,6 +107,20 @@ __device__ __forceinline__ float block_max(float v, float *lds) {
   return fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
 }
 
+// this thread's share of a row, 16 bytes a load with the alignment of a float (odd strides), eight in flight for rows of 1024 and more
+__device__ __forceinline__ float row_max(const float *p, int n) {
+  typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+  float m = 0.f;
+  int k = threadIdx.x * 4;
+#pragma unroll 4
+  for (; k + 4 <= n; k += 1024) {
+    const f4 t = *reinterpret_cast<const f4 *>(p + k);
+    m = fmaxf(fmaxf(fmaxf(m, fabsf(t[0])), fabsf(t[1])), fmaxf(fabsf(t[2]), fabsf(t[3])));
+  }
+  for (; k < n; ++k) m = fmaxf(m, fabsf(p[k]));            // the last, partial group: one thread's
+  return m;
+}
+
 // fp32: the largest |x| of each live row and |x w| of all, the largest |W| (the first `rows` workgroups take x, the rest W).  The maximum of
 // positive floats is the maximum of their bits: an integer atomic, whose order does not matter
 __global__ __launch_bounds__(256) void ce_max_kernel(Ce c, int wblocks) {
@@ -116,8 +130,7 @@ __global__ __launch_bounds__(256) void ce_max_kernel(Ce c, int wblocks) {
     if ((int)blockIdx.x >= c.head[0]) return;
     const int r = c.index[blockIdx.x];
     const float *x = (const float *)c.x + r * c.x_stride;
-    for (int k = threadIdx.x; k < c.hidden; k += 256) m = fmaxf(m, fabsf(x[k]));
-    m = block_max(m, lds);
+    m = block_max(row_max(x, c.hidden), lds);
     if (threadIdx.x == 0) {
       c.xmax[blockIdx.x] = m;
       const float w = m * fabsf(c.row_weight ? c.row_weight[r] : 1.f);
@@ -125,10 +138,7 @@ __global__ __launch_bounds__(256) void ce_max_kernel(Ce c, int wblocks) {
       else atomicMax(&c.head[3], 0x7f800000);
     }
   } else {
-    for (int v = blockIdx.x - c.rows; v < c.classes; v += wblocks) {
-      const float *w = (const float *)c.w + v * c.w_stride;
-      for (int k = threadIdx.x; k < c.hidden; k += 256) m = fmaxf(m, fabsf(w[k]));
-    }
+    for (int v = blockIdx.x - c.rows; v < c.classes; v += wblocks) m = fmaxf(m, row_max((const float *)c.w + v * c.w_stride, c.hidden));
     m = block_max(m, lds);
     if (threadIdx.x == 0) atomicMax(&c.head[2], __float_as_int(m));
   }
@@ -236,9 +246,9 @@ __global__ __launch_bounds__(T::THREADS, 2) void ce_logits_kernel(Ce c, int row0
           if constexpr (T::SPLIT) {
             *reinterpret_cast<float4 *>(row + i * 4) = make_float4(acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]);
           } else {
-            bf16 t[4];
+            _Float16 t[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) t[e] = (bf16)acc[a][b][4 * q + e];
+            for (int e = 0; e < 4; ++e) t[e] = (_Float16)acc[a][b][4 * q + e];
             *reinterpret_cast<uint2 *>(row + i * 2) = *reinterpret_cast<uint2 *>(t);
           }
         }
@@ -311,11 +321,12 @@ __global__ __launch_bounds__(256) void ce_grad_kernel(Ce c, int row0, int wcols)
       }
     } else {
       for (long long k = threadIdx.x * 8; k < c.ldg / 2; k += 2048) {
+        _Float16 p[8];
         bf16 t[8];
-        *reinterpret_cast<uint4 *>(t) = *reinterpret_cast<const uint4 *>(row + k * 2);
+        *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(row + k * 2);
         const float e = __expf(st[k / wcols].x - l) * f;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) t[q] = (bf16)(k + q == label ? at * f : (float)t[q] * e);
+        for (int q = 0; q < 8; ++q) t[q] = (bf16)(k + q == label ? at * f : (float)p[q] * e);
         *reinterpret_cast<uint4 *>(row + k * 2) = *reinterpret_cast<uint4 *>(t);
       }
     }
@@ -445,40 +456,58 @@ __global__ __launch_bounds__(256) void ce_dw_round_kernel(const float *__restric
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) dw[i] = (bf16)acc[i];
 }
 
-// db: column sums of g, a workgroup adds kDbRows rows of 512 columns; the parts are added in order afterwards
-constexpr int kDbRows = 256;
+// db: column sums of g.  A workgroup adds kDbRows rows of 256 columns: 8 columns (16 bytes, split: of each plane) a thread and 8 rows side
+// by side, which meet in LDS; the parts are added in order afterwards
+constexpr int kDbRows = 64;
 template <bool F32>
 __global__ __launch_bounds__(256) void ce_db_kernel(Ce c, int row0) {
+  __shared__ float sum[8][256];
   const int live = min(c.head[0] - row0, c.cap);
   const int slice = blockIdx.y, j0 = slice * kDbRows, j1 = min(j0 + kDbRows, live);
-  const int i = (blockIdx.x * 256 + threadIdx.x) * 2;
-  if (i >= c.classes) return;
-  float s0 = 0.f, s1 = 0.f;
-  const float f = F32 ? 1.f / (kSG * ((const float *)c.head)[1]) : 1.f;
-  for (int j = j0; j < j1; ++j) {
-    const char *row = c.g + j * c.ldg;
-    if constexpr (F32) {
-      const char *d = row + (i >> 5) * 128 + (i & 31) * 2;
-      const _Float16 *h = (const _Float16 *)d, *l = (const _Float16 *)(d + 64);
-      const int r = c.index[row0 + j];
-      const float w = c.row_weight ? c.row_weight[r] : 1.f;
-      s0 += ((float)h[0] + (float)l[0]) * w;
-      s1 += ((float)h[1] + (float)l[1]) * w;
-    } else {
-      const bf16 *d = (const bf16 *)row + i;
-      s0 += (float)d[0];
-      s1 += (float)d[1];
+  const int col = (threadIdx.x & 31) * 8, i = blockIdx.x * 256 + col, sub = threadIdx.x >> 5;
+  float s[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s[e] = 0.f;
+  if (i < c.classes) {                                       // whole groups of 8 exist: rows are padded with zeros
+#pragma unroll 4
+    for (int j = j0 + sub; j < j1; j += 8) {
+      const char *row = c.g + j * c.ldg;
+      if constexpr (F32) {
+        const char *d = row + (i >> 5) * 128 + (i & 31) * 2;
+        const f16x8 h = *reinterpret_cast<const f16x8 *>(d), l = *reinterpret_cast<const f16x8 *>(d + 64);
+        const float w = c.row_weight ? c.row_weight[c.index[row0 + j]] : 1.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] += ((float)h[e] + (float)l[e]) * w;
+      } else {
+        const bf16x8 v = *reinterpret_cast<const bf16x8 *>(row + i * 2);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] += (float)v[e];
+      }
     }
   }
-  float *o = c.dbpart + (long long)(row0 / kDbRows + slice) * c.classes + i;
-  o[0] = s0 * f;
-  if (i + 1 < c.classes) o[1] = s1 * f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sum[sub][col + e] = s[e];
+  __syncthreads();
+  const int o = blockIdx.x * 256 + threadIdx.x;
+  if (o >= c.classes) return;
+  float t = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) t += sum[k][threadIdx.x];
+  c.dbpart[(long long)(row0 / kDbRows + slice) * c.classes + o] = F32 ? t / (kSG * ((const float *)c.head)[1]) : t;
 }
+// 64 columns a workgroup, the slices four side by side
 __global__ __launch_bounds__(256) void ce_db_sum_kernel(Ce c, int slices) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= c.classes) return;
+  __shared__ double sum[4][64];
+  const int col = threadIdx.x & 63, sub = threadIdx.x >> 6, i = blockIdx.x * 64 + col;
   double s = 0;
-  for (int k = 0; k < slices; ++k) s += (double)c.dbpart[(long long)k * c.classes + i];
+  if (i < c.classes) {
+#pragma unroll 8
+    for (int k = sub; k < slices; k += 4) s += (double)c.dbpart[(long long)k * c.classes + i];
+  }
+  sum[sub][col] = s;
+  __syncthreads();
+  if (sub || i >= c.classes) return;
+  s = sum[0][col] + sum[1][col] + sum[2][col] + sum[3][col];
   if (c.db_f32) ((float *)c.db)[i] = (float)s;
   else ((bf16 *)c.db)[i] = (bf16)(float)s;
 }
@@ -636,10 +665,10 @@ template <bool F32> int run_ce(const mr3d_linear_ce *a, const Layout &l, Ce &c, 
       e = large_tiles(a->hidden, a->classes, 1) ? launch_dw<typename TW::Large>(c, row0, mode, q) : launch_dw<typename TW::Small>(c, row0, mode, q);
       if (e) return e;
     }
-    if (a->want_dbias) ce_db_kernel<F32><<<dim3((a->classes + 511) / 512, (l.cap + kDbRows - 1) / kDbRows), 256, 0, q>>>(c, row0);
+    if (a->want_dbias) ce_db_kernel<F32><<<dim3((a->classes + 255) / 256, (l.cap + kDbRows - 1) / kDbRows), 256, 0, q>>>(c, row0);
   }
   if (a->want_dweight && l.dwacc) ce_dw_round_kernel<<<2048, 256, 0, q>>>(c.dwacc, (bf16 *)c.dw, (long long)a->classes * a->hidden);
-  if (a->want_dbias) ce_db_sum_kernel<<<(a->classes + 255) / 256, 256, 0, q>>>(c, l.db_slices);
+  if (a->want_dbias) ce_db_sum_kernel<<<(a->classes + 63) / 64, 256, 0, q>>>(c, l.db_slices);
   ce_loss_kernel<<<1, 256, 0, q>>>(c);
   return mr3d_launch_status();
 }

@@ -153,46 +153,50 @@ __device__ __forceinline__ void load_planes(const char *row, int i, float (&v)[4
   for (int e = 0; e < 4; ++e) v[e] = (float)hh[e] + (float)ll[e];
 }
 
-// a symmetric result: rows j of tile tj, columns i of tile ti, and mirrored off the diagonal.  POLY: a I + b A + c acc instead of acc
+// 32 x 32 block (bi, bj) of a tile of a symmetric result: rows j of tile tj, columns i of tile ti, and mirrored off the diagonal.
+// POLY: a I + b A + c acc instead of acc
+template <bool POLY>
+__device__ __forceinline__ void store_symmetric_block(const Mat &p, char *dst, int ti, int tj, int bi, int bj, const f32x16 &acc, float ca, float cb, float cc) {
+  const int lane = threadIdx.x & 63, mp = (p.m + 31) / 32 * 32;
+  const int j = tj * kT + bj * 32 + (lane & 31);
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int i = ti * kT + bi * 32 + g * 8 + (lane >> 5) * 4;
+    float v[4];
+    if constexpr (POLY) {
+      float f[4] = {0.f, 0.f, 0.f, 0.f};
+      if (j < p.m && i < mp) load_planes(p.a + (long long)j * p.lda, i, f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float t = cc * (acc[g * 4 + e] * (1.f / (kSA * kSA))) + cb * (f[e] * (1.f / kSA));
+        v[e] = (t + (i + e == j ? ca : 0.f)) * kSB;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = acc[g * 4 + e] * (kSA / (kSX * kSX));
+    }
+    if (j < p.m && i < mp) store_planes(dst + (long long)j * p.lda, i, v);
+    if (ti != tj && j < mp) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + e < p.m) {
+          _Float16 h, l;
+          split16(v[e], h, l);
+          _Float16 *d = reinterpret_cast<_Float16 *>(dst + (long long)(i + e) * p.lda + (j >> 5) * 128) + (j & 31);
+          d[0] = h;
+          d[32] = l;
+        }
+    }
+  }
+}
+
 template <bool POLY>
 __device__ __forceinline__ void store_symmetric(const Mat &p, char *dst, int ti, int tj, const f32x16 (&acc)[2][2], float ca, float cb, float cc) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave & 1, wj = wave >> 1;
-  const int mp = (p.m + 31) / 32 * 32;
+  const int wave = threadIdx.x >> 6;
 #pragma unroll
   for (int a = 0; a < 2; ++a)
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int j = tj * kT + (wj * 2 + b) * 32 + (lane & 31);
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int i = ti * kT + (wi * 2 + a) * 32 + g * 8 + (lane >> 5) * 4;
-        float v[4];
-        if constexpr (POLY) {
-          float f[4] = {0.f, 0.f, 0.f, 0.f};
-          if (j < p.m && i < mp) load_planes(p.a + (long long)j * p.lda, i, f);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float t = cc * (acc[a][b][g * 4 + e] * (1.f / (kSA * kSA))) + cb * (f[e] * (1.f / kSA));
-            v[e] = (t + (i + e == j ? ca : 0.f)) * kSB;
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = acc[a][b][g * 4 + e] * (kSA / (kSX * kSX));
-        }
-        if (j < p.m && i < mp) store_planes(dst + (long long)j * p.lda, i, v);
-        if (ti != tj && j < mp) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (i + e < p.m) {
-              _Float16 h, l;
-              split16(v[e], h, l);
-              _Float16 *d = reinterpret_cast<_Float16 *>(dst + (long long)(i + e) * p.lda + (j >> 5) * 128) + (j & 31);
-              d[0] = h;
-              d[32] = l;
-            }
-        }
-      }
-    }
+    for (int b = 0; b < 2; ++b) store_symmetric_block<POLY>(p, dst, ti, tj, (wave & 1) * 2 + a, (wave >> 1) * 2 + b, acc[a][b], ca, cb, cc);
 }
 
 __global__ __launch_bounds__(kThreads, 2) void ortho_gram_kernel(const Mat *__restrict__ mats, const int *__restrict__ map, int cur) {
@@ -203,7 +207,7 @@ __global__ __launch_bounds__(kThreads, 2) void ortho_gram_kernel(const Mat *__re
   const int t = local / p.z, zi = local % p.z, tj = triangle(t, ti);
   const int total = (p.n + 31) / 32;
   const int s0 = (int)((long long)total * zi / p.z), s1 = (int)((long long)total * (zi + 1) / p.z);
-  const char *x = p.x[cur];
+  const char *x = cur ? p.x[1] : p.x[0];
   f32x16 acc[2][2];
   run<TileGram>(lds, side_kc(x, p.ldx, p.m, p.ldx, ti * kT, s0), side_kc(x, p.ldx, p.m, p.ldx, tj * kT, s0), s1 - s0, acc);
   if (p.z == 1) {
@@ -220,29 +224,34 @@ __global__ __launch_bounds__(kThreads, 2) void ortho_gram_kernel(const Mat *__re
   }
 }
 
-// the parts of a split Gram tile, added in a fixed order
+// the parts of a split Gram tile, added in a fixed order; a workgroup takes one of the four 32 x 32 blocks of every wave
 __global__ __launch_bounds__(kThreads) void ortho_reduce_kernel(const Mat *__restrict__ mats, const int *__restrict__ map) {
   const Mat p = mats[map[blockIdx.x]];
-  const int t = blockIdx.x - p.first[kReduce];
+  const int local = blockIdx.x - p.first[kReduce], t = local >> 2, q = local & 3;
   int ti;
   const int tj = triangle(t, ti), tm = (p.m + kT - 1) / kT;
-  f32x16 acc[2][2];
+  const long long stride = (long long)(tm * (tm + 1) / 2) * (kT * kT);
+  const float *s = p.part + (long long)t * (kT * kT) + q * 16 * kThreads + threadIdx.x;
+  f32x16 acc;
 #pragma unroll
-  for (int a = 0; a < 2; ++a)
+  for (int e = 0; e < 16; ++e) acc[e] = s[e * kThreads];
+  for (int zi = 1; zi < p.z; zi += 2) {                     // 32 loads in flight
+    const float *s1 = s + zi * stride, *s2 = zi + 1 < p.z ? s1 + stride : s1;
+    const float keep = zi + 1 < p.z ? 1.f : 0.f;
+    float u[16], v[16];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int e = 0; e < 16; ++e) {
+      u[e] = s1[e * kThreads];
+      v[e] = s2[e * kThreads];
+    }
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.f;
-  for (int zi = 0; zi < p.z; ++zi) {
-    const float *s = p.part + ((long long)zi * (tm * (tm + 1) / 2) + t) * (kT * kT) + threadIdx.x;
-#pragma unroll
-    for (int a = 0; a < 2; ++a)
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[a][b][e] += s[((a * 2 + b) * 16 + e) * kThreads];
+    for (int e = 0; e < 16; ++e) {
+      acc[e] += u[e];
+      if (keep != 0.f) acc[e] += v[e];
+    }
   }
-  store_symmetric<false>(p, p.a, ti, tj, acc, 0.f, 0.f, 0.f);
+  const int wave = threadIdx.x >> 6;
+  store_symmetric_block<false>(p, p.a, ti, tj, (wave & 1) * 2 + (q >> 1), (wave >> 1) * 2 + (q & 1), acc, 0.f, 0.f, 0.f);
 }
 
 __global__ __launch_bounds__(kThreads, 2) void ortho_poly_kernel(const Mat *__restrict__ mats, const int *__restrict__ map, float ca, float cb, float cc) {
@@ -261,7 +270,7 @@ __global__ __launch_bounds__(kThreads, 2) void ortho_apply_kernel(const Mat *__r
   const int local = blockIdx.x - p.first[kApply], tm = (p.m + kT - 1) / kT;
   const int tj = local % tm, ti = local / tm;
   f32x16 acc[2][2];
-  run<TileApply>(lds, side_ks<true>(p.x[cur], p.ldx, p.m, p.ldx, ti * kT * 4, 0), side_kc(p.b, p.lda, p.m, p.lda, tj * kT, 0), (p.m + 31) / 32, acc);
+  run<TileApply>(lds, side_ks<true>(cur ? p.x[1] : p.x[0], p.ldx, p.m, p.ldx, ti * kT * 4, 0), side_kc(p.b, p.lda, p.m, p.lda, tj * kT, 0), (p.m + 31) / 32, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave & 1, wj = wave >> 1;
   const int np = (p.n + 31) / 32 * 32;
 #pragma unroll
@@ -277,7 +286,7 @@ __global__ __launch_bounds__(kThreads, 2) void ortho_apply_kernel(const Mat *__r
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = acc[a][b][g * 4 + e] * (last ? 1.f / (kSB * kSX) : 1.f / kSB);
         if (!last) {
-          if (i < np) store_planes(p.x[cur ^ 1] + (long long)j * p.ldx, i, v);
+          if (i < np) store_planes((cur ? p.x[0] : p.x[1]) + (long long)j * p.ldx, i, v);
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
@@ -344,7 +353,7 @@ int plan_list(const mr3d_matrix *in, int count, char *base, Plan &plan, Mat *mat
     p.b = base + ob;
     p.part = (float *)(base + op);
     p.norm = (double *)(base + on);
-    const long long need[kStages] = {p.norm_blocks, (long long)((p.m + 63) / 64) * ((p.n + 63) / 64), (long long)tri * p.z, p.z > 1 ? tri : 0, tri, (long long)tm * tn};
+    const long long need[kStages] = {p.norm_blocks, (long long)((p.m + 63) / 64) * ((p.n + 63) / 64), (long long)tri * p.z, p.z > 1 ? 4 * tri : 0, tri, (long long)tm * tn};
     for (int s = 0; s < kStages; ++s) {
       p.first[s] = (int)blocks[s];
       blocks[s] += need[s];
