@@ -34,63 +34,81 @@ struct Side {
   unsigned ldb;
 };
 
-// KC: rows [row0, rows), k-steps from k0 on.  `row_bytes`: bytes of a row that are data (padding to 128 included)
-__device__ __forceinline__ Side side_kc(const void *p, long long ldb, long long rows, long long row_bytes, long long row0, long long kstep0) {
-  const long long off = row0 * ldb + kstep0 * 128;
-  return {(const char *)p + off, (rows - 1) * ldb + row_bytes - off, 128, (unsigned)ldb};
-}
-// KS: k rows [kstep0 * KR, krows), columns from byte `col_bytes` on
-template <bool SPLIT>
-__device__ __forceinline__ Side side_ks(const void *p, long long ldb, long long krows, long long row_bytes, long long col_bytes, long long kstep0) {
-  constexpr int KR = SPLIT ? 32 : 64;
-  const long long off = kstep0 * KR * ldb + col_bytes;
-  return {(const char *)p + off, (krows - 1) * ldb + row_bytes - off, KR * ldb, (unsigned)ldb};
-}
-
-template <int BI_, int BJ_, int NWI_, int NWJ_, bool IKS_, bool JKS_, bool SPLIT_> struct Tile {
+template <int BI_, int BJ_, int NWI_, int NWJ_, bool IKS_, bool JKS_, bool SPLIT_, int RB_, int STAGES_> struct Tile {
   static constexpr int BI = BI_, BJ = BJ_, NWI = NWI_, NWJ = NWJ_, NW = NWI * NWJ, THREADS = NW * 64;
   static constexpr bool IKS = IKS_, JKS = JKS_, SPLIT = SPLIT_;
+  static constexpr int RB = RB_, STAGES = STAGES_;                          // bytes of a KC row per k-step, tiles in LDS
   static constexpr int TI = BI / NWI / 32, TJ = BJ / NWJ / 32;              // 32 x 32 blocks of a wave
-  static constexpr int IBYTES = BI * 128, JBYTES = BJ * 128, STAGE = IBYTES + JBYTES, LDS_BYTES = 2 * STAGE;
-  static constexpr int KK = SPLIT ? 32 : 64;                                // k of a k-step
-  static_assert(BI % (8 * NW) == 0 && BJ % (8 * NW) == 0, "whole 1 KB loads per wave");
+  static constexpr int IBYTES = BI * RB, JBYTES = BJ * RB, STAGE = IBYTES + JBYTES, LDS_BYTES = STAGES * STAGE;
+  static constexpr int KK = SPLIT ? RB / 4 : RB / 2;                        // k of a k-step
+  static constexpr int NLI = IBYTES / 1024 / NW, NLJ = JBYTES / 1024 / NW;  // 1 KB loads of a wave per k-step
+  static_assert(IBYTES % (1024 * NW) == 0 && JBYTES % (1024 * NW) == 0, "whole 1 KB loads per wave");
+  static_assert(RB == 128 || (RB == 64 && !SPLIT), "a split row's group is 128 bytes");
+  static_assert(KK % 32 == 0, "fragment buffers alternate");
 };
 
+// KC: rows [row0, rows) of `row_bytes` bytes (padding to the k-step included), from k-step kstep0 on
+template <class T>
+__device__ __forceinline__ Side side_kc(const void *p, long long ldb, long long rows, long long row_bytes, long long row0, long long kstep0) {
+  const long long off = row0 * ldb + kstep0 * T::RB;
+  return {(const char *)p + off, (rows - 1) * ldb + row_bytes - off, T::RB, (unsigned)ldb};
+}
+// KS: k rows [kstep0 * KK, krows), columns from byte `col_bytes` on
+template <class T>
+__device__ __forceinline__ Side side_ks(const void *p, long long ldb, long long krows, long long row_bytes, long long col_bytes, long long kstep0) {
+  const long long off = kstep0 * T::KK * ldb + col_bytes;
+  return {(const char *)p + off, (krows - 1) * ldb + row_bytes - off, T::KK * ldb, (unsigned)ldb};
+}
+
+template <int RB> __device__ __forceinline__ int swizzle(int row) { return RB == 128 ? (row >> 1) & 7 : (row >> 2) & 3; }
+
 // source byte offset of this lane in load q of the wave (BT = tile extent, NL loads per wave)
-template <int BT, int NW, bool KS, bool SPLIT>
+template <class T, int BT, int NL, bool KS>
 __device__ __forceinline__ unsigned source_offset(int wave, int lane, int q, unsigned ldb) {
-  constexpr int NL = BT / 8 / NW;
-  const int piece = wave * NL + q;
+  const int pos = (wave * NL + q) * 64 + lane;                              // 16-byte slot of the tile
   if constexpr (!KS) {
-    const int row = piece * 8 + (lane >> 3);
-    return row * ldb + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
+    constexpr int CPR = T::RB / 16;
+    const int row = pos / CPR;
+    return row * ldb + (((pos % CPR) ^ swizzle<T::RB>(row)) << 4);
   } else {
-    constexpr int CPR = BT * (SPLIT ? 4 : 2) / 16;                          // 16-byte chunks of a k-row
-    const int pos = piece * 64 + lane, kr = pos / CPR, c = pos % CPR;
+    constexpr int CPR = BT * (T::SPLIT ? 4 : 2) / 16;
+    const int kr = pos / CPR, c = pos % CPR;
     return kr * ldb + ((((c >> 2) ^ (kr & 3)) << 6) | ((c & 3) << 4));
   }
 }
 
-template <int BT, int NW>
-__device__ __forceinline__ void stage_load(const Side &s, const unsigned (&off)[BT / 8 / NW], char *lds, int wave) {
-  constexpr int NL = BT / 8 / NW;
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// 64 lanes x 16 bytes to LDS bytes [lds, lds + 1024) in lane order.  In assembly, because the compiler puts a wait for ALL such loads in front of every
+// transposing LDS read (it cannot tell the tiles apart); the waits are run()'s own.  M0 holds the LDS address and needs one state in between
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"            // m0 is reserved: the clobber is meant all the same
+__device__ __forceinline__ void load_to_lds(i32x4 rsrc, unsigned off, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+template <int NL>
+__device__ __forceinline__ void stage_load(const Side &s, const unsigned (&off)[NL], unsigned lds) {
   const long long l = s.left;
   const int records = (int)(l < 0 ? 0 : (l > 0x7ffffff0 ? 0x7ffffff0 : l));
-  __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(s.base), 0, records, 0x00020000);
+  const uint64_t base = (uint64_t)s.base;
+  // a raw buffer: no stride, byte offsets checked against `records`; every word is wave-uniform
+  const i32x4 rsrc = {__builtin_amdgcn_readfirstlane((int)(uint32_t)base), __builtin_amdgcn_readfirstlane((int)(uint32_t)(base >> 32) & 0xffff),
+                      __builtin_amdgcn_readfirstlane(records), 0x00020000};
 #pragma unroll
-  for (int q = 0; q < NL; ++q)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(lds + (wave * NL + q) * 1024), 16, (int)off[q], 0, 0, 0);
+  for (int q = 0; q < NL; ++q) load_to_lds(rsrc, off[q], lds + q * 1024);
 }
 
 // fragment of 32 rows (block `b` of the tile) x 16 k (substep ks, plane p): lane l holds row l % 32, k = 8 (l / 32) + 0..7
-template <int BT, bool KS, bool SPLIT>
+template <class T, int BT, bool KS>
 __device__ __forceinline__ i16x8 fragment(const char *lds, int b, int ks, int p, int lane) {
   if constexpr (!KS) {
-    const int row = lane & 31, chunk = (SPLIT ? p * 4 : 0) + ks * 2 + (lane >> 5);
-    return *reinterpret_cast<const i16x8 *>(lds + b * 4096 + row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4));
+    const int row = lane & 31, chunk = (T::SPLIT ? p * 4 : 0) + ks * 2 + (lane >> 5);
+    return *reinterpret_cast<const i16x8 *>(lds + b * 32 * T::RB + row * T::RB + ((chunk ^ swizzle<T::RB>(row)) << 4));
   } else {
-    constexpr int ROWB = BT * (SPLIT ? 4 : 2);
-    const int s = lane & 15, j = s >> 2, unit = SPLIT ? b * 2 + p : b;
+    constexpr int ROWB = BT * (T::SPLIT ? 4 : 2);
+    const int s = lane & 15, j = s >> 2, unit = T::SPLIT ? b * 2 + p : b;
     const char *a = lds + (ks * 16 + (lane >> 5) * 8 + j) * ROWB + ((unit ^ j) << 6) + ((lane >> 4) & 1) * 32 + (s & 3) * 8;
     const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4 *)a);
     const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4 *)(a + 4 * ROWB));
@@ -104,17 +122,30 @@ __device__ __forceinline__ f32x16 mfma(i16x8 a, i16x8 b, f32x16 c) {
   else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+template <class T> __device__ __forceinline__ void interleave() {
+  constexpr int M = T::TI * T::TJ * (T::SPLIT ? 3 : 1), R = (T::TI * (T::IKS ? 2 : 1) + T::TJ * (T::JKS ? 2 : 1)) * (T::SPLIT ? 2 : 1);
+  constexpr int PER = (R + M - 1) / M;
+#pragma unroll
+  for (int k = 0; k < M; ++k) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+  }
+}
+
 // acc[ti][tj][e] of wave (wi, wj), lane l:  i = (wi TI + ti) 32 + 8 (e / 4) + 4 (l / 32) + e % 4,  j = (wj TJ + tj) 32 + l % 32
+//
+// STAGES - 1 k-steps are on their way while one is multiplied (a trip to L2 or HBM is longer than a k-step of 0.3 - 0.9 us).  Loads past the
+// last k-step are issued with an empty range (zeros into a tile nobody reads), so that the count of outstanding loads is the same in every step.
+// A wave reads the fragments of the next 16 k before it multiplies the current ones, across the barrier of a k-step too.
 template <class T>
 __device__ __forceinline__ void run(char *lds, Side si, Side sj, int nsteps, f32x16 (&acc)[T::TI][T::TJ]) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave % T::NWI, wj = wave / T::NWI;
-  constexpr int NLI = T::BI / 8 / T::NW, NLJ = T::BJ / 8 / T::NW;
-  unsigned oi[NLI], oj[NLJ];
+  unsigned oi[T::NLI], oj[T::NLJ];
 #pragma unroll
-  for (int q = 0; q < NLI; ++q) oi[q] = source_offset<T::BI, T::NW, T::IKS, T::SPLIT>(wave, lane, q, si.ldb);
+  for (int q = 0; q < T::NLI; ++q) oi[q] = source_offset<T, T::BI, T::NLI, T::IKS>(wave, lane, q, si.ldb);
 #pragma unroll
-  for (int q = 0; q < NLJ; ++q) oj[q] = source_offset<T::BJ, T::NW, T::JKS, T::SPLIT>(wave, lane, q, sj.ldb);
+  for (int q = 0; q < T::NLJ; ++q) oj[q] = source_offset<T, T::BJ, T::NLJ, T::JKS>(wave, lane, q, sj.ldb);
 #pragma unroll
   for (int a = 0; a < T::TI; ++a)
 #pragma unroll
@@ -122,42 +153,70 @@ __device__ __forceinline__ void run(char *lds, Side si, Side sj, int nsteps, f32
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.f;
   if (nsteps <= 0) return;
+  int to_load = nsteps;
+  const unsigned lds0 = __builtin_amdgcn_readfirstlane((int)(uintptr_t)(__attribute__((address_space(3))) char *)lds);
   auto load = [&](int buf) {
-    stage_load<T::BI, T::NW>(si, oi, lds + buf * T::STAGE, wave);
-    stage_load<T::BJ, T::NW>(sj, oj, lds + buf * T::STAGE + T::IBYTES, wave);
+    if (to_load-- <= 0) si.left = sj.left = 0;
+    stage_load<T::NLI>(si, oi, lds0 + buf * T::STAGE + wave * (T::NLI * 1024));
+    stage_load<T::NLJ>(sj, oj, lds0 + buf * T::STAGE + T::IBYTES + wave * (T::NLJ * 1024));
     si.base += si.step; si.left -= si.step;
     sj.base += sj.step; sj.left -= sj.step;
   };
-  load(0);
+  constexpr int NP = T::SPLIT ? 2 : 1, KS = T::KK / 16;
+  i16x8 fi[2][T::TI][NP], fj[2][T::TJ][NP];
+  auto fetch = [&](int which, int buf, int ks) {
+    const char *li = lds + buf * T::STAGE, *lj = li + T::IBYTES;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+#pragma unroll
+      for (int b = 0; b < T::TJ; ++b) fj[which][b][p] = fragment<T, T::BJ, T::JKS>(lj, wj * T::TJ + b, ks, p, lane);
+#pragma unroll
+      for (int a = 0; a < T::TI; ++a) fi[which][a][p] = fragment<T, T::BI, T::IKS>(li, wi * T::TI + a, ks, p, lane);
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < T::STAGES - 1; ++k) load(k);
+  // outstanding loads that may remain when stage s + 1 is needed: those of stages s + 2 .. s + STAGES - 1
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((T::STAGES - 2) * (T::NLI + T::NLJ)) : "memory");
+  __builtin_amdgcn_s_barrier();
+  if constexpr (T::STAGES == 2) load(1);
+  else load(T::STAGES - 1);
+  fetch(0, 0, 0);
+  int buf = 0;
   for (int s = 0; s < nsteps; ++s) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // this wave's part of stage s has landed
-    __syncthreads();                                       // everyone's has, and the other buffer is free
-    if (s + 1 < nsteps) load((s + 1) & 1);
-    const char *li = lds + (s & 1) * T::STAGE, *lj = li + T::IBYTES;
+    const int next = buf + 1 == T::STAGES ? 0 : buf + 1;
 #pragma unroll
-    for (int ks = 0; ks < T::KK / 16; ++ks) {
-      constexpr int NP = T::SPLIT ? 2 : 1;
-      i16x8 fi[T::TI][NP], fj[T::TJ][NP];
-#pragma unroll
-      for (int p = 0; p < NP; ++p) {
-#pragma unroll
-        for (int b = 0; b < T::TJ; ++b) fj[b][p] = fragment<T::BJ, T::JKS, T::SPLIT>(lj, wj * T::TJ + b, ks, p, lane);
-#pragma unroll
-        for (int a = 0; a < T::TI; ++a) fi[a][p] = fragment<T::BI, T::IKS, T::SPLIT>(li, wi * T::TI + a, ks, p, lane);
+    for (int ks = 0; ks < KS; ++ks) {
+      if (ks + 1 < KS) {
+        fetch((ks + 1) & 1, buf, ks + 1);
+      } else {
+        // this wave's last fragments of stage s are in registers and its loads of stage s + 1 have landed: behind the barrier both hold for
+        // every wave, stage s's tile is free
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((T::STAGES - 2) * (T::NLI + T::NLJ)) : "memory");
+        __builtin_amdgcn_s_barrier();
+        load(buf);
+        fetch(0, next, 0);
       }
+      const int w = ks & 1;
 #pragma unroll
       for (int a = 0; a < T::TI; ++a)
 #pragma unroll
         for (int b = 0; b < T::TJ; ++b) {
           if constexpr (T::SPLIT) {                        // small terms first: one rounding at the size of the result instead of three
-            acc[a][b] = mfma<true>(fi[a][0], fj[b][1], acc[a][b]);
-            acc[a][b] = mfma<true>(fi[a][1], fj[b][0], acc[a][b]);
+            acc[a][b] = mfma<true>(fi[w][a][0], fj[w][b][1], acc[a][b]);
+            acc[a][b] = mfma<true>(fi[w][a][1], fj[w][b][0], acc[a][b]);
           }
-          acc[a][b] = mfma<T::SPLIT>(fi[a][0], fj[b][0], acc[a][b]);
+          acc[a][b] = mfma<T::SPLIT>(fi[w][a][0], fj[w][b][0], acc[a][b]);
         }
+      // the reads go between the products, not in front of them: a wave that queues LDS reads issues nothing else
+      interleave<T>();
+      __builtin_amdgcn_sched_barrier(0);
     }
+    buf = next;
   }
-  __syncthreads();                                         // LDS is the caller's again
+  // the fragments read last belong to no k-step; the loads of empty ranges must not land in what LDS holds next
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
 }
 
 // x = hi + lo in fp16 (x already scaled into fp16's range)

@@ -196,7 +196,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void ce_logits_kernel(Ce c, int row0
   int ti, tj;
   tile_of(blockIdx.x, nti * ntj, nti, ntj, ti, tj);
   f32x16 acc[T::TI][T::TJ];
-  run<T>(lds, side_kc(c.wp, c.ldw, c.classes, c.ldx, ti * T::BI, 0), side_kc(c.xp + row0 * c.ldx, c.ldx, live, c.ldx, tj * T::BJ, 0),
+  run<T>(lds, side_kc<T>(c.wp, c.ldw, c.classes, c.ldx, ti * T::BI, 0), side_kc<T>(c.xp + row0 * c.ldx, c.ldx, live, c.ldx, tj * T::BJ, 0),
          (int)(c.ldx / 128), acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave % T::NWI, wj = wave / T::NWI;
   const float rsw = T::SPLIT ? 1.f / scale_of(c, 2) : 1.f;
@@ -346,7 +346,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void ce_dx_kernel(Ce c, int row0) {
   const int total = (c.classes + T::KK - 1) / T::KK;
   const int s0 = (int)((long long)total * zi / c.z), s1 = (int)((long long)total * (zi + 1) / c.z);
   f32x16 acc[T::TI][T::TJ];
-  run<T>(lds, side_ks<T::SPLIT>(c.wp, c.ldw, c.classes, c.ldx, ti * T::BI * (T::SPLIT ? 4 : 2), s0), side_kc(c.g, c.ldg, live, c.ldg, tj * T::BJ, s0),
+  run<T>(lds, side_ks<T>(c.wp, c.ldw, c.classes, c.ldx, ti * T::BI * (T::SPLIT ? 4 : 2), s0), side_kc<T>(c.g, c.ldg, live, c.ldg, tj * T::BJ, s0),
          s1 - s0, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave % T::NWI, wj = wave / T::NWI;
   const int hp = (c.hidden + 3) / 4 * 4;
@@ -405,7 +405,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void ce_dw_kernel(Ce c, int row0, in
   constexpr int E = T::SPLIT ? 4 : 2;
   f32x16 acc[T::TI][T::TJ];
   const char *x = (T::SPLIT ? c.xwp : c.xp) + row0 * c.ldx;
-  run<T>(lds, side_ks<T::SPLIT>(x, c.ldx, live, c.ldx, ti * T::BI * E, 0), side_ks<T::SPLIT>(c.g, c.ldg, live, c.ldg, (long long)tj * T::BJ * E, 0),
+  run<T>(lds, side_ks<T>(x, c.ldx, live, c.ldx, ti * T::BI * E, 0), side_ks<T>(c.g, c.ldg, live, c.ldg, (long long)tj * T::BJ * E, 0),
          (live + T::KK - 1) / T::KK, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave % T::NWI, wj = wave / T::NWI;
   const float f = T::SPLIT ? 1.f / (kSG * ((const float *)c.head)[1] * scale_of(c, 3)) : 1.f;
@@ -534,8 +534,8 @@ __global__ __launch_bounds__(256) void ce_scale_kernel(char *p, long long n, int
 // Tiles.  256 x 256 (8 waves of 128 x 64, one workgroup a CU) has the fewest LDS bytes per product; it needs enough tiles to fill 256 CUs.
 // 128 x 128 (4 waves of 64 x 64, two workgroups a CU) below that.
 template <bool IKS, bool JKS, bool SPLIT> struct Tiles {
-  typedef Tile<256, 256, 2, 4, IKS, JKS, SPLIT> Large;
-  typedef Tile<128, 128, 2, 2, IKS, JKS, SPLIT> Small;
+  typedef Tile<256, 256, 2, 4, IKS, JKS, SPLIT, 128, 2> Large;
+  typedef Tile<128, 128, 2, 2, IKS, JKS, SPLIT, 128, 2> Small;
 };
 bool large_tiles(long long i, long long j, long long z) { return ((i + 255) / 256) * ((j + 255) / 256) * z >= 192; }
 

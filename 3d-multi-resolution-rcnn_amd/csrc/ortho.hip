@@ -17,8 +17,8 @@ namespace {
 // powers of two that bring X, A and B into fp16's range: |X| < 16, |A| < 16, |B| < 64
 constexpr float kSX = 4096.f, kSA = 4096.f, kSB = 1024.f;
 constexpr int kT = 128;                                     // tile of every product
-typedef Tile<kT, kT, 2, 2, false, false, true> TileGram;
-typedef Tile<kT, kT, 2, 2, true, false, true> TileApply;
+typedef Tile<kT, kT, 2, 2, false, false, true, 128, 2> TileGram;
+typedef Tile<kT, kT, 2, 2, true, false, true, 128, 2> TileApply;
 constexpr int kThreads = TileGram::THREADS;
 
 enum Stage { kNorm, kPack, kGram, kReduce, kPoly, kApply, kStages };
@@ -209,7 +209,7 @@ __global__ __launch_bounds__(kThreads, 2) void ortho_gram_kernel(const Mat *__re
   const int s0 = (int)((long long)total * zi / p.z), s1 = (int)((long long)total * (zi + 1) / p.z);
   const char *x = cur ? p.x[1] : p.x[0];
   f32x16 acc[2][2];
-  run<TileGram>(lds, side_kc(x, p.ldx, p.m, p.ldx, ti * kT, s0), side_kc(x, p.ldx, p.m, p.ldx, tj * kT, s0), s1 - s0, acc);
+  run<TileGram>(lds, side_kc<TileGram>(x, p.ldx, p.m, p.ldx, ti * kT, s0), side_kc<TileGram>(x, p.ldx, p.m, p.ldx, tj * kT, s0), s1 - s0, acc);
   if (p.z == 1) {
     store_symmetric<false>(p, p.a, ti, tj, acc, 0.f, 0.f, 0.f);
   } else {
@@ -260,7 +260,7 @@ __global__ __launch_bounds__(kThreads, 2) void ortho_poly_kernel(const Mat *__re
   int ti;
   const int tj = triangle(blockIdx.x - p.first[kPoly], ti);
   f32x16 acc[2][2];
-  run<TileGram>(lds, side_kc(p.a, p.lda, p.m, p.lda, ti * kT, 0), side_kc(p.a, p.lda, p.m, p.lda, tj * kT, 0), (p.m + 31) / 32, acc);
+  run<TileGram>(lds, side_kc<TileGram>(p.a, p.lda, p.m, p.lda, ti * kT, 0), side_kc<TileGram>(p.a, p.lda, p.m, p.lda, tj * kT, 0), (p.m + 31) / 32, acc);
   store_symmetric<true>(p, p.b, ti, tj, acc, ca, cb, cc);
 }
 
@@ -270,7 +270,7 @@ __global__ __launch_bounds__(kThreads, 2) void ortho_apply_kernel(const Mat *__r
   const int local = blockIdx.x - p.first[kApply], tm = (p.m + kT - 1) / kT;
   const int tj = local % tm, ti = local / tm;
   f32x16 acc[2][2];
-  run<TileApply>(lds, side_ks<true>(cur ? p.x[1] : p.x[0], p.ldx, p.m, p.ldx, ti * kT * 4, 0), side_kc(p.b, p.lda, p.m, p.lda, tj * kT, 0), (p.m + 31) / 32, acc);
+  run<TileApply>(lds, side_ks<TileApply>(cur ? p.x[1] : p.x[0], p.ldx, p.m, p.ldx, ti * kT * 4, 0), side_kc<TileApply>(p.b, p.lda, p.m, p.lda, tj * kT, 0), (p.m + 31) / 32, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave & 1, wj = wave >> 1;
   const int np = (p.n + 31) / 32 * 32;
 #pragma unroll
