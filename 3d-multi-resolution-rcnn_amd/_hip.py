@@ -45,26 +45,8 @@ def lib():
         L.mr3d_status_string.argtypes = [ctypes.c_int]
         L.mr3d_nms3d_workspace_bytes.restype = ctypes.c_size_t
         L.mr3d_nms3d_workspace_bytes.argtypes = [ctypes.c_int]
-        _declare(L)
         _lib = L
     return _lib
-
-
-def _declare(L):
-    """argument types of the calls whose cost at the smallest sizes is the binding's: converted without a look at each value"""
-    p, i, ll, f, z = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_size_t
-    for name, res, args in (
-            ('mr3d_linear_cross_entropy_workspace_bytes', z, [p]),
-            ('mr3d_linear_cross_entropy', i, [p, p, z, p]),
-            ('mr3d_scale_by', i, [p, ll, i, p, p]),
-            ('mr3d_orthogonalize_workspace_bytes', z, [p, i]),
-            ('mr3d_orthogonalize', i, [p, i, i, f, f, f, f, p, z, p]),
-            ('mr3d_layer_norm_workspace_bytes', z, [ll, i, i]),
-            ('mr3d_layer_norm_forward', i, [p, ll, p, p, p, p, p, ll, i, f, i, i, p]),
-            ('mr3d_layer_norm_backward', i, [p, ll, p, ll, p, p, p, p, p, p, ll, i, i, i, p, z, p])):
-        fn = getattr(L, name, None)          # MR3D_LIB may name an older build
-        if fn is not None:
-            fn.restype, fn.argtypes = res, args
 
 
 def check(status, what):
@@ -1369,98 +1351,18 @@ def mask_bce(pred, target, labels, valid_rows=None, want_grad=True):
 
 
 # --------------------------------------------------------------------------------------------
-STORAGE_DTYPES = {torch.float32: 0, torch.bfloat16: 1}                   # MR3D_DTYPE_F32 / _BF16
+_train = None
 
 
-def _addr(t):
-    return None if t is None else t.data_ptr()
-
-
-def layer_norm_forward(x, weight, bias, eps, want_stats):
-    """x [rows, cols] (last axis contiguous) -> y, mean, rstd (None without want_stats)"""
-    rows, cols = x.shape
-    y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if want_stats else None
-    param = weight if weight is not None else bias
-    pd = STORAGE_DTYPES[param.dtype if param is not None else x.dtype]
-    sp = None if stats is None else stats.data_ptr()
-    with torch.cuda.device(x.device):
-        check(lib().mr3d_layer_norm_forward(x.data_ptr(), x.stride(0), _addr(weight), _addr(bias), y.data_ptr(), sp,
-                                            None if sp is None else sp + 4 * rows, rows, cols, eps, STORAGE_DTYPES[x.dtype], pd,
-                                            torch.cuda.current_stream(x.device).cuda_stream), 'mr3d_layer_norm_forward')
-    return y, stats
-
-
-def layer_norm_backward(x, dy, weight, stats, param_dtype, want_dx, want_dw, want_db):
-    rows, cols = x.shape
-    dev = x.device
-    dx = torch.empty((rows, cols), dtype=x.dtype, device=dev) if want_dx else None
-    dw = torch.empty((cols,), dtype=param_dtype, device=dev) if want_dw else None
-    db = torch.empty((cols,), dtype=param_dtype, device=dev) if want_db else None
-    dt = STORAGE_DTYPES[x.dtype]
-    with torch.cuda.device(dev):
-        need = lib().mr3d_layer_norm_workspace_bytes(rows, cols, dt) if want_dw or want_db else 0
-        ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
-        check(lib().mr3d_layer_norm_backward(x.data_ptr(), x.stride(0), dy.data_ptr(), dy.stride(0), _addr(weight), stats.data_ptr(),
-                                             stats.data_ptr() + 4 * rows, _addr(dx), _addr(dw), _addr(db), rows, cols, dt,
-                                             STORAGE_DTYPES[param_dtype], _addr(ws), need,
-                                             torch.cuda.current_stream(dev).cuda_stream), 'mr3d_layer_norm_backward')
-    return dx, dw, db
-
-
-class Matrix(ctypes.Structure):
-    """mr3d_matrix (include/mr3d.h)"""
-    _fields_ = [('in_', ctypes.c_void_p), ('out', ctypes.c_void_p), ('rows', ctypes.c_longlong), ('cols', ctypes.c_longlong),
-                ('in_row_stride', ctypes.c_longlong), ('in_col_stride', ctypes.c_longlong), ('dtype', ctypes.c_int), ('reserved', ctypes.c_int)]
-
-
-def orthogonalize(mats, outs, steps, coefficients, eps):
-    """mats: 2-D tensors of one device, none of them empty; outs: packed tensors of the same types and sizes (may be mats themselves)"""
-    dev = mats[0].device
-    table = (Matrix * len(mats))(*[(m.data_ptr(), o.data_ptr(), m.shape[0], m.shape[1], *m.stride(), STORAGE_DTYPES[m.dtype], 0)
-                                   for m, o in zip(mats, outs)])
-    a, b, c = coefficients
-    with torch.cuda.device(dev):
-        need = lib().mr3d_orthogonalize_workspace_bytes(table, len(mats))
-        ws = torch.empty((max(need, 256),), dtype=torch.uint8, device=dev)
-        check(lib().mr3d_orthogonalize(table, len(mats), steps, a, b, c, eps, ws.data_ptr(), need, torch.cuda.current_stream(dev).cuda_stream),
-              'mr3d_orthogonalize')
-
-
-class LinearCe(ctypes.Structure):
-    """mr3d_linear_ce (include/mr3d.h)"""
-    _fields_ = [(n, ctypes.c_void_p) for n in ('x', 'weight', 'bias', 'labels', 'row_weight', 'avg_factor_dev', 'valid_rows_dev', 'loss', 'dx',
-                                               'dweight', 'dbias')] + \
-               [(n, ctypes.c_longlong) for n in ('x_stride', 'weight_stride', 'ignore_index')] + [('avg_factor', ctypes.c_float)] + \
-               [(n, ctypes.c_int) for n in ('rows', 'hidden', 'classes', 'dtype', 'param_dtype', 'want_dx', 'want_dweight', 'want_dbias')]
-
-
-def linear_cross_entropy(x, weight, bias, labels, row_weight, avg_factor, valid_rows, ignore_index, want_dx, want_dw, want_db):
-    """x [rows, hidden], weight [classes, hidden] (last axes contiguous) -> loss [1], dx, dweight, dbias (None where not wanted)"""
-    dev = x.device
-    rows, hidden = x.shape
-    classes = weight.shape[0]
-    loss = torch.empty((1,), dtype=torch.float32, device=dev)
-    dx = torch.empty((rows, hidden), dtype=x.dtype, device=dev) if want_dx else None
-    dw = torch.empty((classes, hidden), dtype=x.dtype, device=dev) if want_dw else None
-    db = torch.empty((classes,), dtype=bias.dtype, device=dev) if want_db else None
-    on_dev = torch.is_tensor(avg_factor)
-    a = LinearCe(x.data_ptr(), weight.data_ptr(), _addr(bias), labels.data_ptr(), _addr(row_weight), avg_factor.data_ptr() if on_dev else None,
-                 _addr(valid_rows), loss.data_ptr(), _addr(dx), _addr(dw), _addr(db), x.stride(0), weight.stride(0), ignore_index,
-                 0.0 if on_dev or avg_factor is None else avg_factor, rows, hidden, classes, STORAGE_DTYPES[x.dtype],
-                 STORAGE_DTYPES[x.dtype if bias is None else bias.dtype], want_dx, want_dw, want_db)
-    ref = ctypes.byref(a)
-    with torch.cuda.device(dev):
-        need = lib().mr3d_linear_cross_entropy_workspace_bytes(ref)
-        ws = torch.empty((need + 1024,), dtype=torch.uint8, device=dev)
-        check(lib().mr3d_linear_cross_entropy(ref, ws.data_ptr() + -ws.data_ptr() % 1024, need, torch.cuda.current_stream(dev).cuda_stream),
-              'mr3d_linear_cross_entropy')
-    return loss, dx, dw, db
-
-
-def scale_by(t, factor):
-    """t *= factor (a device scalar) in place; free when the factor is 1"""
-    with torch.cuda.device(t.device):
-        check(lib().mr3d_scale_by(t.data_ptr(), t.numel(), STORAGE_DTYPES[t.dtype], factor.data_ptr(),
-                                  torch.cuda.current_stream(t.device).cuda_stream), 'mr3d_scale_by')
-    return t
+def train_ops():
+    """the extension module over layer norm, linear cross entropy and orthogonalised updates (csrc/torch_ext/train_ops.cpp)"""
+    global _train
+    if _train is None:
+        lib()
+        try:
+            from . import _train_ops
+        except ImportError as e:
+            raise Mr3dError(f'the extension module _train_ops is missing ({e}): build it with '
+                            f'`python -c "import __graft_entry__ as g; g.build()"` (or `make -C {_CSRC} ext`)') from e
+        _train = _train_ops
+    return _train

@@ -19,6 +19,7 @@ using namespace gemm16;
 namespace {
 
 typedef __bf16 bf16;
+constexpr float kLog2e = 1.44269504f;
 constexpr float kSG = 16384.f;                               // fp32: g without its weight, in [-1, 1], times this
 constexpr long long kPiece = 1ll << 31;
 constexpr int kStatCols = 128;                               // classes per (max, sum) pair
@@ -47,6 +48,10 @@ struct Ce {
   float *loss;
   int db_f32;
 };
+
+// four values at any element's alignment
+typedef float vf4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef bf16 vb4 __attribute__((ext_vector_type(4), aligned(2)));
 
 template <bool F32> __device__ __forceinline__ float elem(const char *p, long long i) {
   return F32 ? ((const float *)p)[i] : (float)((const bf16 *)p)[i];
@@ -107,41 +112,44 @@ __device__ __forceinline__ float block_max(float v, float *lds) {
   return fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
 }
 
-// this thread's share of a row, 16 bytes a load with the alignment of a float (odd strides), eight in flight for rows of 1024 and more
+// largest |p[k]| of a row, by one wave: 16 bytes a load with the alignment of a float (odd strides)
 __device__ __forceinline__ float row_max(const float *p, int n) {
   typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
   float m = 0.f;
-  int k = threadIdx.x * 4;
+  int k = (threadIdx.x & 63) * 4;
 #pragma unroll 4
-  for (; k + 4 <= n; k += 1024) {
+  for (; k + 4 <= n; k += 256) {
     const f4 t = *reinterpret_cast<const f4 *>(p + k);
     m = fmaxf(fmaxf(fmaxf(m, fabsf(t[0])), fabsf(t[1])), fmaxf(fabsf(t[2]), fabsf(t[3])));
   }
-  for (; k < n; ++k) m = fmaxf(m, fabsf(p[k]));            // the last, partial group: one thread's
+  for (; k < n; ++k) m = fmaxf(m, fabsf(p[k]));            // the last, partial group: one lane's
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
   return m;
 }
 
-// fp32: the largest |x| of each live row and |x w| of all, the largest |W| (the first `rows` workgroups take x, the rest W).  The maximum of
-// positive floats is the maximum of their bits: an integer atomic, whose order does not matter
-__global__ __launch_bounds__(256) void ce_max_kernel(Ce c, int wblocks) {
+// fp32: the largest |x| of each live row and |x w| of all, the largest |W|; a wave per row, the first `xblocks` workgroups take x, the rest W.
+// The maximum of positive floats is the maximum of their bits: an integer atomic, whose order does not matter -- one per workgroup, because
+// a thousand of them on one address take 15 us
+__global__ __launch_bounds__(256) void ce_max_kernel(Ce c, int xblocks, int wblocks) {
   __shared__ float lds[4];
   float m = 0.f;
-  if ((int)blockIdx.x < c.rows) {
-    if ((int)blockIdx.x >= c.head[0]) return;
-    const int r = c.index[blockIdx.x];
-    const float *x = (const float *)c.x + r * c.x_stride;
-    m = block_max(row_max(x, c.hidden), lds);
-    if (threadIdx.x == 0) {
-      c.xmax[blockIdx.x] = m;
-      const float w = m * fabsf(c.row_weight ? c.row_weight[r] : 1.f);
-      if (w < 3.0e38f) atomicMax(&c.head[3], __float_as_int(w));
-      else atomicMax(&c.head[3], 0x7f800000);
+  const int wave = threadIdx.x >> 6;
+  const bool is_x = (int)blockIdx.x < xblocks;
+  if (is_x) {
+    const int live = c.head[0];
+    for (int j = blockIdx.x * 4 + wave; j < live; j += xblocks * 4) {
+      const int r = c.index[j];
+      const float v = row_max((const float *)c.x + r * c.x_stride, c.hidden);
+      if ((threadIdx.x & 63) == 0) c.xmax[j] = v;
+      const float w = v * fabsf(c.row_weight ? c.row_weight[r] : 1.f);
+      m = fmaxf(m, w < 3.0e38f ? w : INFINITY);             // a NaN weight counts as infinite: the scale falls back to 1
     }
   } else {
-    for (int v = blockIdx.x - c.rows; v < c.classes; v += wblocks) m = fmaxf(m, row_max((const float *)c.w + v * c.w_stride, c.hidden));
-    m = block_max(m, lds);
-    if (threadIdx.x == 0) atomicMax(&c.head[2], __float_as_int(m));
+    for (int v = (blockIdx.x - xblocks) * 4 + wave; v < c.classes; v += wblocks * 4) m = fmaxf(m, row_max((const float *)c.w + v * c.w_stride, c.hidden));
   }
+  m = block_max(m, lds);
+  if (threadIdx.x == 0 && m > 0.f) atomicMax(&c.head[is_x ? 3 : 2], __float_as_int(m));
 }
 
 // one stored row of an operand: bf16 copied, fp32 split; zeros behind the last column
@@ -199,28 +207,43 @@ __global__ __launch_bounds__(T::THREADS, 2) void ce_logits_kernel(Ce c, int row0
   run<T>(lds, side_kc<T>(c.wp, c.ldw, c.classes, c.ldx, ti * T::BI, 0), side_kc<T>(c.xp + row0 * c.ldx, c.ldx, live, c.ldx, tj * T::BJ, 0),
          (int)(c.ldx / 128), acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave % T::NWI, wj = wave / T::NWI;
-  const float rsw = T::SPLIT ? 1.f / scale_of(c, 2) : 1.f;
+  const float rsw = T::SPLIT ? kLog2e / scale_of(c, 2) : kLog2e;
   const int vpad = (int)(c.ldg / (T::SPLIT ? 4 : 2));
   constexpr int WI = T::TI * 32;
-  static_assert(WI <= kStatCols && kStatCols % WI == 0, "a wave's classes lie in one pair or its own part of it");
+  static_assert(kStatCols % WI == 0, "a wave's classes lie in one pair");
+  const bool ragged = (ti + 1) * T::BI > c.classes;
 #pragma unroll
   for (int b = 0; b < T::TJ; ++b) {
-    const int j = tj * T::BJ + (wj * T::TJ + b) * 32 + (lane & 31);
-    const float rs = T::SPLIT ? rsw / scale_for(j < live ? c.xmax[row0 + j] : 0.f) : 1.f;
+    const int jl = (wj * T::TJ + b) * 32 + (lane & 31), j = tj * T::BJ + jl;
+    const float rs = T::SPLIT ? rsw / scale_for(j < live ? c.xmax[row0 + j] : 0.f) : rsw;
     const int iw = ti * T::BI + wi * WI + (lane >> 5) * 4;
+    // z log2 e: exponentials and sums are taken to base 2, one instruction each
+    if (c.bias) {
+#pragma unroll
+      for (int a = 0; a < T::TI; ++a)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int i = min(iw + a * 32 + (e / 4) * 8 + (e & 3), c.classes - 1);
+          acc[a][b][e] = fmaf(acc[a][b][e], rs, kLog2e * (c.bias_f32 ? ((const float *)c.bias)[i] : (float)((const bf16 *)c.bias)[i]));
+        }
+    } else {
+#pragma unroll
+      for (int a = 0; a < T::TI; ++a)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[a][b][e] *= rs;
+    }
+    if (ragged) {
+#pragma unroll
+      for (int a = 0; a < T::TI; ++a)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (iw + a * 32 + (e / 4) * 8 + (e & 3) >= c.classes) acc[a][b][e] = -INFINITY;
+    }
     float m = -INFINITY;
 #pragma unroll
     for (int a = 0; a < T::TI; ++a)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int i = iw + a * 32 + (e / 4) * 8 + (e & 3);
-        float z = acc[a][b][e];
-        if constexpr (T::SPLIT) z *= rs;
-        if (c.bias) z += i < c.classes ? (c.bias_f32 ? ((const float *)c.bias)[i] : (float)((const bf16 *)c.bias)[i]) : 0.f;
-        if (i >= c.classes) z = -INFINITY;
-        acc[a][b][e] = z;
-        m = fmaxf(m, z);
-      }
+      for (int e = 0; e < 16; ++e) m = fmaxf(m, acc[a][b][e]);
     m = fmaxf(m, __shfl_xor(m, 32));
     const float ms = m == -INFINITY ? 0.f : m;
     float s = 0.f;
@@ -228,30 +251,47 @@ __global__ __launch_bounds__(T::THREADS, 2) void ce_logits_kernel(Ce c, int row0
     for (int a = 0; a < T::TI; ++a)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const float p = __expf(acc[a][b][e] - ms);
+        const float p = __builtin_amdgcn_exp2f(acc[a][b][e] - ms);
         s += p;
         acc[a][b][e] = p;
       }
     s += __shfl_xor(s, 32);
-    if (j >= live) continue;
-    if (lane < 32) c.stats[(long long)j * c.pieces + (ti * T::BI + wi * WI) / WI] = make_float2(m, s);
-    if constexpr (TRAIN) {
-      char *row = c.g + j * c.ldg;
+    if (lane < 32 && j < live) c.stats[(long long)j * c.pieces + (ti * T::BI + wi * WI) / WI] = make_float2(m, s);
+    if constexpr (TRAIN && T::SPLIT) {
+      if (j < live) {
+        char *row = c.g + j * c.ldg;
+#pragma unroll
+        for (int a = 0; a < T::TI; ++a)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int i = iw + a * 32 + q * 8;
+            if (i < vpad)
+              *reinterpret_cast<float4 *>(row + i * 4) = make_float4(acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]);
+          }
+      }
+    } else if constexpr (TRAIN) {
+      // through LDS, so that a row leaves in whole 16-byte pieces side by side; piece u of row jl sits at u ^ jl (a lane is a row)
 #pragma unroll
       for (int a = 0; a < T::TI; ++a)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int i = iw + a * 32 + q * 8;
-          if (i >= vpad) continue;
-          if constexpr (T::SPLIT) {
-            *reinterpret_cast<float4 *>(row + i * 4) = make_float4(acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]);
-          } else {
-            _Float16 t[4];
+          const int u = (wi * WI + a * 32 + q * 8) >> 3;
+          _Float16 t[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) t[e] = (_Float16)acc[a][b][4 * q + e];
-            *reinterpret_cast<uint2 *>(row + i * 2) = *reinterpret_cast<uint2 *>(t);
-          }
+          for (int e = 0; e < 4; ++e) t[e] = (_Float16)acc[a][b][4 * q + e];
+          *reinterpret_cast<uint2 *>(lds + jl * (T::BI * 2) + ((u ^ (jl & (T::BI / 8 - 1))) << 4) + (lane >> 5) * 8) = *reinterpret_cast<uint2 *>(t);
         }
+    }
+  }
+  if constexpr (TRAIN && !T::SPLIT) {
+    constexpr int U = T::BI / 8;                             // 16-byte pieces of a row
+    __syncthreads();
+    const int u = threadIdx.x % U, i = ti * T::BI + u * 8;
+#pragma unroll 4
+    for (int jl = threadIdx.x / U; jl < T::BJ; jl += T::THREADS / U) {
+      const int j = tj * T::BJ + jl;
+      if (j < live && i < vpad)
+        *reinterpret_cast<uint4 *>(c.g + j * c.ldg + i * 2) = *reinterpret_cast<const uint4 *>(lds + jl * (T::BI * 2) + ((u ^ (jl & (U - 1))) << 4));
     }
   }
 }
@@ -285,7 +325,7 @@ __global__ __launch_bounds__(256) void ce_grad_kernel(Ce c, int row0, int wcols)
   nan = __syncthreads_or(nan);
   const float ms = m == -INFINITY ? 0.f : m;
   double s = 0;
-  for (int k = threadIdx.x; k < c.pieces; k += 256) s += (double)st[k].y * (double)expf(st[k].x - ms);
+  for (int k = threadIdx.x; k < c.pieces; k += 256) s += (double)st[k].y * (double)__builtin_amdgcn_exp2f(st[k].x - ms);
   s = block_sum(s, lds);
   const long long label = c.labels[r];
   const bool known = label >= 0 && label < c.classes;        // else: the loss and this row's gradient are NaN
@@ -295,18 +335,18 @@ __global__ __launch_bounds__(256) void ce_grad_kernel(Ce c, int row0, int wcols)
       dot += (double)elem<F32>(c.x, r * c.x_stride + k) * (double)elem<F32>(c.w, label * c.w_stride + k);
   dot = block_sum(dot, lds);
   if (known && c.bias) dot += c.bias_f32 ? (double)((const float *)c.bias)[label] : (double)(float)((const bf16 *)c.bias)[label];
-  const double lse = known && !nan ? (double)m + log(s) : (double)NAN;
+  const double lse2 = known && !nan ? (double)m + log2(s) : (double)NAN, lse = lse2 * 0.69314718055994530942;
   const float w = c.row_weight ? c.row_weight[r] : 1.f;
   if (threadIdx.x == 0) c.row_loss[row0 + j] = (lse - dot) * (double)w;
   if constexpr (TRAIN) {
-    const float l = (float)lse, avg = ((const float *)c.head)[1];
+    const float l = (float)lse2, avg = ((const float *)c.head)[1];
     const float f = F32 ? kSG : w / avg;
     const float at = (float)expm1(dot - lse);                // p - 1 of the label, without the cancellation
     char *row = c.g + j * c.ldg;
     if constexpr (F32) {
       for (long long k = threadIdx.x * 4; k < c.ldg / 4; k += 1024) {
         float4 p = *reinterpret_cast<const float4 *>(row + k * 4);
-        const float e = __expf(st[k / wcols].x - l) * f;
+        const float e = __builtin_amdgcn_exp2f(st[k / wcols].x - l) * f;
         float v[4] = {p.x * e, p.y * e, p.z * e, p.w * e};
 #pragma unroll
         for (int q = 0; q < 4; ++q)
@@ -324,7 +364,7 @@ __global__ __launch_bounds__(256) void ce_grad_kernel(Ce c, int row0, int wcols)
         _Float16 p[8];
         bf16 t[8];
         *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(row + k * 2);
-        const float e = __expf(st[k / wcols].x - l) * f;
+        const float e = __builtin_amdgcn_exp2f(st[k / wcols].x - l) * f;
 #pragma unroll
         for (int q = 0; q < 8; ++q) t[q] = (bf16)(k + q == label ? at * f : (float)p[q] * e);
         *reinterpret_cast<uint4 *>(row + k * 2) = *reinterpret_cast<uint4 *>(t);
@@ -384,12 +424,18 @@ __global__ __launch_bounds__(256) void ce_dx_rows_kernel(Ce c, int row0) {
       if constexpr (F32) { v.x *= f; v.y *= f; v.z *= f; v.w *= f; }
     }
     const float o[4] = {v.x, v.y, v.z, v.w};
+    const long long at = (long long)r * c.hidden + k;
+    if (k + 4 <= c.hidden) {
+      if (F32) *reinterpret_cast<vf4 *>((float *)c.dx + at) = vf4{o[0], o[1], o[2], o[3]};
+      else *reinterpret_cast<vb4 *>((bf16 *)c.dx + at) = vb4{(bf16)o[0], (bf16)o[1], (bf16)o[2], (bf16)o[3]};
+    } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (k + e < c.hidden) {
-        if (F32) ((float *)c.dx)[(long long)r * c.hidden + k + e] = o[e];
-        else ((bf16 *)c.dx)[(long long)r * c.hidden + k + e] = (bf16)o[e];
-      }
+      for (int e = 0; e < 4; ++e)
+        if (k + e < c.hidden) {
+          if (F32) ((float *)c.dx)[at + e] = o[e];
+          else ((bf16 *)c.dx)[at + e] = (bf16)o[e];
+        }
+    }
   }
 }
 
@@ -422,16 +468,13 @@ __global__ __launch_bounds__(T::THREADS, 2) void ce_dw_kernel(Ce c, int row0, in
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = T::SPLIT ? acc[a][b][4 * q + e] * f : acc[a][b][4 * q + e];
         const long long at = (long long)j * c.hidden + i;
-        const bool whole = i + 4 <= c.hidden && (c.hidden & 3) == 0;
+        const bool whole = i + 4 <= c.hidden;
         if (T::SPLIT || mode) {
           float *d = (T::SPLIT ? (float *)c.dw : c.dwacc) + at;
           if (whole) {
-            float4 t = make_float4(v[0], v[1], v[2], v[3]);
-            if (mode == 2) {
-              const float4 o = *reinterpret_cast<const float4 *>(d);
-              t = make_float4(o.x + t.x, o.y + t.y, o.z + t.z, o.w + t.w);
-            }
-            *reinterpret_cast<float4 *>(d) = t;
+            vf4 t = {v[0], v[1], v[2], v[3]};
+            if (mode == 2) t += *reinterpret_cast<const vf4 *>(d);
+            *reinterpret_cast<vf4 *>(d) = t;
           } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -439,14 +482,13 @@ __global__ __launch_bounds__(T::THREADS, 2) void ce_dw_kernel(Ce c, int row0, in
           }
         } else {
           bf16 *d = (bf16 *)c.dw + at;
-          bf16 t[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) t[e] = (bf16)v[e];
-          if (whole) *reinterpret_cast<uint2 *>(d) = *reinterpret_cast<uint2 *>(t);
-          else
+          if (whole) {
+            *reinterpret_cast<vb4 *>(d) = vb4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
+          } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (i + e < c.hidden) d[e] = t[e];
+              if (i + e < c.hidden) d[e] = (bf16)v[e];
+          }
         }
       }
   }
@@ -521,13 +563,15 @@ __global__ __launch_bounds__(256) void ce_loss_kernel(Ce c) {
   if (threadIdx.x == 0) c.loss[0] = (float)(s / (double)((const float *)c.head)[1]);
 }
 
-// grad *= *factor, unless the factor is 1 (the usual root of a backward pass): then nothing is read or written
-__global__ __launch_bounds__(256) void ce_scale_kernel(char *p, long long n, int f32, const float *__restrict__ factor) {
+// gradients *= *factor, unless the factor is 1 (the usual root of a backward pass): then nothing is read or written
+struct Spans { mr3d_span s[4]; };
+__global__ __launch_bounds__(256) void ce_scale_kernel(Spans spans, const float *__restrict__ factor) {
   const float f = *factor;
   if (f == 1.f) return;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-    if (f32) ((float *)p)[i] *= f;
-    else ((bf16 *)p)[i] = (bf16)((float)((bf16 *)p)[i] * f);
+  const mr3d_span p = spans.s[blockIdx.y];
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < p.count; i += (long long)gridDim.x * 256) {
+    if (p.dtype == MR3D_DTYPE_F32) ((float *)p.data)[i] *= f;
+    else ((bf16 *)p.data)[i] = (bf16)((float)((bf16 *)p.data)[i] * f);
   }
 }
 
@@ -640,8 +684,8 @@ template <bool F32> int run_ce(const mr3d_linear_ce *a, const Layout &l, Ce &c, 
   typedef Tiles<true, true, F32> TW;
   ce_rows_kernel<<<1, 1024, 0, q>>>(c);
   if (F32) {
-    const int wb = a->classes < 1024 ? a->classes : 1024;
-    ce_max_kernel<<<a->rows + wb, 256, 0, q>>>(c, wb);
+    const int xb = a->rows < 512 ? (a->rows + 3) / 4 : 128, wb = a->classes < 2048 ? (a->classes + 3) / 4 : 512;
+    ce_max_kernel<<<xb + wb, 256, 0, q>>>(c, xb, wb);
   }
   ce_pack_kernel<F32><<<a->rows + (l.pack_w ? a->classes : 0), 256, 0, q>>>(c, a->want_dweight);
   for (int k = 0; k < l.chunks; ++k) {
@@ -708,11 +752,19 @@ extern "C" int mr3d_linear_cross_entropy(const mr3d_linear_ce *a, void *workspac
   return a->dtype == MR3D_DTYPE_F32 ? run_ce<true>(a, l, c, mr3d_stream(s)) : run_ce<false>(a, l, c, mr3d_stream(s));
 }
 
-extern "C" int mr3d_scale_by(void *data, long long count, int dtype, const float *factor_dev, mr3d_stream_t s) {
-  if (!data || count < 0 || !factor_dev) return MR3D_ERR_INVALID_ARG;
-  if (dtype != MR3D_DTYPE_F32 && dtype != MR3D_DTYPE_BF16) return MR3D_ERR_UNSUPPORTED;
-  if (!count) return MR3D_OK;
-  const long long blocks = (count + 2047) / 2048;
-  ce_scale_kernel<<<(unsigned)(blocks > 2048 ? 2048 : blocks), 256, 0, mr3d_stream(s)>>>((char *)data, count, dtype == MR3D_DTYPE_F32, factor_dev);
+extern "C" int mr3d_scale_by(const mr3d_span *spans_host, int num_spans, const float *factor_dev, mr3d_stream_t s) {
+  if (!spans_host || num_spans < 1 || num_spans > 4 || !factor_dev) return MR3D_ERR_INVALID_ARG;
+  Spans spans{};
+  long long most = 0;
+  for (int i = 0; i < num_spans; ++i) {
+    const mr3d_span &p = spans_host[i];
+    if (p.count < 0 || (p.count && !p.data)) return MR3D_ERR_INVALID_ARG;
+    if (p.dtype != MR3D_DTYPE_F32 && p.dtype != MR3D_DTYPE_BF16) return MR3D_ERR_UNSUPPORTED;
+    spans.s[i] = p;
+    most = p.count > most ? p.count : most;
+  }
+  if (!most) return MR3D_OK;
+  const long long blocks = (most + 2047) / 2048;
+  ce_scale_kernel<<<dim3((unsigned)(blocks > 1024 ? 1024 : blocks), num_spans), 256, 0, mr3d_stream(s)>>>(spans, factor_dev);
   return mr3d_launch_status();
 }

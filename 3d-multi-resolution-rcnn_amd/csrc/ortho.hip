@@ -84,8 +84,25 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(const Mat *__restrict__
   double s = 0;
   long long e = (long long)chunk * 256 + threadIdx.x;
   const long long stride = (long long)p.norm_blocks * 256;
-  if (si == 1 && so == inner) {
-    for (; e < total; e += stride) {
+  if (si == 1 && so == inner && ((uintptr_t)p.in & 15) == 0) {            // packed: 16 bytes a load
+    const int per = p.bf16 ? 8 : 4;
+    const long long groups = total / per;
+#pragma unroll 2
+    for (; e < groups; e += stride) {
+      float v[8];
+      if (p.bf16) {
+        const bf16x8 t = *reinterpret_cast<const bf16x8 *>(p.in + e * 16);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = (float)t[k];
+      } else {
+        const float4 t = *reinterpret_cast<const float4 *>(p.in + e * 16);
+        v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+        v[4] = v[5] = v[6] = v[7] = 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += (double)v[k] * (double)v[k];
+    }
+    for (e = groups * per + (long long)chunk * 256 + threadIdx.x; e < total; e += stride) {
       const double v = (double)read_in(p, e);
       s += v * v;
     }
@@ -111,7 +128,8 @@ __global__ __launch_bounds__(256) void ortho_pack_kernel(const Mat *__restrict__
   const Mat p = mats[map[blockIdx.x]];
   const int tile = blockIdx.x - p.first[kPack], tn = (p.n + 63) / 64;
   const int j0 = tile / tn * 64, i0 = tile % tn * 64;
-  double s = (int)threadIdx.x < p.norm_blocks ? p.norm[threadIdx.x] : 0.;
+  double s = 0;
+  for (int k = threadIdx.x; k < p.norm_blocks; k += 256) s += p.norm[k];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
   if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = s;
@@ -344,7 +362,7 @@ int plan_list(const mr3d_matrix *in, int count, char *base, Plan &plan, Mat *mat
     if (z > steps / 8) z = steps / 8;
     p.z = (int)(z < 1 ? 1 : z);
     const long long numel = (long long)p.m * p.n;
-    p.norm_blocks = (int)((numel + 8191) / 8192 > 256 ? 256 : (numel + 8191) / 8192);
+    p.norm_blocks = (int)((numel + 8191) / 8192 > 1024 ? 1024 : (numel + 8191) / 8192);
     const size_t ox0 = take(at, (size_t)p.m * p.ldx), ox1 = take(at, (size_t)p.m * p.ldx), oa = take(at, (size_t)p.m * p.lda), ob = take(at, (size_t)p.m * p.lda);
     const size_t op = p.z > 1 ? take(at, (size_t)p.z * tri * kT * kT * sizeof(float)) : 0, on = take(at, (size_t)p.norm_blocks * sizeof(double));
     p.x[0] = base + ox0;

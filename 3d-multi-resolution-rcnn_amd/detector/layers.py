@@ -219,78 +219,12 @@ def linear(x, weight, bias=None, relu=False, impl=None):
     return y5.permute(0, 2, 3, 4, 1).reshape(rp, weight.shape[0])[:R]
 
 
-LAYER_NORM_MAX_COLS = 16384
-
-
-def _rows_view(t, cols):
-    """[rows, cols] with a contiguous last axis: a view where the strides allow it, else a copy.  (A one-column view may carry any
-    last stride, a one-row view any row stride.)"""
-    t = t.reshape(-1, cols)
-    return t if (t.stride(1) == 1 or cols == 1 and t.stride(0) == 1) and t.stride(0) >= 0 else t.contiguous()
-
-
-class _LayerNormFn(Function):
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        cols = x.shape[-1]
-        xr = _rows_view(x.detach(), cols)
-        w = weight.detach().contiguous() if weight is not None else None
-        b = bias.detach().contiguous() if bias is not None else None
-        train = any(ctx.needs_input_grad[:3])
-        if xr.shape[0] == 0:
-            y, stats = torch.empty_like(xr), None
-        else:
-            y, stats = _hip.layer_norm_forward(xr, w, b, eps, train)
-        if train:
-            # x itself is saved as the autograd input it is (its version is checked), the row view is made again in backward
-            ctx.save_for_backward(x, weight, stats)
-            ctx.param_dtype = (weight if weight is not None else bias).dtype if weight is not None or bias is not None else x.dtype
-        return y.reshape(x.shape)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        x, weight, stats = ctx.saved_tensors
-        cols = x.shape[-1]
-        xr = _rows_view(x.detach(), cols)
-        want_x, want_w, want_b = ctx.needs_input_grad[:3]
-        if xr.shape[0] == 0:
-            zero = lambda want: torch.zeros((cols,), dtype=ctx.param_dtype, device=x.device) if want else None
-            return (torch.empty_like(x) if want_x else None), zero(want_w), zero(want_b), None
-        w = weight.detach().contiguous() if weight is not None else None
-        dx, dw, db = _hip.layer_norm_backward(xr, _rows_view(g, cols), w, stats, ctx.param_dtype, want_x, want_w, want_b)
-        return (dx.reshape(x.shape) if want_x else None), dw, db, None
-
-
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Layer norm over the last axis (csrc/norm.hip): (x - mean) / sqrt(var + eps) * weight + bias, differentiable in x, weight and bias.
     x [..., C], fp32 or bf16, on the GPU; weight / bias [C] in x's type or (both) in fp32; C <= 16384.  Rows may be strided as long as the
     last axis is contiguous (the voxels of a channels_last_3d map: `m.permute(0, 2, 3, 4, 1)` needs no copy); the result is contiguous, in x's
     type.  Statistics and sums are fp32; the parameter gradients are summed in a fixed order (bit-reproducible)."""
-    if not torch.is_tensor(x) or x.dim() < 1:
-        raise TypeError('layer_norm: x is a tensor [..., C]')
-    if x.dtype not in _hip.STORAGE_DTYPES:
-        raise TypeError(f'layer_norm: x is float32 or bfloat16, got {x.dtype}')
-    cols = x.shape[-1]
-    if not 1 <= cols <= LAYER_NORM_MAX_COLS:
-        raise NotImplementedError(f'layer_norm: 1 to {LAYER_NORM_MAX_COLS} columns, got {cols}')
-    if not float(eps) >= 0:
-        raise ValueError(f'layer_norm: eps is at least 0, got {eps}')
-    types = set()
-    for name, p in (('weight', weight), ('bias', bias)):
-        if p is None:
-            continue
-        if tuple(p.shape) != (cols,) or p.device != x.device:
-            raise ValueError(f'layer_norm: {name} is [{cols}] on {x.device}, got {tuple(p.shape)} on {p.device}')
-        if p.dtype not in (torch.float32, x.dtype):
-            raise TypeError(f'layer_norm: {name} is float32 or {x.dtype}, got {p.dtype}')
-        types.add(p.dtype)
-    if len(types) > 1:
-        raise TypeError('layer_norm: weight and bias have one type')
-    if not x.is_cuda:
-        raise NotImplementedError('layer_norm has no CPU fallback')
-    return _LayerNormFn.apply(x, weight, bias, float(eps))
+    return _hip.train_ops().layer_norm(x, weight, bias, eps)
 
 
 class _Deconv2Fn(Function):

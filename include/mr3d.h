@@ -540,7 +540,7 @@ int mr3d_layer_norm_backward(const void *x, long long x_stride, const void *dy, 
  * fp32 products carry 22 bits of each factor, bf16 gradients of the logits are rounded to bf16 once more; sums are fp32 or wider, in a
  * fixed order.  hidden <= 65536, classes <= 2^20, rows <= 2^22.  workspace: 1024-byte aligned device memory of
  * mr3d_linear_cross_entropy_workspace_bytes (0 = refused; the exponentials in it are bounded by 2 GiB, rows go through in pieces).
- * mr3d_scale_by: data *= *factor_dev in place; nothing is touched when the factor is 1.
+ * mr3d_scale_by: up to 4 arrays *= *factor_dev in place, in one launch; nothing is touched when the factor is 1.
  * ---------------------------------------------------------------------------------------------- */
 typedef struct {
   const void *x, *weight, *bias;
@@ -555,7 +555,12 @@ typedef struct {
 } mr3d_linear_ce;
 size_t mr3d_linear_cross_entropy_workspace_bytes(const mr3d_linear_ce *args_host);
 int mr3d_linear_cross_entropy(const mr3d_linear_ce *args_host, void *workspace, size_t workspace_bytes, mr3d_stream_t s);
-int mr3d_scale_by(void *data, long long count, int dtype, const float *factor_dev, mr3d_stream_t s);
+typedef struct {
+  void *data;
+  long long count;
+  int dtype, reserved;
+} mr3d_span;
+int mr3d_scale_by(const mr3d_span *spans_host, int num_spans, const float *factor_dev, mr3d_stream_t s);
 
 /* ------------------------------------------------------------------------------------------------
  * Orthogonalised updates of a list of matrices by Newton-Schulz products (csrc/ortho.hip); not part of the reference, whose optimiser is SGD.

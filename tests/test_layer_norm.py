@@ -144,6 +144,20 @@ def test_rows_of_nan_and_infinity_stay_in_their_rows():
 
 
 @pytest.mark.gpu
+def test_second_derivatives_are_refused_and_a_changed_input_is_noticed():
+    from mr3d_amd.detector.layers import layer_norm
+    x = torch.randn(4, 8, device='cuda', requires_grad=True)
+    (g,) = torch.autograd.grad(layer_norm(x).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match='second derivatives'):
+        g.sum().backward()
+    h = x * 1
+    y = layer_norm(h)
+    h.add_(1)
+    with pytest.raises(RuntimeError, match='modified by an inplace'):
+        y.sum().backward()
+
+
+@pytest.mark.gpu
 def test_no_rows():
     from mr3d_amd.detector.layers import layer_norm
     x = torch.zeros(0, 32, device='cuda', requires_grad=True)
@@ -176,12 +190,13 @@ def test_gradient_against_differences():
 
 @pytest.mark.gpu
 def test_same_bits_every_run_on_another_stream_and_in_a_graph():
-    from mr3d_amd import _hip
+    from mr3d_amd.detector.layers import layer_norm
     x, w, b, dy = (t.cuda() for t in _inputs(3000, 96, torch.bfloat16, torch.float32))
 
     def both():
-        y, stats = _hip.layer_norm_forward(x, w, b, 1e-5, True)
-        return (y,) + _hip.layer_norm_backward(x, dy, w, stats, torch.float32, True, True, True)
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        y = layer_norm(*leaves)
+        return (y.detach(),) + torch.autograd.grad(y, leaves, dy)
 
     first = both()
     assert all(torch.equal(p, q) for p, q in zip(first, both()))
@@ -202,8 +217,7 @@ def test_same_bits_every_run_on_another_stream_and_in_a_graph():
 
 
 def test_refusals_need_no_gpu():
-    import ctypes
-    import mr3d_amd
+    from abi import lib
     from mr3d_amd.detector.layers import layer_norm
     x = torch.zeros(4, 8)
     with pytest.raises(NotImplementedError):
@@ -222,7 +236,7 @@ def test_refusals_need_no_gpu():
         layer_norm(torch.zeros(1, 16385))
     with pytest.raises(NotImplementedError):
         layer_norm(torch.zeros(3, 0))
-    L = mr3d_amd._hip.lib()
+    L = lib()
     p = 64                                                    # never read: every call below is refused on the host
     assert L.mr3d_layer_norm_forward(None, 8, p, p, p, p, p, 4, 8, 1e-5, 0, 0, None) == 1
     assert L.mr3d_layer_norm_forward(p, 8, p, p, p, p, None, 4, 8, 1e-5, 0, 0, None) == 1

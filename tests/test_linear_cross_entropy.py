@@ -264,10 +264,15 @@ def test_gradient_against_differences():
 
 @pytest.mark.gpu
 def test_same_bits_every_run_on_another_stream_and_in_a_graph():
-    from mr3d_amd import _hip
+    from mr3d_amd.core import linear_cross_entropy
     for dtype in (torch.float32, torch.bfloat16):
         x, w, b, label, rw = (t.cuda() for t in _inputs(300, 256, 900, dtype))
-        both = lambda: _hip.linear_cross_entropy(x, w, b, label, rw, None, None, -100, True, True, True)
+
+        def both():
+            leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+            loss = linear_cross_entropy(leaves[0], leaves[1], label, rw, bias=leaves[2])
+            return (loss.detach(),) + torch.autograd.grad(loss, leaves)
+
         first = both()
         assert all(torch.equal(p, q) for p, q in zip(first, both()))
         side = torch.cuda.Stream()
@@ -319,8 +324,7 @@ def test_no_rows():
 
 def test_refusals_need_no_gpu():
     import ctypes
-    import mr3d_amd
-    from mr3d_amd import _hip
+    from abi import LinearCe, Span, lib
     from mr3d_amd.core import linear_cross_entropy as ce
     x, w, lab = torch.zeros(4, 8), torch.zeros(10, 8), torch.zeros(4, dtype=torch.int64)
     with pytest.raises(NotImplementedError):
@@ -338,10 +342,10 @@ def test_refusals_need_no_gpu():
         ce(x, torch.zeros(1, 8).expand((1 << 20) + 1, 8), lab)
     with pytest.raises(NotImplementedError):
         ce(x, w, lab, torch.ones(4, requires_grad=True))
-    L = mr3d_amd._hip.lib()
+    L = lib()
     base = dict(x=1024, weight=1024, bias=1024, labels=1024, loss=1024, dx=1024, dweight=1024, dbias=1024, x_stride=8, weight_stride=8, ignore_index=-100,
                 rows=4, hidden=8, classes=10, dtype=0, param_dtype=0, want_dx=1, want_dweight=1, want_dbias=1)
-    mk = lambda **kw: ctypes.byref(_hip.LinearCe(**{**base, **kw}))
+    mk = lambda **kw: ctypes.byref(LinearCe(**{**base, **kw}))
     need = L.mr3d_linear_cross_entropy_workspace_bytes(mk())
     call = lambda ws=1024, by=need, **kw: L.mr3d_linear_cross_entropy(mk(**kw), ws, by, None)
     assert need > 0
@@ -352,5 +356,8 @@ def test_refusals_need_no_gpu():
                dict(rows=(1 << 22) + 1)):
         assert call(**kw) == 4, kw
     assert call(ws=None) == 2 and call(ws=1032) == 2 and call(by=need - 1) == 2
-    assert L.mr3d_scale_by(None, 4, 0, 1024, None) == 1 and L.mr3d_scale_by(1024, 4, 0, None, None) == 1 and L.mr3d_scale_by(1024, 4, 2, 1024, None) == 4
-    assert L.mr3d_scale_by(1024, 0, 0, 1024, None) == 0
+    span = lambda *a: (Span * 1)(Span(*a))
+    assert L.mr3d_scale_by(None, 1, 1024, None) == 1 and L.mr3d_scale_by(span(1024, 4, 0), 1, None, None) == 1
+    assert L.mr3d_scale_by(span(1024, 4, 0), 0, 1024, None) == 1 and L.mr3d_scale_by(span(1024, 4, 0), 5, 1024, None) == 1
+    assert L.mr3d_scale_by(span(None, 4, 0), 1, 1024, None) == 1 and L.mr3d_scale_by(span(1024, 4, 2), 1, 1024, None) == 4
+    assert L.mr3d_scale_by(span(1024, 0, 0), 1, 1024, None) == 0

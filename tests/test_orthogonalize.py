@@ -146,8 +146,7 @@ def test_other_stream_and_replayed_graph():
 
 
 def test_refusals_need_no_gpu():
-    import mr3d_amd
-    from mr3d_amd import _hip
+    from abi import Matrix, lib
     from mr3d_amd.core import orthogonalize
     g = torch.zeros(4, 8)
     with pytest.raises(NotImplementedError):
@@ -161,8 +160,8 @@ def test_refusals_need_no_gpu():
             orthogonalize(g, **kw)
     with pytest.raises(NotImplementedError):
         orthogonalize(torch.zeros(1, 1).expand(1, (1 << 20) + 1))
-    L = mr3d_amd._hip.lib()
-    mk = lambda **kw: (_hip.Matrix * 1)(_hip.Matrix(**{**dict(in_=256, out=256, rows=4, cols=8, in_row_stride=8, in_col_stride=1, dtype=0), **kw}))
+    L = lib()
+    mk = lambda **kw: (Matrix * 1)(Matrix(**{**dict(in_=256, out=256, rows=4, cols=8, in_row_stride=8, in_col_stride=1, dtype=0), **kw}))
     need = L.mr3d_orthogonalize_workspace_bytes(mk(), 1)
     call = lambda t, n=1, steps=5, a=1.0, eps=0.0, ws=256, by=need: L.mr3d_orthogonalize(t, n, steps, a, 0.0, 0.0, eps, ws, by, None)
     assert need > 0 and need % 256 == 0
