@@ -578,10 +578,14 @@ __global__ __launch_bounds__(256) void ce_scale_kernel(Spans spans, const float 
 // Tiles.  256 x 256 (8 waves of 128 x 64, one workgroup a CU) has the fewest LDS bytes per product; it needs enough tiles to fill 256 CUs.
 // 128 x 128 (4 waves of 64 x 64, two workgroups a CU) below that.
 template <bool IKS, bool JKS, bool SPLIT> struct Tiles {
-  typedef Tile<256, 256, 2, 4, IKS, JKS, SPLIT, 128, 2> Large;
   typedef Tile<128, 128, 2, 2, IKS, JKS, SPLIT, 128, 2> Small;
+  typedef Tile<256, 256, 2, 4, IKS, JKS, SPLIT, 128, 2> Large;
 };
-bool large_tiles(long long i, long long j, long long z) { return ((i + 255) / 256) * ((j + 255) / 256) * z >= 192; }
+template <bool IKS, bool JKS> struct Tiles<IKS, JKS, true> {               // no room for two sets of accumulators in the large tile
+  typedef Tile<128, 128, 2, 2, IKS, JKS, true, 128, 2> Small;
+  typedef Small Large;
+};
+bool large_tiles(bool f32, long long i, long long j) { return !f32 && ((i + 255) / 256) * ((j + 255) / 256) >= 192; }
 
 long long up(long long v, long long a) { return (v + a - 1) / a * a; }
 
@@ -620,7 +624,7 @@ int layout_of(const mr3d_linear_ce *a, Layout &l) {
     l.chunks = (int)((a->rows + cap - 1) / cap);
   }
   l.cap = (int)cap;
-  l.big_logits = large_tiles(a->classes, cap, 1);
+  l.big_logits = large_tiles(f32, a->classes, cap);
   l.wcols = l.big_logits ? 128 : 64;
   l.pieces = (int)(up(a->classes, l.big_logits ? 256 : 128) / l.wcols);
   l.head = take(at, 64);
@@ -637,7 +641,7 @@ int layout_of(const mr3d_linear_ce *a, Layout &l) {
     // parts over the classes until two workgroups a CU have work; a part keeps 16 k-steps
     const long long tiles = ((a->hidden + 127) / 128) * ((cap + 127) / 128), steps = l.ldg / 128;
     long long z = tiles >= 512 ? 1 : 512 / tiles;
-    if (large_tiles(a->hidden, cap, 1)) z = 1;
+    if (large_tiles(f32, a->hidden, cap)) z = 1;
     if (z > steps / 16) z = steps / 16;
     l.z = (int)(z < 1 ? 1 : z);
     l.part = take(at, (size_t)l.z * cap * up(a->hidden, 4) * 4);
@@ -700,13 +704,13 @@ template <bool F32> int run_ce(const mr3d_linear_ce *a, const Layout &l, Ce &c, 
     }
     if (e) return e;
     if (a->want_dx) {
-      e = large_tiles(a->hidden, l.cap, l.z) && l.z == 1 ? launch_dx<typename TX::Large>(c, row0, q) : launch_dx<typename TX::Small>(c, row0, q);
+      e = large_tiles(F32, a->hidden, l.cap) ? launch_dx<typename TX::Large>(c, row0, q) : launch_dx<typename TX::Small>(c, row0, q);
       if (e) return e;
       ce_dx_rows_kernel<F32><<<a->rows, 256, 0, q>>>(c, row0);
     }
     if (a->want_dweight) {
       const int mode = k ? 2 : (l.chunks > 1 ? 1 : 0);
-      e = large_tiles(a->hidden, a->classes, 1) ? launch_dw<typename TW::Large>(c, row0, mode, q) : launch_dw<typename TW::Small>(c, row0, mode, q);
+      e = large_tiles(F32, a->hidden, a->classes) ? launch_dw<typename TW::Large>(c, row0, mode, q) : launch_dw<typename TW::Small>(c, row0, mode, q);
       if (e) return e;
     }
     if (a->want_dbias) ce_db_kernel<F32><<<dim3((a->classes + 255) / 256, (l.cap + kDbRows - 1) / kDbRows), 256, 0, q>>>(c, row0);

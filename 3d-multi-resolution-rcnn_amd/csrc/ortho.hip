@@ -1,12 +1,18 @@
 // Orthogonalised updates: Newton-Schulz products of a LIST of matrices, all of them in one launch per stage.
-//   X = G / (|G|_F + eps), wide (m <= n; a tall G is read transposed);  steps times:
-//     A = X X^T          B = a I + b A + c A A          X = B X
-// (a I sits inside B, so the third product needs no second read of X).  A and A A are symmetric: only the tiles on and below the diagonal are computed
-// and stored twice.
-// Every factor is kept as two fp16 planes (gemm16.h, split storage), scaled by powers of two into fp16's range: 22 bits, three passes of the
-// 16-bit matrix pipe, fp32 accumulators.  Plain bf16 or fp16 factors would lose 2e-2 / 2e-3 of the result over five steps (the
-// polynomial's slope at 0 is a = 3.4: rounding errors of the first steps are amplified a few hundred times).
-// MFMA-bound on large matrices; on small ones the 4 dependent launches of a step are what counts, hence the list.
+//   X = G / (|G|_F + eps), wide (m <= n; a tall G is read transposed);  steps times:  A = X X^T,  P = a I + b A + c A A,  X = P X
+//
+// Up to 64 rows (small path): three launches.  The iteration is a function of A alone, X = Q(A) G, so A is formed once in DOUBLE, all steps run
+// on the m x m matrices in one workgroup's LDS (A <- P A P, Q <- P Q: polynomials of A commute, products of them are symmetric), and Q is applied
+// once.  Double, because the noise of A is amplified by a^2 a step where singular values are small: fp32 loses 1e-5 .. 1e-4 over five steps.
+// It also gives |G|_F = sqrt(trace A) without overflow.
+//
+// Larger ones: every factor is kept as two fp16 planes (gemm16.h, split storage), scaled by powers of two into fp16's range: 22 bits, three passes
+// of the 16-bit matrix pipe, fp32 accumulators.  Plain bf16 or fp16 factors would lose 2e-2 / 2e-3 of the result over five steps (p's slope at 0
+// is a = 3.4: rounding errors of the first steps are amplified a few hundred times).  Symmetric results: only the tiles on and below the diagonal are
+// computed and stored twice.  Iterating on A here too, in rounds of two or three steps between looks at X, was measured: 1.6 to 2.4 times fewer
+// products at n = 9 m, but no less time (940 us for the 64 matrices of a detector either way: the m x m products are short) and A's noise, amplified,
+// takes the result from 1.0e-6 to 2.5e-6 (two steps) or 5e-6 (three) where plain fp32 loses 1.6e-6.
+// MFMA-bound on large matrices; on small ones the dependent launches are what counts, hence the list and the small path.
 #include "gemm16.h"
 #include <new>
 
@@ -14,29 +20,38 @@ using namespace gemm16;
 
 namespace {
 
-// powers of two that bring X, A and B into fp16's range: |X| < 16, |A| < 16, |B| < 64
-constexpr float kSX = 4096.f, kSA = 4096.f, kSB = 1024.f;
-constexpr int kT = 128;                                     // tile of every product
-typedef Tile<kT, kT, 2, 2, false, false, true, 128, 2> TileGram;
-typedef Tile<kT, kT, 2, 2, true, false, true, 128, 2> TileApply;
-constexpr int kThreads = TileGram::THREADS;
+// powers of two that bring X, A and P into fp16's range: |X| < 16, |A| < 16, |P| < 64
+constexpr float kSX = 4096.f, kSA = 4096.f, kSP = 1024.f;
+constexpr int kSmall = 64;                                  // rows of the small path
+constexpr int kThreads = 256;
 
-enum Stage { kNorm, kPack, kGram, kReduce, kPoly, kApply, kStages };
+// 128 x 128 with two tiles in LDS, or 64 x 64 with four, two workgroups a CU each
+template <int BT, bool APPLY, bool FINE> struct Pick { typedef Tile<BT, BT, 2, 2, APPLY, false, true, 128, BT == 128 ? 2 : 4, FINE> T; };
+
+enum Stage { kNorm, kPack, kGram, kGramJoin, kSquare, kSquareJoin, kApply, kApplyJoin, kSmallGram, kSmallPoly, kSmallApply, kStages };
+enum Buf { kA, kP, kX0, kX1, kBufs };
+
+// tiles [0, whole) are computed by one workgroup each, the others by z workgroups with a share of the k-steps; their parts are joined afterwards
+struct Split { int tiles, whole, z; };
 
 struct Mat {
   const char *in;
   char *out;
   long long in_i, in_j, out_i, out_j;                       // element strides along n (i) and m (j)
-  char *x[2], *a, *b;                                       // planes: [m][ldx], [m][ldx], [m][lda], [m][lda]
-  float *part;                                              // [z][tiles][kT * kT]
-  double *norm;
+  char *buf[kBufs];                                         // planes
+  float *part;                                              // parts of split tiles, [tile - whole][z][BT * BT]
+  double *norm;                                             // small path: parts of A, [z][mp][mp], then Q
   int m, n, ldx, lda;                                       // ld in bytes
-  int z, bf16, norm_blocks, pad;
+  int bf16, norm_blocks;
+  Split gram, square, apply;
   int first[kStages];                                       // first workgroup of this matrix in each stage
 };
+static_assert(sizeof(Mat) <= 240, "sixteen of them are kernel arguments");
 
 struct Plan {
   int blocks[kStages];
+  int bt_square, bt_gram, bt_apply;
+  bool fine;
   size_t bytes, mats_off, map_off[kStages];
 };
 
@@ -121,6 +136,28 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(const Mat *__restrict__
   if (threadIdx.x == 0) p.norm[chunk] = w[0] + w[1] + w[2] + w[3];
 }
 
+constexpr int kChunk = 64;                                  // columns of X in LDS
+
+// rows [0, 64) x columns [i0, i0 + 64) of the wide matrix, zeros outside -> t[row][col]; read along the contiguous axis, 16 loads a thread in flight
+__device__ __forceinline__ void load_tile(const Mat *__restrict__ p, int i0, int j0, float (*t)[kChunk + 1]) {
+  const long long si = p->in_i, sj = p->in_j;
+  const bool wide = si == 1;
+  const int fast = threadIdx.x & 63, slow = threadIdx.x >> 6, m = p->m - j0, n = p->n - i0;
+  const long long base = i0 * si + j0 * sj;
+  float v[16];
+  auto each = [&](auto *in) {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const int q = wide ? fast : slow + 4 * k, r = wide ? slow + 4 * k : fast;
+      v[k] = q < n && r < m ? (float)in[base + q * si + r * sj] : 0.f;
+    }
+  };
+  if (p->bf16) each((const __bf16 *)p->in);
+  else each((const float *)p->in);
+#pragma unroll
+  for (int k = 0; k < 16; ++k) t[wide ? slow + 4 * k : fast][wide ? fast : slow + 4 * k] = v[k];
+}
+
 // 64 x 64 of the input -> planes of X; the tile goes through LDS so that a tall input is read along its rows too
 __global__ __launch_bounds__(256) void ortho_pack_kernel(const Mat *__restrict__ mats, const int *__restrict__ map, float eps) {
   __shared__ float t[64][65];
@@ -133,12 +170,7 @@ __global__ __launch_bounds__(256) void ortho_pack_kernel(const Mat *__restrict__
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
   if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = s;
-  const bool wide = p.in_i == 1;
-  for (int k = threadIdx.x; k < 4096; k += 256) {
-    const int q = k & 63, r = k >> 6;
-    const int i = wide ? q : r, j = wide ? r : q;
-    t[j][i] = (i0 + i < p.n && j0 + j < p.m) ? read_in(p, (i0 + i) * p.in_i + (j0 + j) * p.in_j) : 0.f;
-  }
+  load_tile(mats + map[blockIdx.x], i0, j0, t);
   __syncthreads();
   const double scale = (double)kSX / (sqrt(w[0] + w[1] + w[2] + w[3]) + (double)eps);      // may leave fp32's range where G does not
   const int np = (p.n + 31) / 32 * 32;
@@ -148,7 +180,7 @@ __global__ __launch_bounds__(256) void ortho_pack_kernel(const Mat *__restrict__
     _Float16 h[4], l[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) split16((float)((double)t[j][i + e] * scale), h[e], l[e]);
-    char *d = p.x[0] + (long long)(j0 + j) * p.ldx + (i0 + i) / 32 * 128 + (i & 31) * 2;
+    char *d = p.buf[kX0] + (long long)(j0 + j) * p.ldx + (i0 + i) / 32 * 128 + (i & 31) * 2;
     *reinterpret_cast<uint2 *>(d) = *reinterpret_cast<uint2 *>(h);
     *reinterpret_cast<uint2 *>(d + 64) = *reinterpret_cast<uint2 *>(l);
   }
@@ -171,151 +203,347 @@ __device__ __forceinline__ void load_planes(const char *row, int i, float (&v)[4
   for (int e = 0; e < 4; ++e) v[e] = (float)hh[e] + (float)ll[e];
 }
 
-// 32 x 32 block (bi, bj) of a tile of a symmetric result: rows j of tile tj, columns i of tile ti, and mirrored off the diagonal.
-// POLY: a I + b A + c acc instead of acc
-template <bool POLY>
-__device__ __forceinline__ void store_symmetric_block(const Mat &p, char *dst, int ti, int tj, int bi, int bj, const f32x16 &acc, float ca, float cb, float cc) {
-  const int lane = threadIdx.x & 63, mp = (p.m + 31) / 32 * 32;
-  const int j = tj * kT + bj * 32 + (lane & 31);
+// The three products of a step.  kind 0: A = X X^T.  1: P = a I + b A + c A A (symmetric too; alpha acc + beta A + gamma I in raw plane values).
+// 2: alpha P X, to planes or (last) to the caller's matrix
+struct Op {
+  int x;                                                    // buffer of X
+  float alpha, beta, gamma;
+  int last;
+};
+
+// 32 x 32 block (bi, bj) of tile (ti, tj), one accumulator of a wave
+template <int KIND, int BT>
+__device__ __forceinline__ void finish_block(const Mat *__restrict__ mat, const Op &op, int ti, int tj, int bi, int bj, const f32x16 &acc) {
+  const int lane = threadIdx.x & 63, m = mat->m;
+  const int j = tj * BT + bj * 32 + (lane & 31);
+  if constexpr (KIND < 2) {
+    const int mp = (m + 31) / 32 * 32, lda = mat->lda;
+    char *dst = mat->buf[KIND == 0 ? kA : kP];
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const int i = ti * kT + bi * 32 + g * 8 + (lane >> 5) * 4;
-    float v[4];
-    if constexpr (POLY) {
-      float f[4] = {0.f, 0.f, 0.f, 0.f};
-      if (j < p.m && i < mp) load_planes(p.a + (long long)j * p.lda, i, f);
+    for (int g = 0; g < 4; ++g) {
+      const int i = ti * BT + bi * 32 + g * 8 + (lane >> 5) * 4;
+      float v[4];
+      if constexpr (KIND == 0) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float t = cc * (acc[g * 4 + e] * (1.f / (kSA * kSA))) + cb * (f[e] * (1.f / kSA));
-        v[e] = (t + (i + e == j ? ca : 0.f)) * kSB;
+        for (int e = 0; e < 4; ++e) v[e] = op.alpha * acc[g * 4 + e];
+      } else {
+        float f[4] = {0.f, 0.f, 0.f, 0.f};
+        if (j < m && i < mp) load_planes(mat->buf[kA] + (long long)j * lda, i, f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = op.alpha * acc[g * 4 + e] + op.beta * f[e] + (i + e == j ? op.gamma : 0.f);
       }
-    } else {
+      if (j < m && i < mp) store_planes(dst + (long long)j * lda, i, v);
+      if (ti != tj && j < mp) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = acc[g * 4 + e] * (kSA / (kSX * kSX));
+        for (int e = 0; e < 4; ++e)
+          if (i + e < m) {
+            _Float16 h, l;
+            split16(v[e], h, l);
+            _Float16 *d = reinterpret_cast<_Float16 *>(dst + (long long)(i + e) * lda + (j >> 5) * 128) + (j & 31);
+            d[0] = h;
+            d[32] = l;
+          }
+      }
     }
-    if (j < p.m && i < mp) store_planes(dst + (long long)j * p.lda, i, v);
-    if (ti != tj && j < mp) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (i + e < p.m) {
-          _Float16 h, l;
-          split16(v[e], h, l);
-          _Float16 *d = reinterpret_cast<_Float16 *>(dst + (long long)(i + e) * p.lda + (j >> 5) * 128) + (j & 31);
-          d[0] = h;
-          d[32] = l;
-        }
-    }
-  }
-}
-
-template <bool POLY>
-__device__ __forceinline__ void store_symmetric(const Mat &p, char *dst, int ti, int tj, const f32x16 (&acc)[2][2], float ca, float cb, float cc) {
-  const int wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int a = 0; a < 2; ++a)
-#pragma unroll
-    for (int b = 0; b < 2; ++b) store_symmetric_block<POLY>(p, dst, ti, tj, (wave & 1) * 2 + a, (wave >> 1) * 2 + b, acc[a][b], ca, cb, cc);
-}
-
-__global__ __launch_bounds__(kThreads, 2) void ortho_gram_kernel(const Mat *__restrict__ mats, const int *__restrict__ map, int cur) {
-  extern __shared__ __attribute__((aligned(1024))) char lds[];
-  const Mat p = mats[map[blockIdx.x]];
-  const int local = blockIdx.x - p.first[kGram];
-  int ti;
-  const int t = local / p.z, zi = local % p.z, tj = triangle(t, ti);
-  const int total = (p.n + 31) / 32;
-  const int s0 = (int)((long long)total * zi / p.z), s1 = (int)((long long)total * (zi + 1) / p.z);
-  const char *x = cur ? p.x[1] : p.x[0];
-  f32x16 acc[2][2];
-  run<TileGram>(lds, side_kc<TileGram>(x, p.ldx, p.m, p.ldx, ti * kT, s0), side_kc<TileGram>(x, p.ldx, p.m, p.ldx, tj * kT, s0), s1 - s0, acc);
-  if (p.z == 1) {
-    store_symmetric<false>(p, p.a, ti, tj, acc, 0.f, 0.f, 0.f);
   } else {
-    const int tm = (p.m + kT - 1) / kT;
-    float *d = p.part + ((long long)zi * (tm * (tm + 1) / 2) + t) * (kT * kT) + threadIdx.x;
+    if (j >= m) return;
+    const int n = mat->n, np = (n + 31) / 32 * 32;
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+    for (int g = 0; g < 4; ++g) {
+      const int i = ti * BT + bi * 32 + g * 8 + (lane >> 5) * 4;
+      float v[4];
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+      for (int e = 0; e < 4; ++e) v[e] = acc[g * 4 + e] * op.alpha;
+      if (!op.last) {
+        if (i < np) store_planes(mat->buf[op.x == kX0 ? kX1 : kX0] + (long long)j * mat->ldx, i, v);
+      } else {
+        const long long oj = mat->out_j, oi = mat->out_i;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) d[((a * 2 + b) * 16 + e) * kThreads] = acc[a][b][e];
+        for (int e = 0; e < 4; ++e)
+          if (i + e < n) {
+            const long long at = j * oj + (i + e) * oi;
+            if (mat->bf16) ((__bf16 *)mat->out)[at] = (__bf16)v[e];
+            else ((float *)mat->out)[at] = v[e];
+          }
+      }
+    }
   }
 }
 
-// the parts of a split Gram tile, added in a fixed order; a workgroup takes one of the four 32 x 32 blocks of every wave
-__global__ __launch_bounds__(kThreads) void ortho_reduce_kernel(const Mat *__restrict__ mats, const int *__restrict__ map) {
-  const Mat p = mats[map[blockIdx.x]];
-  const int local = blockIdx.x - p.first[kReduce], t = local >> 2, q = local & 3;
-  int ti;
-  const int tj = triangle(t, ti), tm = (p.m + kT - 1) / kT;
-  const long long stride = (long long)(tm * (tm + 1) / 2) * (kT * kT);
-  const float *s = p.part + (long long)t * (kT * kT) + q * 16 * kThreads + threadIdx.x;
+template <int KIND> __device__ __forceinline__ Split split_of(const Mat *__restrict__ m) { return KIND == 0 ? m->gram : KIND == 1 ? m->square : m->apply; }
+
+template <int KIND, int BT>
+__device__ __forceinline__ void tile_at(const Mat *__restrict__ mat, int t, int &ti, int &tj) {
+  if constexpr (KIND < 2) {
+    tj = triangle(t, ti);
+  } else {
+    const int tm = (mat->m + BT - 1) / BT;
+    tj = t % tm;
+    ti = t / tm;
+  }
+}
+
+template <int KIND, int BT, bool FINE>
+__global__ __launch_bounds__(kThreads, 2) void ortho_product_kernel(const Mat *__restrict__ mats, const int *__restrict__ map, Op op) {
+  typedef typename Pick<BT, KIND == 2, FINE>::T T;
+  constexpr int kFirst = KIND == 0 ? kGram : KIND == 1 ? kSquare : kApply;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int b = blockIdx.x;
+  const Mat *__restrict__ mat = mats + map[b];
+  const Split sp = split_of<KIND>(mat);
+  const int local = b - mat->first[kFirst], m = mat->m;
+  int t = local, zi = 0, z = 1;
+  if (local >= sp.whole) {
+    z = sp.z;
+    t = sp.whole + (local - sp.whole) / z;
+    zi = (local - sp.whole) % z;
+  }
+  int ti, tj;
+  tile_at<KIND, BT>(mat, t, ti, tj);
+  const int total = ((KIND == 0 ? mat->n : m) + 31) / 32;
+  const int s0 = (int)((long long)total * zi / z), s1 = (int)((long long)total * (zi + 1) / z);
+  const int ldl = KIND == 1 ? mat->lda : mat->ldx, ldr = KIND == 0 ? mat->ldx : mat->lda;
+  const char *l = mat->buf[KIND == 1 ? kA : op.x], *r = mat->buf[KIND == 0 ? op.x : KIND == 1 ? kA : kP];
+  f32x16 acc[T::TI][T::TJ];
+  if constexpr (KIND == 2) run<T>(lds, side_ks<T>(l, ldl, m, ldl, (long long)ti * BT * 4, s0), side_kc<T>(r, ldr, m, ldr, tj * BT, s0), s1 - s0, acc);
+  else run<T>(lds, side_kc<T>(l, ldl, m, ldl, ti * BT, s0), side_kc<T>(r, ldr, m, ldr, tj * BT, s0), s1 - s0, acc);
+  const int wave = threadIdx.x >> 6, wi = wave % T::NWI, wj = wave / T::NWI;
+  if (z == 1) {
+#pragma unroll
+    for (int x = 0; x < T::TI; ++x)
+#pragma unroll
+      for (int y = 0; y < T::TJ; ++y) finish_block<KIND, BT>(mat, op, ti, tj, wi * T::TI + x, wj * T::TJ + y, acc[x][y]);
+  } else {
+    float *d = mat->part + ((long long)(t - sp.whole) * z + zi) * (BT * BT) + threadIdx.x;
+#pragma unroll
+    for (int x = 0; x < T::TI; ++x)
+#pragma unroll
+      for (int y = 0; y < T::TJ; ++y)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) d[((x * T::TJ + y) * 16 + e) * kThreads] = acc[x][y][e];
+  }
+}
+
+// the parts of split tiles, added in a fixed order; a workgroup takes one 32 x 32 block of every wave
+template <int KIND, int BT>
+__global__ __launch_bounds__(kThreads) void ortho_join_kernel(const Mat *__restrict__ mats, const int *__restrict__ map, Op op) {
+  typedef typename Pick<BT, KIND == 2, false>::T T;
+  constexpr int kFirst = KIND == 0 ? kGramJoin : KIND == 1 ? kSquareJoin : kApplyJoin, Q = T::TI * T::TJ;
+  const int b = blockIdx.x;
+  const Mat *__restrict__ mat = mats + map[b];
+  const Split sp = split_of<KIND>(mat);
+  const int local = b - mat->first[kFirst], u = local / Q, q = local % Q;
+  int ti, tj;
+  tile_at<KIND, BT>(mat, sp.whole + u, ti, tj);
+  const float *s = mat->part + (long long)u * sp.z * (BT * BT) + q * 16 * kThreads + threadIdx.x;
   f32x16 acc;
 #pragma unroll
   for (int e = 0; e < 16; ++e) acc[e] = s[e * kThreads];
-  for (int zi = 1; zi < p.z; zi += 2) {                     // 32 loads in flight
-    const float *s1 = s + zi * stride, *s2 = zi + 1 < p.z ? s1 + stride : s1;
-    const float keep = zi + 1 < p.z ? 1.f : 0.f;
-    float u[16], v[16];
+  for (int zi = 1; zi < sp.z; zi += 2) {                    // 32 loads in flight
+    const float *s1 = s + (long long)zi * (BT * BT);
+    const bool two = zi + 1 < sp.z;
+    const float *s2 = two ? s1 + BT * BT : s1;
+    float x[16], y[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      u[e] = s1[e * kThreads];
-      v[e] = s2[e * kThreads];
+      x[e] = s1[e * kThreads];
+      y[e] = s2[e * kThreads];
     }
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      acc[e] += u[e];
-      if (keep != 0.f) acc[e] += v[e];
+      acc[e] += x[e];
+      if (two) acc[e] += y[e];
     }
   }
-  const int wave = threadIdx.x >> 6;
-  store_symmetric_block<false>(p, p.a, ti, tj, (wave & 1) * 2 + (q >> 1), (wave >> 1) * 2 + (q & 1), acc, 0.f, 0.f, 0.f);
+  const int wave = threadIdx.x >> 6, wi = wave % T::NWI, wj = wave / T::NWI;
+  finish_block<KIND, BT>(mat, op, ti, tj, wi * T::TI + q / T::TJ, wj * T::TJ + q % T::TJ, acc);
 }
 
-__global__ __launch_bounds__(kThreads, 2) void ortho_poly_kernel(const Mat *__restrict__ mats, const int *__restrict__ map, float ca, float cb, float cc) {
-  extern __shared__ __attribute__((aligned(1024))) char lds[];
-  const Mat p = mats[map[blockIdx.x]];
-  int ti;
-  const int tj = triangle(blockIdx.x - p.first[kPoly], ti);
-  f32x16 acc[2][2];
-  run<TileGram>(lds, side_kc<TileGram>(p.a, p.lda, p.m, p.lda, ti * kT, 0), side_kc<TileGram>(p.a, p.lda, p.m, p.lda, tj * kT, 0), (p.m + 31) / 32, acc);
-  store_symmetric<true>(p, p.b, ti, tj, acc, ca, cb, cc);
-}
+// ------------------------------------------------------------------------------------------------ small path
+typedef double f64x4 __attribute__((ext_vector_type(4)));
 
-__global__ __launch_bounds__(kThreads, 2) void ortho_apply_kernel(const Mat *__restrict__ mats, const int *__restrict__ map, int cur, int last) {
-  extern __shared__ __attribute__((aligned(1024))) char lds[];
-  const Mat p = mats[map[blockIdx.x]];
-  const int local = blockIdx.x - p.first[kApply], tm = (p.m + kT - 1) / kT;
-  const int tj = local % tm, ti = local / tm;
-  f32x16 acc[2][2];
-  run<TileApply>(lds, side_ks<TileApply>(cur ? p.x[1] : p.x[0], p.ldx, p.m, p.ldx, ti * kT * 4, 0), side_kc<TileApply>(p.b, p.lda, p.m, p.lda, tj * kT, 0), (p.m + 31) / 32, acc);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave & 1, wj = wave >> 1;
-  const int np = (p.n + 31) / 32 * 32;
+__device__ __forceinline__ int pad16(int m) { return (m + 15) / 16 * 16; }
+
+// share z of the lower triangle of A = G G^T: v_mfma_f64_16x16x4_f64.  Lane l holds row l % 16, k = l / 16 of a factor, and column l % 16,
+// rows l / 16 + 0, 4, 8, 12 of the result
+__global__ __launch_bounds__(kThreads) void ortho_small_gram_kernel(const Mat *__restrict__ mats, const int *__restrict__ map) {
+  __shared__ float t[kSmall][kChunk + 1];
+  const Mat *__restrict__ p = mats + map[blockIdx.x];
+  const int zi = blockIdx.x - p->first[kSmallGram], z = p->gram.z, mp = pad16(p->m), nb = mp / 16;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kq = lane >> 4;
+  const int blocks = nb * (nb + 1) / 2;                     // on and below the diagonal: at most 10, three a wave
+  int bi[3], bj[3];
+  f64x4 acc[3];
 #pragma unroll
-  for (int a = 0; a < 2; ++a)
+  for (int b = 0; b < 3; ++b) {
+    bi[b] = triangle(min(wave + 4 * b, blocks - 1), bj[b]);
+    acc[b] = f64x4{0, 0, 0, 0};
+  }
+  const int chunks = (p->n + kChunk - 1) / kChunk;
+  for (int c = zi; c < chunks; c += z) {
+    __syncthreads();
+    load_tile(p, c * kChunk, 0, t);
+    __syncthreads();
+#pragma unroll 4
+    for (int k = 0; k < kChunk; k += 4) {
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int j = tj * kT + (wj * 2 + b) * 32 + (lane & 31);
-      if (j >= p.m) continue;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int i = ti * kT + (wi * 2 + a) * 32 + g * 8 + (lane >> 5) * 4;
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[a][b][g * 4 + e] * (last ? 1.f / (kSB * kSX) : 1.f / kSB);
-        if (!last) {
-          if (i < np) store_planes((cur ? p.x[0] : p.x[1]) + (long long)j * p.ldx, i, v);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (i + e < p.n) {
-              const long long at = j * p.out_j + (i + e) * p.out_i;
-              if (p.bf16) ((__bf16 *)p.out)[at] = (__bf16)v[e];
-              else ((float *)p.out)[at] = v[e];
-            }
-        }
-      }
+      for (int b = 0; b < 3; ++b)
+        if (wave + 4 * b < blocks)
+          acc[b] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)t[bi[b] * 16 + r][k + kq], (double)t[bj[b] * 16 + r][k + kq], acc[b], 0, 0, 0);
     }
+  }
+  double *o = p->norm + (long long)zi * mp * mp;
+#pragma unroll
+  for (int b = 0; b < 3; ++b)
+    if (wave + 4 * b < blocks)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = bi[b] * 16 + 4 * e + kq, j = bj[b] * 16 + r;
+        if (i >= j) o[i * mp + j] = acc[b][e];
+      }
+}
+
+constexpr int kPolyThreads = 1024, kLdd = kSmall + 2;        // doubles of an LDS row
+
+// out = alpha L R (+ beta E + gamma I): symmetric, the blocks on and below the diagonal are computed and stored twice
+template <int NB>
+__device__ __forceinline__ void small_product(const double *l, const double *r, double *out, const double *add, double alpha, double beta, double gamma) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane & 15, kq = lane >> 4;
+  __syncthreads();
+  if (wave < NB * (NB + 1) / 2) {                           // a wave per block
+    int bj;
+    const int bi = triangle(wave, bj);                      // bi >= bj
+    const double *pl = l + (bi * 16 + q) * kLdd + kq, *pr = r + (bj * 16 + q) * kLdd + kq;
+    double fl[NB * 4], fr[NB * 4];
+#pragma unroll
+    for (int k = 0; k < NB * 4; ++k) {
+      fl[k] = pl[4 * k];
+      fr[k] = pr[4 * k];
+    }
+    f64x4 acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < NB * 4; ++k) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(fl[k], fr[k], acc, 0, 0, 0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = bi * 16 + 4 * e + kq, j = bj * 16 + q;
+      const double v = alpha * acc[e] + (add ? beta * add[i * kLdd + j] : 0.) + (i == j ? gamma : 0.);
+      if (i < j) continue;                                  // a block on the diagonal: its upper half is the lower one's copy
+      out[i * kLdd + j] = v;
+      out[j * kLdd + i] = v;
+    }
+  }
+  __syncthreads();
+}
+
+template <int NB>
+__device__ __forceinline__ double *small_steps(double *a, double *poly, double *q0, double *q1, int steps, float ca, float cb, float cc) {
+  double *q = nullptr;
+  for (int s = 0; s < steps; ++s) {
+    double *pn = q ? poly : q0;                             // the first polynomial is Q itself
+    small_product<NB>(a, a, pn, a, cc, cb, ca);
+    if (s + 1 < steps) {                                    // A <- P A P by way of the free buffer
+      double *tmp = q == q1 ? q0 : q1;
+      small_product<NB>(pn, a, tmp, nullptr, 1., 0., 0.);
+      small_product<NB>(pn, tmp, a, nullptr, 1., 0., 0.);
+    }
+    if (q) {
+      double *nq = q == q0 ? q1 : q0;
+      small_product<NB>(pn, q, nq, nullptr, 1., 0., 0.);
+      q = nq;
+    } else {
+      q = q0;
+    }
+  }
+  return q;
+}
+
+// all steps of one matrix: A -> Q, stored behind the parts of A
+__global__ __launch_bounds__(kPolyThreads) void ortho_small_poly_kernel(const Mat *__restrict__ mats, const int *__restrict__ map, int steps, float ca, float cb,
+                                                                        float cc, float eps) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  __shared__ double trace;
+  const Mat *__restrict__ p = mats + map[blockIdx.x];
+  const int m = p->m, mp = pad16(m), z = p->gram.z;
+  double *a = (double *)lds, *poly = a + kSmall * kLdd, *q0 = poly + kSmall * kLdd, *q1 = q0 + kSmall * kLdd;
+  double s[4] = {0, 0, 0, 0};                               // 4 elements a thread, 16 loads in flight
+  const double *part = p->norm;
+  const int size = mp * mp;
+#pragma unroll 4
+  for (int zi = 0; zi < z; ++zi)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int e = threadIdx.x + k * kPolyThreads;
+      if (e < size && e / mp >= e % mp) s[k] += part[(long long)zi * size + e];
+    }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int e = threadIdx.x + k * kPolyThreads, i = e / mp, j = e % mp;
+    if (e < size && i >= j) a[i * kLdd + j] = a[j * kLdd + i] = s[k];
+  }
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    double t = (int)threadIdx.x < m ? a[threadIdx.x * kLdd + threadIdx.x] : 0.;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o);
+    if (threadIdx.x == 0) trace = t;
+  }
+  __syncthreads();
+  const double inv = 1. / (sqrt(trace) + (double)eps);
+  for (int k = threadIdx.x; k < size; k += kPolyThreads) a[k / mp * kLdd + k % mp] *= inv * inv;
+  const double *q;
+  switch (mp / 16) {
+    case 1: q = small_steps<1>(a, poly, q0, q1, steps, ca, cb, cc); break;
+    case 2: q = small_steps<2>(a, poly, q0, q1, steps, ca, cb, cc); break;
+    case 3: q = small_steps<3>(a, poly, q0, q1, steps, ca, cb, cc); break;
+    default: q = small_steps<4>(a, poly, q0, q1, steps, ca, cb, cc);
+  }
+  double *o = p->norm + (long long)z * size;
+  for (int k = threadIdx.x; k < size; k += kPolyThreads) o[k] = q[k / mp * kLdd + k % mp] * inv;
+}
+
+// out = Q G, 64 columns a workgroup, in double too: Q reaches a^steps in the directions of small singular values, and its rounding to fp32 would show in
+// the others (1e-6).  Wave w has the columns 16 w .. 16 w + 15
+__global__ __launch_bounds__(kThreads) void ortho_small_apply_kernel(const Mat *__restrict__ mats, const int *__restrict__ map) {
+  __shared__ float t[kSmall][kChunk + 1];
+  __shared__ double q[kSmall][kSmall + 2];
+  const Mat *__restrict__ p = mats + map[blockIdx.x];
+  const int m = p->m, n = p->n, mp = pad16(m), nb = mp / 16, i0 = (blockIdx.x - p->first[kSmallApply]) * kChunk;
+  const double *qs = p->norm + (long long)p->gram.z * mp * mp;
+#pragma unroll
+  for (int k = 0; k < kSmall * kSmall / kThreads; ++k) {
+    const int e = threadIdx.x + k * kThreads;
+    if (e < mp * mp) q[e / mp][e % mp] = qs[e];
+  }
+  load_tile(p, i0, 0, t);
+  __syncthreads();
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kq = lane >> 4;
+  f64x4 acc[4];
+#pragma unroll
+  for (int b = 0; b < 4; ++b) acc[b] = f64x4{0, 0, 0, 0};
+  for (int k = 0; k < mp; k += 4) {
+    const double x = (double)t[k + kq][wave * 16 + r];
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+      if (b < nb) acc[b] = __builtin_amdgcn_mfma_f64_16x16x4f64(q[b * 16 + r][k + kq], x, acc[b], 0, 0, 0);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+    if (b < nb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[b * 16 + 4 * e + kq][wave * 16 + r] = (float)acc[b][e];
+  __syncthreads();
+  const bool wide = p->out_i == 1;
+  const long long oi = p->out_i, oj = p->out_j;
+  const int f32 = !p->bf16;
+  char *out = p->out;
+  for (int k = threadIdx.x; k < mp * kChunk; k += kThreads) {
+    const int c = wide ? k % kChunk : k / mp, j = wide ? k / kChunk : k % mp;
+    if (j >= m || i0 + c >= n) continue;
+    const long long at = j * oj + (i0 + c) * oi;
+    if (f32) ((float *)out)[at] = t[j][c];
+    else ((__bf16 *)out)[at] = (__bf16)t[j][c];
+  }
 }
 
 size_t take(size_t &at, size_t bytes) {
@@ -324,20 +552,60 @@ size_t take(size_t &at, size_t bytes) {
   return here;
 }
 
+// Splitting.  512 workgroups are resident (two a CU).  Fewer tiles than that in the whole list: each is split so that the chip is full, as long as a part
+// keeps 16 k-steps (a part costs a trip of its tile through memory).  More: what is left over after whole rounds would leave most of the chip idle for a
+// round; those tiles are split, down to 4 k-steps (4096 x 4096: 528 tiles on and below the diagonal, 238 -> 140 us a product).
+constexpr int kResident = 512;
+Split split_for(long long tiles, long long list_tiles, bool carries_rest, int steps) {
+  long long whole = tiles, z = 1;
+  if (list_tiles < kResident) {
+    z = kResident / list_tiles;
+    if (z > steps / 16) z = steps / 16;
+    if (z > 1) whole = 0;
+  } else if (carries_rest) {
+    const long long rest = list_tiles % kResident;
+    if (rest && rest <= tiles) {
+      z = kResident / rest;
+      if (z > steps / 4) z = steps / 4;
+      if (z > 1) whole = tiles - rest;
+    }
+  }
+  return {(int)tiles, (int)whole, (int)(z < 1 ? 1 : z)};
+}
+int split_blocks(const Split &s) { return s.whole + (s.tiles - s.whole) * s.z; }
+
 // Everything about the list that depends on its shapes: workspace places and workgroups.  `base` null: sizes only.
 int plan_list(const mr3d_matrix *in, int count, char *base, Plan &plan, Mat *mats, bool pointers) {
   if (!in || count <= 0 || count > 65536) return MR3D_ERR_INVALID_ARG;
   plan = Plan{};
   size_t at = 0;
   plan.mats_off = take(at, (size_t)count * sizeof(Mat));
-  long long gram_tiles = 0;
+  struct { long long sym[2], apply[2], parts, most; int carrier; } sum{};
+  sum.carrier = -1;
   for (int k = 0; k < count; ++k) {
     const mr3d_matrix &g = in[k];
     if (g.rows <= 0 || g.cols <= 0 || g.rows > (1 << 20) || g.cols > (1 << 20) || (pointers && (!g.in || !g.out))) return MR3D_ERR_INVALID_ARG;
     if (g.dtype != MR3D_DTYPE_F32 && g.dtype != MR3D_DTYPE_BF16) return MR3D_ERR_UNSUPPORTED;
-    const long long m = g.rows < g.cols ? g.rows : g.cols, tm = (m + kT - 1) / kT;
-    gram_tiles += tm * (tm + 1) / 2;
+    const long long m = g.rows < g.cols ? g.rows : g.cols, n = g.rows < g.cols ? g.cols : g.rows;
+    if (m <= kSmall) continue;
+    plan.fine |= g.dtype == MR3D_DTYPE_F32;
+    for (int b = 0; b < 2; ++b) {
+      const long long bt = b ? 128 : 64, tm = (m + bt - 1) / bt, tn = (n + bt - 1) / bt;
+      sum.sym[b] += tm * (tm + 1) / 2;
+      sum.apply[b] += tm * tn;
+      if (b) sum.parts += tm * (tm + 1) / 2 * ((n + 511) / 512);
+    }
+    if (m * n > sum.most) {
+      sum.most = m * n;
+      sum.carrier = k;
+    }
   }
+  // 64-wide tiles where 128-wide ones would leave CUs without one
+  plan.bt_square = sum.sym[1] >= 192 ? 128 : 64;
+  // X X^T has the long axis to split: 128-wide tiles as long as 16 k-steps a part make 256 workgroups of them
+  plan.bt_gram = sum.parts >= 256 ? 128 : 64;
+  plan.bt_apply = sum.apply[1] >= 192 ? 128 : 64;
+  const long long list_gram = sum.sym[plan.bt_gram == 128], list_sym = sum.sym[plan.bt_square == 128], list_apply = sum.apply[plan.bt_apply == 128];
   long long blocks[kStages] = {};
   for (int k = 0; k < count; ++k) {
     const mr3d_matrix &g = in[k];
@@ -352,30 +620,51 @@ int plan_list(const mr3d_matrix *in, int count, char *base, Plan &plan, Mat *mat
     p.out_j = tall ? 1 : g.cols;
     p.out_i = tall ? g.cols : 1;
     p.bf16 = g.dtype == MR3D_DTYPE_BF16;
-    p.ldx = (p.n + 31) / 32 * 128;
-    p.lda = (p.m + 31) / 32 * 128;
-    const int tm = (p.m + kT - 1) / kT, tn = (p.n + kT - 1) / kT, tri = tm * (tm + 1) / 2;
-    // Split the long axis of X X^T where the whole list has too few tiles to fill 256 CUs with two workgroups each; a part keeps at
-    // least 8 k-steps, so that its loads and its fp32 round trip through memory pay
-    const int steps = (p.n + 31) / 32;
-    long long z = gram_tiles >= 512 ? 1 : 512 / gram_tiles;
-    if (z > steps / 8) z = steps / 8;
-    p.z = (int)(z < 1 ? 1 : z);
-    const long long numel = (long long)p.m * p.n;
-    p.norm_blocks = (int)((numel + 8191) / 8192 > 1024 ? 1024 : (numel + 8191) / 8192);
-    const size_t ox0 = take(at, (size_t)p.m * p.ldx), ox1 = take(at, (size_t)p.m * p.ldx), oa = take(at, (size_t)p.m * p.lda), ob = take(at, (size_t)p.m * p.lda);
-    const size_t op = p.z > 1 ? take(at, (size_t)p.z * tri * kT * kT * sizeof(float)) : 0, on = take(at, (size_t)p.norm_blocks * sizeof(double));
-    p.x[0] = base + ox0;
-    p.x[1] = base + ox1;
-    p.a = base + oa;
-    p.b = base + ob;
-    p.part = (float *)(base + op);
-    p.norm = (double *)(base + on);
-    const long long need[kStages] = {p.norm_blocks, (long long)((p.m + 63) / 64) * ((p.n + 63) / 64), (long long)tri * p.z, p.z > 1 ? 4 * tri : 0, tri, (long long)tm * tn};
+    long long need[kStages] = {};
+    if (p.m <= kSmall) {
+      // a share of A takes at least 64 columns, at most 32 shares (one workgroup adds them up)
+      const int chunks = (p.n + kChunk - 1) / kChunk, mp = (p.m + 15) / 16 * 16;
+      p.gram.z = chunks < 32 ? chunks : 32;
+      p.norm = (double *)(base + take(at, ((size_t)p.gram.z + 1) * mp * mp * 8));
+      need[kSmallGram] = p.gram.z;
+      need[kSmallPoly] = 1;
+      need[kSmallApply] = chunks;
+    } else {
+      p.ldx = (p.n + 31) / 32 * 128;
+      p.lda = (p.m + 31) / 32 * 128;
+      const long long tg = (p.m + plan.bt_gram - 1) / plan.bt_gram, ts = (p.m + plan.bt_square - 1) / plan.bt_square, tm = (p.m + plan.bt_apply - 1) / plan.bt_apply, tn = (p.n + plan.bt_apply - 1) / plan.bt_apply;
+      const int ksm = (p.m + 31) / 32, ksn = (p.n + 31) / 32, qg = plan.bt_gram == 128 ? 4 : 1, qs = plan.bt_square == 128 ? 4 : 1, qa = plan.bt_apply == 128 ? 4 : 1;
+      if (ts * (ts + 1) / 2 > 0x3fffffff || tg * (tg + 1) / 2 > 0x3fffffff || tm * tn > 0x3fffffff) return MR3D_ERR_UNSUPPORTED;
+      p.gram = split_for(tg * (tg + 1) / 2, list_gram, k == sum.carrier, ksn);
+      p.square = split_for(ts * (ts + 1) / 2, list_sym, k == sum.carrier, ksm);
+      p.apply = split_for(tm * tn, list_apply, k == sum.carrier, ksm);
+      const long long numel = (long long)p.m * p.n;
+      p.norm_blocks = (int)((numel + 8191) / 8192 > 1024 ? 1024 : (numel + 8191) / 8192);
+      for (int b = 0; b < kBufs; ++b) {
+        const bool x = b == kX0 || b == kX1;
+        p.buf[b] = base + take(at, (size_t)p.m * (x ? p.ldx : p.lda));
+      }
+      size_t part = 0;
+      const struct { Split s; int bt; } uses[3] = {{p.gram, plan.bt_gram}, {p.square, plan.bt_square}, {p.apply, plan.bt_apply}};
+      for (const auto &u : uses) {
+        const size_t b = (size_t)(u.s.tiles - u.s.whole) * u.s.z * u.bt * u.bt * sizeof(float);
+        part = b > part ? b : part;
+      }
+      if (part) p.part = (float *)(base + take(at, part));
+      p.norm = (double *)(base + take(at, (size_t)p.norm_blocks * sizeof(double)));
+      need[kNorm] = p.norm_blocks;
+      need[kPack] = (long long)((p.m + 63) / 64) * ((p.n + 63) / 64);
+      need[kGram] = split_blocks(p.gram);
+      need[kGramJoin] = (long long)(p.gram.tiles - p.gram.whole) * qg;
+      need[kSquare] = split_blocks(p.square);
+      need[kSquareJoin] = (long long)(p.square.tiles - p.square.whole) * qs;
+      need[kApply] = split_blocks(p.apply);
+      need[kApplyJoin] = (long long)(p.apply.tiles - p.apply.whole) * qa;
+    }
     for (int s = 0; s < kStages; ++s) {
       p.first[s] = (int)blocks[s];
       blocks[s] += need[s];
-      if (blocks[s] > 0x7fffffff) return MR3D_ERR_UNSUPPORTED;
+      if (blocks[s] > 0x3fffffff) return MR3D_ERR_UNSUPPORTED;
     }
     if (mats) mats[k] = p;
   }
@@ -386,6 +675,28 @@ int plan_list(const mr3d_matrix *in, int count, char *base, Plan &plan, Mat *mat
   plan.bytes = at;
   return MR3D_OK;
 }
+
+struct Launcher {
+  const Plan &plan;
+  const Mat *mats;
+  const Maps &maps;
+  hipStream_t q;
+
+  template <int KIND, int BT, bool FINE> void tiles(const Op &op, int stage) const {
+    ortho_product_kernel<KIND, BT, FINE><<<plan.blocks[stage], kThreads, Pick<BT, KIND == 2, FINE>::T::LDS_BYTES, q>>>(mats, maps.map[stage], op);
+    if (plan.blocks[stage + 1]) ortho_join_kernel<KIND, BT><<<plan.blocks[stage + 1], kThreads, 0, q>>>(mats, maps.map[stage + 1], op);
+  }
+  // fp32 results: sums restarted every 16 k (2e-6 -> 1e-6 of the result); bf16 ones are rounded to 2^-9 anyway
+  template <int KIND> void product(const Op &op, int stage, int bt) const {
+    if (bt == 128) plan.fine ? tiles<KIND, 128, true>(op, stage) : tiles<KIND, 128, false>(op, stage);
+    else plan.fine ? tiles<KIND, 64, true>(op, stage) : tiles<KIND, 64, false>(op, stage);
+  }
+  void step(int x, bool last, float ca, float cb, float cc) const {
+    product<0>(Op{x, kSA / (kSX * kSX), 0.f, 0.f, 0}, kGram, plan.bt_gram);
+    product<1>(Op{x, cc * kSP / (kSA * kSA), cb * kSP / kSA, ca * kSP, 0}, kSquare, plan.bt_square);
+    product<2>(Op{x, last ? 1.f / (kSP * kSX) : 1.f / kSP, 0.f, 0.f, last}, kApply, plan.bt_apply);
+  }
+};
 
 }  // namespace
 
@@ -406,6 +717,10 @@ extern "C" int mr3d_orthogonalize(const mr3d_matrix *mats_host, int count, int s
   char *base = (char *)workspace;
   int st = plan_list(mats_host, count, base, plan, table, true);
   if (st == MR3D_OK && workspace_bytes < plan.bytes) st = MR3D_ERR_WORKSPACE;
+  constexpr int kPolyLds = 4 * kSmall * kLdd * 8;
+  if (st == MR3D_OK && plan.blocks[kSmallPoly] &&
+      hipFuncSetAttribute(reinterpret_cast<const void *>(ortho_small_poly_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kPolyLds) != hipSuccess)
+    st = MR3D_ERR_LAUNCH;
   if (st != MR3D_OK) {
     delete[] table;
     return st;
@@ -428,14 +743,16 @@ extern "C" int mr3d_orthogonalize(const mr3d_matrix *mats_host, int count, int s
   }
   const int mb = (most + 255) / 256;
   ortho_map_kernel<<<mb < 256 ? mb : 256, 256, 0, q>>>(mats, count, maps);
-  ortho_norm_kernel<<<plan.blocks[kNorm], 256, 0, q>>>(mats, maps.map[kNorm]);
-  ortho_pack_kernel<<<plan.blocks[kPack], 256, 0, q>>>(mats, maps.map[kPack], eps);
-  for (int k = 0; k < steps; ++k) {
-    const int cur = k & 1;
-    ortho_gram_kernel<<<plan.blocks[kGram], kThreads, TileGram::LDS_BYTES, q>>>(mats, maps.map[kGram], cur);
-    if (plan.blocks[kReduce]) ortho_reduce_kernel<<<plan.blocks[kReduce], kThreads, 0, q>>>(mats, maps.map[kReduce]);
-    ortho_poly_kernel<<<plan.blocks[kPoly], kThreads, TileGram::LDS_BYTES, q>>>(mats, maps.map[kPoly], ca, cb, cc);
-    ortho_apply_kernel<<<plan.blocks[kApply], kThreads, TileApply::LDS_BYTES, q>>>(mats, maps.map[kApply], cur, k == steps - 1);
+  if (plan.blocks[kSmallPoly]) {
+    ortho_small_gram_kernel<<<plan.blocks[kSmallGram], kThreads, 0, q>>>(mats, maps.map[kSmallGram]);
+    ortho_small_poly_kernel<<<plan.blocks[kSmallPoly], kPolyThreads, kPolyLds, q>>>(mats, maps.map[kSmallPoly], steps, ca, cb, cc, eps);
+    ortho_small_apply_kernel<<<plan.blocks[kSmallApply], kThreads, 0, q>>>(mats, maps.map[kSmallApply]);
+  }
+  if (plan.blocks[kNorm]) {
+    ortho_norm_kernel<<<plan.blocks[kNorm], 256, 0, q>>>(mats, maps.map[kNorm]);
+    ortho_pack_kernel<<<plan.blocks[kPack], 256, 0, q>>>(mats, maps.map[kPack], eps);
+    const Launcher run{plan, mats, maps, q};
+    for (int k = 0; k < steps; ++k) run.step(k & 1 ? kX1 : kX0, k == steps - 1, ca, cb, cc);
   }
   return mr3d_launch_status();
 }
