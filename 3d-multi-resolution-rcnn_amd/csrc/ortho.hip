@@ -35,12 +35,11 @@ enum Buf { kA, kP, kX0, kX1, kBufs };
 struct Split { int tiles, whole, z; };
 
 struct Mat {
-  const char *in;
-  char *out;
+  long long in, out;                                        // places: bytes from the workspace (also the caller's matrices)
   long long in_i, in_j, out_i, out_j;                       // element strides along n (i) and m (j)
-  char *buf[kBufs];                                         // planes
-  float *part;                                              // parts of split tiles, [tile - whole][z][BT * BT]
-  double *norm;                                             // small path: parts of A, [z][mp][mp], then Q
+  long long buf[kBufs];                                     // planes
+  long long part;                                           // parts of split tiles, [tile - whole][z][BT * BT] floats
+  long long norm;                                           // doubles; small path: parts of A, [z][mp][mp], then Q
   int m, n, ldx, lda;                                       // ld in bytes
   int bf16, norm_blocks;
   Split gram, square, apply;
@@ -57,6 +56,10 @@ struct Plan {
 
 constexpr int kBatch = 16;
 struct MatBatch { Mat m[kBatch]; };
+
+// Places are stored as distances from the workspace, a kernel argument: a pointer read from the table would count as generic, and generic (flat)
+// accesses wait for LDS and memory alike, one after the other
+template <class T> __device__ __forceinline__ T *at(char *ws, long long place) { return reinterpret_cast<T *>(ws + place); }
 
 __device__ __forceinline__ int triangle(int t, int &ti) {
   int tj = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
@@ -84,12 +87,12 @@ __global__ __launch_bounds__(256) void ortho_map_kernel(const Mat *__restrict__ 
     }
 }
 
-__device__ __forceinline__ float read_in(const Mat &p, long long off) {
-  return p.bf16 ? (float)((const __bf16 *)p.in)[off] : ((const float *)p.in)[off];
+__device__ __forceinline__ float read_in(char *ws, const Mat &p, long long off) {
+  return p.bf16 ? (float)at<const __bf16>(ws, p.in)[off] : at<const float>(ws, p.in)[off];
 }
 
 // squares of the input in double: fp32 squares would overflow from 2^64 on
-__global__ __launch_bounds__(256) void ortho_norm_kernel(const Mat *__restrict__ mats, const int *__restrict__ map) {
+__global__ __launch_bounds__(256) void ortho_norm_kernel(char *ws, const Mat *__restrict__ mats, const int *__restrict__ map) {
   const Mat p = mats[map[blockIdx.x]];
   const int chunk = blockIdx.x - p.first[kNorm];
   const bool wide = p.in_i == 1;                            // walk the contiguous axis with the threads
@@ -99,18 +102,18 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(const Mat *__restrict__
   double s = 0;
   long long e = (long long)chunk * 256 + threadIdx.x;
   const long long stride = (long long)p.norm_blocks * 256;
-  if (si == 1 && so == inner && ((uintptr_t)p.in & 15) == 0) {            // packed: 16 bytes a load
+  if (si == 1 && so == inner && ((uintptr_t)(ws + p.in) & 15) == 0) {            // packed: 16 bytes a load
     const int per = p.bf16 ? 8 : 4;
     const long long groups = total / per;
 #pragma unroll 2
     for (; e < groups; e += stride) {
       float v[8];
       if (p.bf16) {
-        const bf16x8 t = *reinterpret_cast<const bf16x8 *>(p.in + e * 16);
+        const bf16x8 t = at<const bf16x8>(ws, p.in)[e];
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = (float)t[k];
       } else {
-        const float4 t = *reinterpret_cast<const float4 *>(p.in + e * 16);
+        const float4 t = at<const float4>(ws, p.in)[e];
         v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
         v[4] = v[5] = v[6] = v[7] = 0.f;
       }
@@ -118,13 +121,13 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(const Mat *__restrict__
       for (int k = 0; k < 8; ++k) s += (double)v[k] * (double)v[k];
     }
     for (e = groups * per + (long long)chunk * 256 + threadIdx.x; e < total; e += stride) {
-      const double v = (double)read_in(p, e);
+      const double v = (double)read_in(ws, p, e);
       s += v * v;
     }
   } else {
     for (; e < total; e += stride) {
       const int o = (int)(e / inner), i = (int)(e - (long long)o * inner);
-      const double v = (double)read_in(p, o * so + i * si);
+      const double v = (double)read_in(ws, p, o * so + i * si);
       s += v * v;
     }
   }
@@ -133,13 +136,13 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(const Mat *__restrict__
   __shared__ double w[4];
   if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) p.norm[chunk] = w[0] + w[1] + w[2] + w[3];
+  if (threadIdx.x == 0) at<double>(ws, p.norm)[chunk] = w[0] + w[1] + w[2] + w[3];
 }
 
 constexpr int kChunk = 64;                                  // columns of X in LDS
 
 // rows [0, 64) x columns [i0, i0 + 64) of the wide matrix, zeros outside -> t[row][col]; read along the contiguous axis, 16 loads a thread in flight
-__device__ __forceinline__ void load_tile(const Mat *__restrict__ p, int i0, int j0, float (*t)[kChunk + 1]) {
+__device__ __forceinline__ void load_tile(char *ws, const Mat *__restrict__ p, int i0, int j0, float (*t)[kChunk + 1]) {
   const long long si = p->in_i, sj = p->in_j;
   const bool wide = si == 1;
   const int fast = threadIdx.x & 63, slow = threadIdx.x >> 6, m = p->m - j0, n = p->n - i0;
@@ -152,25 +155,25 @@ __device__ __forceinline__ void load_tile(const Mat *__restrict__ p, int i0, int
       v[k] = q < n && r < m ? (float)in[base + q * si + r * sj] : 0.f;
     }
   };
-  if (p->bf16) each((const __bf16 *)p->in);
-  else each((const float *)p->in);
+  if (p->bf16) each(at<const __bf16>(ws, p->in));
+  else each(at<const float>(ws, p->in));
 #pragma unroll
   for (int k = 0; k < 16; ++k) t[wide ? slow + 4 * k : fast][wide ? fast : slow + 4 * k] = v[k];
 }
 
 // 64 x 64 of the input -> planes of X; the tile goes through LDS so that a tall input is read along its rows too
-__global__ __launch_bounds__(256) void ortho_pack_kernel(const Mat *__restrict__ mats, const int *__restrict__ map, float eps) {
+__global__ __launch_bounds__(256) void ortho_pack_kernel(char *ws, const Mat *__restrict__ mats, const int *__restrict__ map, float eps) {
   __shared__ float t[64][65];
   __shared__ double w[4];
   const Mat p = mats[map[blockIdx.x]];
   const int tile = blockIdx.x - p.first[kPack], tn = (p.n + 63) / 64;
   const int j0 = tile / tn * 64, i0 = tile % tn * 64;
   double s = 0;
-  for (int k = threadIdx.x; k < p.norm_blocks; k += 256) s += p.norm[k];
+  for (int k = threadIdx.x; k < p.norm_blocks; k += 256) s += at<double>(ws, p.norm)[k];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
   if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = s;
-  load_tile(mats + map[blockIdx.x], i0, j0, t);
+  load_tile(ws, mats + map[blockIdx.x], i0, j0, t);
   __syncthreads();
   const double scale = (double)kSX / (sqrt(w[0] + w[1] + w[2] + w[3]) + (double)eps);      // may leave fp32's range where G does not
   const int np = (p.n + 31) / 32 * 32;
@@ -180,7 +183,7 @@ __global__ __launch_bounds__(256) void ortho_pack_kernel(const Mat *__restrict__
     _Float16 h[4], l[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) split16((float)((double)t[j][i + e] * scale), h[e], l[e]);
-    char *d = p.buf[kX0] + (long long)(j0 + j) * p.ldx + (i0 + i) / 32 * 128 + (i & 31) * 2;
+    char *d = ws + p.buf[kX0] + (long long)(j0 + j) * p.ldx + (i0 + i) / 32 * 128 + (i & 31) * 2;
     *reinterpret_cast<uint2 *>(d) = *reinterpret_cast<uint2 *>(h);
     *reinterpret_cast<uint2 *>(d + 64) = *reinterpret_cast<uint2 *>(l);
   }
@@ -213,12 +216,12 @@ struct Op {
 
 // 32 x 32 block (bi, bj) of tile (ti, tj), one accumulator of a wave
 template <int KIND, int BT>
-__device__ __forceinline__ void finish_block(const Mat *__restrict__ mat, const Op &op, int ti, int tj, int bi, int bj, const f32x16 &acc) {
+__device__ __forceinline__ void finish_block(char *ws, const Mat *__restrict__ mat, const Op &op, int ti, int tj, int bi, int bj, const f32x16 &acc) {
   const int lane = threadIdx.x & 63, m = mat->m;
   const int j = tj * BT + bj * 32 + (lane & 31);
   if constexpr (KIND < 2) {
     const int mp = (m + 31) / 32 * 32, lda = mat->lda;
-    char *dst = mat->buf[KIND == 0 ? kA : kP];
+    char *dst = ws + mat->buf[KIND == 0 ? kA : kP];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int i = ti * BT + bi * 32 + g * 8 + (lane >> 5) * 4;
@@ -228,7 +231,7 @@ __device__ __forceinline__ void finish_block(const Mat *__restrict__ mat, const 
         for (int e = 0; e < 4; ++e) v[e] = op.alpha * acc[g * 4 + e];
       } else {
         float f[4] = {0.f, 0.f, 0.f, 0.f};
-        if (j < m && i < mp) load_planes(mat->buf[kA] + (long long)j * lda, i, f);
+        if (j < m && i < mp) load_planes(ws + mat->buf[kA] + (long long)j * lda, i, f);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = op.alpha * acc[g * 4 + e] + op.beta * f[e] + (i + e == j ? op.gamma : 0.f);
       }
@@ -255,15 +258,15 @@ __device__ __forceinline__ void finish_block(const Mat *__restrict__ mat, const 
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = acc[g * 4 + e] * op.alpha;
       if (!op.last) {
-        if (i < np) store_planes(mat->buf[op.x == kX0 ? kX1 : kX0] + (long long)j * mat->ldx, i, v);
+        if (i < np) store_planes(ws + mat->buf[op.x == kX0 ? kX1 : kX0] + (long long)j * mat->ldx, i, v);
       } else {
         const long long oj = mat->out_j, oi = mat->out_i;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (i + e < n) {
-            const long long at = j * oj + (i + e) * oi;
-            if (mat->bf16) ((__bf16 *)mat->out)[at] = (__bf16)v[e];
-            else ((float *)mat->out)[at] = v[e];
+            const long long k = j * oj + (i + e) * oi;
+            if (mat->bf16) at<__bf16>(ws, mat->out)[k] = (__bf16)v[e];
+            else at<float>(ws, mat->out)[k] = v[e];
           }
       }
     }
@@ -284,7 +287,7 @@ __device__ __forceinline__ void tile_at(const Mat *__restrict__ mat, int t, int 
 }
 
 template <int KIND, int BT, bool FINE>
-__global__ __launch_bounds__(kThreads, 2) void ortho_product_kernel(const Mat *__restrict__ mats, const int *__restrict__ map, Op op) {
+__global__ __launch_bounds__(kThreads, 2) void ortho_product_kernel(char *ws, const Mat *__restrict__ mats, const int *__restrict__ map, Op op) {
   typedef typename Pick<BT, KIND == 2, FINE>::T T;
   constexpr int kFirst = KIND == 0 ? kGram : KIND == 1 ? kSquare : kApply;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
@@ -303,7 +306,7 @@ __global__ __launch_bounds__(kThreads, 2) void ortho_product_kernel(const Mat *_
   const int total = ((KIND == 0 ? mat->n : m) + 31) / 32;
   const int s0 = (int)((long long)total * zi / z), s1 = (int)((long long)total * (zi + 1) / z);
   const int ldl = KIND == 1 ? mat->lda : mat->ldx, ldr = KIND == 0 ? mat->ldx : mat->lda;
-  const char *l = mat->buf[KIND == 1 ? kA : op.x], *r = mat->buf[KIND == 0 ? op.x : KIND == 1 ? kA : kP];
+  const char *l = ws + mat->buf[KIND == 1 ? kA : op.x], *r = ws + mat->buf[KIND == 0 ? op.x : KIND == 1 ? kA : kP];
   f32x16 acc[T::TI][T::TJ];
   if constexpr (KIND == 2) run<T>(lds, side_ks<T>(l, ldl, m, ldl, (long long)ti * BT * 4, s0), side_kc<T>(r, ldr, m, ldr, tj * BT, s0), s1 - s0, acc);
   else run<T>(lds, side_kc<T>(l, ldl, m, ldl, ti * BT, s0), side_kc<T>(r, ldr, m, ldr, tj * BT, s0), s1 - s0, acc);
@@ -312,9 +315,9 @@ __global__ __launch_bounds__(kThreads, 2) void ortho_product_kernel(const Mat *_
 #pragma unroll
     for (int x = 0; x < T::TI; ++x)
 #pragma unroll
-      for (int y = 0; y < T::TJ; ++y) finish_block<KIND, BT>(mat, op, ti, tj, wi * T::TI + x, wj * T::TJ + y, acc[x][y]);
+      for (int y = 0; y < T::TJ; ++y) finish_block<KIND, BT>(ws, mat, op, ti, tj, wi * T::TI + x, wj * T::TJ + y, acc[x][y]);
   } else {
-    float *d = mat->part + ((long long)(t - sp.whole) * z + zi) * (BT * BT) + threadIdx.x;
+    float *d = at<float>(ws, mat->part) + ((long long)(t - sp.whole) * z + zi) * (BT * BT) + threadIdx.x;
 #pragma unroll
     for (int x = 0; x < T::TI; ++x)
 #pragma unroll
@@ -326,7 +329,7 @@ __global__ __launch_bounds__(kThreads, 2) void ortho_product_kernel(const Mat *_
 
 // the parts of split tiles, added in a fixed order; a workgroup takes one 32 x 32 block of every wave
 template <int KIND, int BT>
-__global__ __launch_bounds__(kThreads) void ortho_join_kernel(const Mat *__restrict__ mats, const int *__restrict__ map, Op op) {
+__global__ __launch_bounds__(kThreads) void ortho_join_kernel(char *ws, const Mat *__restrict__ mats, const int *__restrict__ map, Op op) {
   typedef typename Pick<BT, KIND == 2, false>::T T;
   constexpr int kFirst = KIND == 0 ? kGramJoin : KIND == 1 ? kSquareJoin : kApplyJoin, Q = T::TI * T::TJ;
   const int b = blockIdx.x;
@@ -335,7 +338,7 @@ __global__ __launch_bounds__(kThreads) void ortho_join_kernel(const Mat *__restr
   const int local = b - mat->first[kFirst], u = local / Q, q = local % Q;
   int ti, tj;
   tile_at<KIND, BT>(mat, sp.whole + u, ti, tj);
-  const float *s = mat->part + (long long)u * sp.z * (BT * BT) + q * 16 * kThreads + threadIdx.x;
+  const float *s = at<float>(ws, mat->part) + (long long)u * sp.z * (BT * BT) + q * 16 * kThreads + threadIdx.x;
   f32x16 acc;
 #pragma unroll
   for (int e = 0; e < 16; ++e) acc[e] = s[e * kThreads];
@@ -356,7 +359,7 @@ __global__ __launch_bounds__(kThreads) void ortho_join_kernel(const Mat *__restr
     }
   }
   const int wave = threadIdx.x >> 6, wi = wave % T::NWI, wj = wave / T::NWI;
-  finish_block<KIND, BT>(mat, op, ti, tj, wi * T::TI + q / T::TJ, wj * T::TJ + q % T::TJ, acc);
+  finish_block<KIND, BT>(ws, mat, op, ti, tj, wi * T::TI + q / T::TJ, wj * T::TJ + q % T::TJ, acc);
 }
 
 // ------------------------------------------------------------------------------------------------ small path
@@ -366,7 +369,7 @@ __device__ __forceinline__ int pad16(int m) { return (m + 15) / 16 * 16; }
 
 // share z of the lower triangle of A = G G^T: v_mfma_f64_16x16x4_f64.  Lane l holds row l % 16, k = l / 16 of a factor, and column l % 16,
 // rows l / 16 + 0, 4, 8, 12 of the result
-__global__ __launch_bounds__(kThreads) void ortho_small_gram_kernel(const Mat *__restrict__ mats, const int *__restrict__ map) {
+__global__ __launch_bounds__(kThreads) void ortho_small_gram_kernel(char *ws, const Mat *__restrict__ mats, const int *__restrict__ map) {
   __shared__ float t[kSmall][kChunk + 1];
   const Mat *__restrict__ p = mats + map[blockIdx.x];
   const int zi = blockIdx.x - p->first[kSmallGram], z = p->gram.z, mp = pad16(p->m), nb = mp / 16;
@@ -382,7 +385,7 @@ __global__ __launch_bounds__(kThreads) void ortho_small_gram_kernel(const Mat *_
   const int chunks = (p->n + kChunk - 1) / kChunk;
   for (int c = zi; c < chunks; c += z) {
     __syncthreads();
-    load_tile(p, c * kChunk, 0, t);
+    load_tile(ws, p, c * kChunk, 0, t);
     __syncthreads();
 #pragma unroll 4
     for (int k = 0; k < kChunk; k += 4) {
@@ -392,7 +395,7 @@ __global__ __launch_bounds__(kThreads) void ortho_small_gram_kernel(const Mat *_
           acc[b] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)t[bi[b] * 16 + r][k + kq], (double)t[bj[b] * 16 + r][k + kq], acc[b], 0, 0, 0);
     }
   }
-  double *o = p->norm + (long long)zi * mp * mp;
+  double *o = at<double>(ws, p->norm) + (long long)zi * mp * mp;
 #pragma unroll
   for (int b = 0; b < 3; ++b)
     if (wave + 4 * b < blocks)
@@ -405,15 +408,15 @@ __global__ __launch_bounds__(kThreads) void ortho_small_gram_kernel(const Mat *_
 
 constexpr int kPolyThreads = 1024, kLdd = kSmall + 2;        // doubles of an LDS row
 
-// out = alpha L R (+ beta E + gamma I): symmetric, the blocks on and below the diagonal are computed and stored twice
+// m[out] = alpha m[l] m[r] (+ beta m[add] + gamma I): symmetric, the blocks on and below the diagonal are computed and stored twice.  Matrices
+// go by their place in LDS, not by pointers: selected pointers would be read as generic ones
 template <int NB>
-__device__ __forceinline__ void small_product(const double *l, const double *r, double *out, const double *add, double alpha, double beta, double gamma) {
+__device__ __forceinline__ void small_product(double (*m)[kSmall * kLdd], int l, int r, int out, int add, double alpha, double beta, double gamma) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane & 15, kq = lane >> 4;
   __syncthreads();
-  if (wave < NB * (NB + 1) / 2) {                           // a wave per block
-    int bj;
-    const int bi = triangle(wave, bj);                      // bi >= bj
-    const double *pl = l + (bi * 16 + q) * kLdd + kq, *pr = r + (bj * 16 + q) * kLdd + kq;
+  if (wave < NB * (NB + 1) / 2) {                           // a wave per block (bi >= bj)
+    const int bi = wave < 1 ? 0 : wave < 3 ? 1 : wave < 6 ? 2 : 3, bj = wave - bi * (bi + 1) / 2;
+    const double *pl = m[l] + (bi * 16 + q) * kLdd + kq, *pr = m[r] + (bj * 16 + q) * kLdd + kq;
     double fl[NB * 4], fr[NB * 4];
 #pragma unroll
     for (int k = 0; k < NB * 4; ++k) {
@@ -426,55 +429,64 @@ __device__ __forceinline__ void small_product(const double *l, const double *r, 
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int i = bi * 16 + 4 * e + kq, j = bj * 16 + q;
-      const double v = alpha * acc[e] + (add ? beta * add[i * kLdd + j] : 0.) + (i == j ? gamma : 0.);
+      const double v = alpha * acc[e] + (add >= 0 ? beta * m[add < 0 ? 0 : add][i * kLdd + j] : 0.) + (i == j ? gamma : 0.);
       if (i < j) continue;                                  // a block on the diagonal: its upper half is the lower one's copy
-      out[i * kLdd + j] = v;
-      out[j * kLdd + i] = v;
+      m[out][i * kLdd + j] = v;
+      m[out][j * kLdd + i] = v;
     }
   }
   __syncthreads();
 }
 
+// A in m[0] -> Q; returns its place
 template <int NB>
-__device__ __forceinline__ double *small_steps(double *a, double *poly, double *q0, double *q1, int steps, float ca, float cb, float cc) {
-  double *q = nullptr;
+__device__ __forceinline__ int small_steps(double (*m)[kSmall * kLdd], int steps, float ca, float cb, float cc) {
+  int q = -1;
   for (int s = 0; s < steps; ++s) {
-    double *pn = q ? poly : q0;                             // the first polynomial is Q itself
-    small_product<NB>(a, a, pn, a, cc, cb, ca);
+    const int pn = q >= 0 ? 1 : 2;                          // the first polynomial is Q itself
+    small_product<NB>(m, 0, 0, pn, 0, cc, cb, ca);
     if (s + 1 < steps) {                                    // A <- P A P by way of the free buffer
-      double *tmp = q == q1 ? q0 : q1;
-      small_product<NB>(pn, a, tmp, nullptr, 1., 0., 0.);
-      small_product<NB>(pn, tmp, a, nullptr, 1., 0., 0.);
+      const int tmp = q == 3 ? 2 : 3;
+      small_product<NB>(m, pn, 0, tmp, -1, 1., 0., 0.);
+      small_product<NB>(m, pn, tmp, 0, -1, 1., 0., 0.);
     }
-    if (q) {
-      double *nq = q == q0 ? q1 : q0;
-      small_product<NB>(pn, q, nq, nullptr, 1., 0., 0.);
+    if (q >= 0) {
+      const int nq = q == 2 ? 3 : 2;
+      small_product<NB>(m, pn, q, nq, -1, 1., 0., 0.);
       q = nq;
     } else {
-      q = q0;
+      q = 2;
     }
   }
   return q;
 }
 
 // all steps of one matrix: A -> Q, stored behind the parts of A
-__global__ __launch_bounds__(kPolyThreads) void ortho_small_poly_kernel(const Mat *__restrict__ mats, const int *__restrict__ map, int steps, float ca, float cb,
+__global__ __launch_bounds__(kPolyThreads) void ortho_small_poly_kernel(char *ws, const Mat *__restrict__ mats, const int *__restrict__ map, int steps, float ca, float cb,
                                                                         float cc, float eps) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   __shared__ double trace;
   const Mat *__restrict__ p = mats + map[blockIdx.x];
   const int m = p->m, mp = pad16(m), z = p->gram.z;
-  double *a = (double *)lds, *poly = a + kSmall * kLdd, *q0 = poly + kSmall * kLdd, *q1 = q0 + kSmall * kLdd;
-  double s[4] = {0, 0, 0, 0};                               // 4 elements a thread, 16 loads in flight
-  const double *part = p->norm;
+  auto mats4 = reinterpret_cast<double (*)[kSmall * kLdd]>(lds);
+  double *a = mats4[0];
+  double s[4] = {0, 0, 0, 0};                               // 4 elements a thread, 32 loads in flight
+  const double *part = at<double>(ws, p->norm);
   const int size = mp * mp;
-#pragma unroll 4
-  for (int zi = 0; zi < z; ++zi)
+  for (int z0 = 0; z0 < z; z0 += 8) {
+    double v[8][4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int e = threadIdx.x + k * kPolyThreads;
-      if (e < size && e / mp >= e % mp) s[k] += part[(long long)zi * size + e];
-    }
+    for (int y = 0; y < 8; ++y)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int e = threadIdx.x + k * kPolyThreads;
+        v[y][k] = e < size && z0 + y < z ? part[(z0 + y) * size + e] : 0.;
+      }
+#pragma unroll
+    for (int y = 0; y < 8; ++y)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[k] += v[y][k];
+  }
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int e = threadIdx.x + k * kPolyThreads, i = e / mp, j = e % mp;
@@ -490,31 +502,31 @@ __global__ __launch_bounds__(kPolyThreads) void ortho_small_poly_kernel(const Ma
   __syncthreads();
   const double inv = 1. / (sqrt(trace) + (double)eps);
   for (int k = threadIdx.x; k < size; k += kPolyThreads) a[k / mp * kLdd + k % mp] *= inv * inv;
-  const double *q;
+  int q;
   switch (mp / 16) {
-    case 1: q = small_steps<1>(a, poly, q0, q1, steps, ca, cb, cc); break;
-    case 2: q = small_steps<2>(a, poly, q0, q1, steps, ca, cb, cc); break;
-    case 3: q = small_steps<3>(a, poly, q0, q1, steps, ca, cb, cc); break;
-    default: q = small_steps<4>(a, poly, q0, q1, steps, ca, cb, cc);
+    case 1: q = small_steps<1>(mats4, steps, ca, cb, cc); break;
+    case 2: q = small_steps<2>(mats4, steps, ca, cb, cc); break;
+    case 3: q = small_steps<3>(mats4, steps, ca, cb, cc); break;
+    default: q = small_steps<4>(mats4, steps, ca, cb, cc);
   }
-  double *o = p->norm + (long long)z * size;
-  for (int k = threadIdx.x; k < size; k += kPolyThreads) o[k] = q[k / mp * kLdd + k % mp] * inv;
+  double *o = at<double>(ws, p->norm) + (long long)z * size;
+  for (int k = threadIdx.x; k < size; k += kPolyThreads) o[k] = mats4[q][k / mp * kLdd + k % mp] * inv;
 }
 
 // out = Q G, 64 columns a workgroup, in double too: Q reaches a^steps in the directions of small singular values, and its rounding to fp32 would show in
 // the others (1e-6).  Wave w has the columns 16 w .. 16 w + 15
-__global__ __launch_bounds__(kThreads) void ortho_small_apply_kernel(const Mat *__restrict__ mats, const int *__restrict__ map) {
+__global__ __launch_bounds__(kThreads) void ortho_small_apply_kernel(char *ws, const Mat *__restrict__ mats, const int *__restrict__ map) {
   __shared__ float t[kSmall][kChunk + 1];
   __shared__ double q[kSmall][kSmall + 2];
   const Mat *__restrict__ p = mats + map[blockIdx.x];
   const int m = p->m, n = p->n, mp = pad16(m), nb = mp / 16, i0 = (blockIdx.x - p->first[kSmallApply]) * kChunk;
-  const double *qs = p->norm + (long long)p->gram.z * mp * mp;
+  const double *qs = at<double>(ws, p->norm) + (long long)p->gram.z * mp * mp;
 #pragma unroll
   for (int k = 0; k < kSmall * kSmall / kThreads; ++k) {
     const int e = threadIdx.x + k * kThreads;
     if (e < mp * mp) q[e / mp][e % mp] = qs[e];
   }
-  load_tile(p, i0, 0, t);
+  load_tile(ws, p, i0, 0, t);
   __syncthreads();
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kq = lane >> 4;
   f64x4 acc[4];
@@ -536,13 +548,13 @@ __global__ __launch_bounds__(kThreads) void ortho_small_apply_kernel(const Mat *
   const bool wide = p->out_i == 1;
   const long long oi = p->out_i, oj = p->out_j;
   const int f32 = !p->bf16;
-  char *out = p->out;
+  char *out = ws + p->out;
   for (int k = threadIdx.x; k < mp * kChunk; k += kThreads) {
     const int c = wide ? k % kChunk : k / mp, j = wide ? k / kChunk : k % mp;
     if (j >= m || i0 + c >= n) continue;
-    const long long at = j * oj + (i0 + c) * oi;
-    if (f32) ((float *)out)[at] = t[j][c];
-    else ((__bf16 *)out)[at] = (__bf16)t[j][c];
+    const long long e = j * oj + (i0 + c) * oi;
+    if (f32) ((float *)out)[e] = t[j][c];
+    else ((__bf16 *)out)[e] = (__bf16)t[j][c];
   }
 }
 
@@ -613,8 +625,8 @@ int plan_list(const mr3d_matrix *in, int count, char *base, Plan &plan, Mat *mat
     Mat p{};
     p.m = (int)(tall ? g.cols : g.rows);
     p.n = (int)(tall ? g.rows : g.cols);
-    p.in = (const char *)g.in;
-    p.out = (char *)g.out;
+    p.in = (const char *)g.in - base;
+    p.out = (const char *)g.out - base;
     p.in_j = tall ? g.in_col_stride : g.in_row_stride;
     p.in_i = tall ? g.in_row_stride : g.in_col_stride;
     p.out_j = tall ? 1 : g.cols;
@@ -625,7 +637,7 @@ int plan_list(const mr3d_matrix *in, int count, char *base, Plan &plan, Mat *mat
       // a share of A takes at least 64 columns, at most 32 shares (one workgroup adds them up)
       const int chunks = (p.n + kChunk - 1) / kChunk, mp = (p.m + 15) / 16 * 16;
       p.gram.z = chunks < 32 ? chunks : 32;
-      p.norm = (double *)(base + take(at, ((size_t)p.gram.z + 1) * mp * mp * 8));
+      p.norm = take(at, ((size_t)p.gram.z + 1) * mp * mp * 8);
       need[kSmallGram] = p.gram.z;
       need[kSmallPoly] = 1;
       need[kSmallApply] = chunks;
@@ -642,7 +654,7 @@ int plan_list(const mr3d_matrix *in, int count, char *base, Plan &plan, Mat *mat
       p.norm_blocks = (int)((numel + 8191) / 8192 > 1024 ? 1024 : (numel + 8191) / 8192);
       for (int b = 0; b < kBufs; ++b) {
         const bool x = b == kX0 || b == kX1;
-        p.buf[b] = base + take(at, (size_t)p.m * (x ? p.ldx : p.lda));
+        p.buf[b] = take(at, (size_t)p.m * (x ? p.ldx : p.lda));
       }
       size_t part = 0;
       const struct { Split s; int bt; } uses[3] = {{p.gram, plan.bt_gram}, {p.square, plan.bt_square}, {p.apply, plan.bt_apply}};
@@ -650,8 +662,8 @@ int plan_list(const mr3d_matrix *in, int count, char *base, Plan &plan, Mat *mat
         const size_t b = (size_t)(u.s.tiles - u.s.whole) * u.s.z * u.bt * u.bt * sizeof(float);
         part = b > part ? b : part;
       }
-      if (part) p.part = (float *)(base + take(at, part));
-      p.norm = (double *)(base + take(at, (size_t)p.norm_blocks * sizeof(double)));
+      if (part) p.part = take(at, part);
+      p.norm = take(at, (size_t)p.norm_blocks * sizeof(double));
       need[kNorm] = p.norm_blocks;
       need[kPack] = (long long)((p.m + 63) / 64) * ((p.n + 63) / 64);
       need[kGram] = split_blocks(p.gram);
@@ -677,14 +689,15 @@ int plan_list(const mr3d_matrix *in, int count, char *base, Plan &plan, Mat *mat
 }
 
 struct Launcher {
+  char *ws;
   const Plan &plan;
   const Mat *mats;
   const Maps &maps;
   hipStream_t q;
 
   template <int KIND, int BT, bool FINE> void tiles(const Op &op, int stage) const {
-    ortho_product_kernel<KIND, BT, FINE><<<plan.blocks[stage], kThreads, Pick<BT, KIND == 2, FINE>::T::LDS_BYTES, q>>>(mats, maps.map[stage], op);
-    if (plan.blocks[stage + 1]) ortho_join_kernel<KIND, BT><<<plan.blocks[stage + 1], kThreads, 0, q>>>(mats, maps.map[stage + 1], op);
+    ortho_product_kernel<KIND, BT, FINE><<<plan.blocks[stage], kThreads, Pick<BT, KIND == 2, FINE>::T::LDS_BYTES, q>>>(ws, mats, maps.map[stage], op);
+    if (plan.blocks[stage + 1]) ortho_join_kernel<KIND, BT><<<plan.blocks[stage + 1], kThreads, 0, q>>>(ws, mats, maps.map[stage + 1], op);
   }
   // fp32 results: sums restarted every 16 k (2e-6 -> 1e-6 of the result); bf16 ones are rounded to 2^-9 anyway
   template <int KIND> void product(const Op &op, int stage, int bt) const {
@@ -744,14 +757,14 @@ extern "C" int mr3d_orthogonalize(const mr3d_matrix *mats_host, int count, int s
   const int mb = (most + 255) / 256;
   ortho_map_kernel<<<mb < 256 ? mb : 256, 256, 0, q>>>(mats, count, maps);
   if (plan.blocks[kSmallPoly]) {
-    ortho_small_gram_kernel<<<plan.blocks[kSmallGram], kThreads, 0, q>>>(mats, maps.map[kSmallGram]);
-    ortho_small_poly_kernel<<<plan.blocks[kSmallPoly], kPolyThreads, kPolyLds, q>>>(mats, maps.map[kSmallPoly], steps, ca, cb, cc, eps);
-    ortho_small_apply_kernel<<<plan.blocks[kSmallApply], kThreads, 0, q>>>(mats, maps.map[kSmallApply]);
+    ortho_small_gram_kernel<<<plan.blocks[kSmallGram], kThreads, 0, q>>>(base, mats, maps.map[kSmallGram]);
+    ortho_small_poly_kernel<<<plan.blocks[kSmallPoly], kPolyThreads, kPolyLds, q>>>(base, mats, maps.map[kSmallPoly], steps, ca, cb, cc, eps);
+    ortho_small_apply_kernel<<<plan.blocks[kSmallApply], kThreads, 0, q>>>(base, mats, maps.map[kSmallApply]);
   }
   if (plan.blocks[kNorm]) {
-    ortho_norm_kernel<<<plan.blocks[kNorm], 256, 0, q>>>(mats, maps.map[kNorm]);
-    ortho_pack_kernel<<<plan.blocks[kPack], 256, 0, q>>>(mats, maps.map[kPack], eps);
-    const Launcher run{plan, mats, maps, q};
+    ortho_norm_kernel<<<plan.blocks[kNorm], 256, 0, q>>>(base, mats, maps.map[kNorm]);
+    ortho_pack_kernel<<<plan.blocks[kPack], 256, 0, q>>>(base, mats, maps.map[kPack], eps);
+    const Launcher run{base, plan, mats, maps, q};
     for (int k = 0; k < steps; ++k) run.step(k & 1 ? kX1 : kX0, k == steps - 1, ca, cb, cc);
   }
   return mr3d_launch_status();
