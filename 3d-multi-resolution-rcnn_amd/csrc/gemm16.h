@@ -19,7 +19,7 @@
 // Tiles go from global memory to LDS with direct loads (16 bytes a lane, no register stop), double buffered, one barrier a k-step.
 // Such a load writes lane l to base + 16 l, so the bank swizzle is applied to the SOURCE address: in a KC tile the 16-byte chunk c of
 // row r sits at slot c ^ ((r >> 1) & 7) (16 consecutive rows read the same c from 16 different bank groups); in a KS tile the 64-byte unit u of
-// k-row r sits at u ^ (r & 3) (the transposing read ds_read_b64_tr_b16 takes 4 k-rows of one unit at a time).
+// k-row r sits at u ^ (r & 3), rows of two units: u ^ (r >> 1 & 1) (the transposing read ds_read_b64_tr_b16 takes 4 k-rows of one unit at a time).
 #pragma once
 #include "mr3d_common.h"
 
@@ -68,6 +68,8 @@ __device__ __forceinline__ Side side_ks(const void *p, long long ldb, long long 
   return {(const char *)p + off, (krows - 1) * ldb + row_bytes - off, T::KK * ldb, (unsigned)ldb};
 }
 
+// the same for the 64-byte units of a KS row of ROWB bytes: four k-rows of a unit lie in four different bank groups
+template <int ROWB> __device__ __forceinline__ int unit_swizzle(int kr) { return ROWB >= 256 ? kr & 3 : (kr >> 1) & 1; }
 template <int RB> __device__ __forceinline__ int swizzle(int row) { return RB == 128 ? (row >> 1) & 7 : (row >> 2) & 3; }
 
 // source byte offset of this lane in load q of the wave (BT = tile extent, NL loads per wave)
@@ -79,9 +81,9 @@ __device__ __forceinline__ unsigned source_offset(int wave, int lane, int q, uns
     const int row = pos / CPR;
     return row * ldb + (((pos % CPR) ^ swizzle<T::RB>(row)) << 4);
   } else {
-    constexpr int CPR = BT * (T::SPLIT ? 4 : 2) / 16;
+    constexpr int ROWB = BT * (T::SPLIT ? 4 : 2), CPR = ROWB / 16;
     const int kr = pos / CPR, c = pos % CPR;
-    return kr * ldb + ((((c >> 2) ^ (kr & 3)) << 6) | ((c & 3) << 4));
+    return kr * ldb + ((((c >> 2) ^ unit_swizzle<ROWB>(kr)) << 6) | ((c & 3) << 4));
   }
 }
 
@@ -117,7 +119,7 @@ __device__ __forceinline__ i16x8 fragment(const char *lds, int b, int ks, int p,
   } else {
     constexpr int ROWB = BT * (T::SPLIT ? 4 : 2);
     const int s = lane & 15, j = s >> 2, unit = T::SPLIT ? b * 2 + p : b;
-    const char *a = lds + (ks * 16 + (lane >> 5) * 8 + j) * ROWB + ((unit ^ j) << 6) + ((lane >> 4) & 1) * 32 + (s & 3) * 8;
+    const char *a = lds + (ks * 16 + (lane >> 5) * 8 + j) * ROWB + ((unit ^ unit_swizzle<ROWB>(j)) << 6) + ((lane >> 4) & 1) * 32 + (s & 3) * 8;
     const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4 *)a);
     const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4 *)(a + 4 * ROWB));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);

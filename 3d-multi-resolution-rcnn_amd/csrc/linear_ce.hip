@@ -537,10 +537,19 @@ __global__ __launch_bounds__(256) void ce_db_kernel(Ce c, int row0) {
   for (int k = 0; k < 8; ++k) t += sum[k][threadIdx.x];
   c.dbpart[(long long)(row0 / kDbRows + slice) * c.classes + o] = F32 ? t / (kSG * ((const float *)c.head)[1]) : t;
 }
-// 64 columns a workgroup, the slices four side by side
-__global__ __launch_bounds__(256) void ce_db_sum_kernel(Ce c, int slices) {
+// The last launch.  Workgroup 0: the loss, row by row in order; the others (want_db): db, 64 columns each, the slices four side by side
+__global__ __launch_bounds__(256) void ce_finish_kernel(Ce c, int slices) {
   __shared__ double sum[4][64];
-  const int col = threadIdx.x & 63, sub = threadIdx.x >> 6, i = blockIdx.x * 64 + col;
+  if (blockIdx.x == 0) {
+    double s = 0;
+    const int live = c.head[0];
+#pragma unroll 4
+    for (int j = threadIdx.x; j < live; j += 256) s += c.row_loss[j];
+    s = block_sum(s, sum[0]);
+    if (threadIdx.x == 0) c.loss[0] = (float)(s / (double)((const float *)c.head)[1]);
+    return;
+  }
+  const int col = threadIdx.x & 63, sub = threadIdx.x >> 6, i = (blockIdx.x - 1) * 64 + col;
   double s = 0;
   if (i < c.classes) {
 #pragma unroll 8
@@ -552,15 +561,6 @@ __global__ __launch_bounds__(256) void ce_db_sum_kernel(Ce c, int slices) {
   s = sum[0][col] + sum[1][col] + sum[2][col] + sum[3][col];
   if (c.db_f32) ((float *)c.db)[i] = (float)s;
   else ((bf16 *)c.db)[i] = (bf16)(float)s;
-}
-
-__global__ __launch_bounds__(256) void ce_loss_kernel(Ce c) {
-  __shared__ double lds[4];
-  double s = 0;
-  const int live = c.head[0];
-  for (int j = threadIdx.x; j < live; j += 256) s += c.row_loss[j];
-  s = block_sum(s, lds);
-  if (threadIdx.x == 0) c.loss[0] = (float)(s / (double)((const float *)c.head)[1]);
 }
 
 // gradients *= *factor, unless the factor is 1 (the usual root of a backward pass): then nothing is read or written
@@ -575,17 +575,25 @@ __global__ __launch_bounds__(256) void ce_scale_kernel(Spans spans, const float 
   }
 }
 
-// Tiles.  256 x 256 (8 waves of 128 x 64, one workgroup a CU) has the fewest LDS bytes per product; it needs enough tiles to fill 256 CUs.
-// 128 x 128 (4 waves of 64 x 64, two workgroups a CU) below that.
+// Tiles.  bf16: 256 x 256 (8 waves of 128 x 64, one workgroup a CU) has the fewest LDS bytes per product; it needs enough tiles to fill 256 CUs.
+// 128 x 128 (4 waves of 64 x 64, two workgroups a CU) below that, and for fp32, whose restarted sums leave no room for the large tile's
+// accumulators.  64 x 64 (three workgroups a CU) where even those would leave CUs without one: 1024^3, fp32: 25 -> 14 us.
 template <bool IKS, bool JKS, bool SPLIT> struct Tiles {
+  typedef Tile<64, 64, 2, 2, IKS, JKS, SPLIT, 128, 3> Tiny;
   typedef Tile<128, 128, 2, 2, IKS, JKS, SPLIT, 128, 2> Small;
   typedef Tile<256, 256, 2, 4, IKS, JKS, SPLIT, 128, 2> Large;
 };
-template <bool IKS, bool JKS> struct Tiles<IKS, JKS, true> {               // no room for two sets of accumulators in the large tile
+template <bool IKS, bool JKS> struct Tiles<IKS, JKS, true> {
+  typedef Tile<64, 64, 2, 2, IKS, JKS, true, 128, 3> Tiny;
   typedef Tile<128, 128, 2, 2, IKS, JKS, true, 128, 2> Small;
   typedef Small Large;
 };
-bool large_tiles(bool f32, long long i, long long j) { return !f32 && ((i + 255) / 256) * ((j + 255) / 256) >= 192; }
+long long tiles_of(long long i, long long j, int bt) { return ((i + bt - 1) / bt) * ((j + bt - 1) / bt); }
+// z: ways the k axis may be split
+int tile_for(bool f32, long long i, long long j, long long z) {
+  if (!f32 && tiles_of(i, j, 256) >= 192) return 256;
+  return tiles_of(i, j, 128) * z >= 160 ? 128 : 64;
+}
 
 long long up(long long v, long long a) { return (v + a - 1) / a * a; }
 
@@ -593,7 +601,8 @@ struct Layout {
   size_t bytes, head, index, pos, xmax, xp, xwp, wp, g, stats, part, row_loss, dwacc, dbpart;
   long long ldx, ldw, ldg;
   int cap, chunks, pieces, z, wcols, db_slices;
-  bool pack_w, big_logits;
+  int bt_logits, bt_dx, bt_dw;
+  bool pack_w;
 };
 
 size_t take(size_t &at, size_t bytes) {
@@ -624,9 +633,9 @@ int layout_of(const mr3d_linear_ce *a, Layout &l) {
     l.chunks = (int)((a->rows + cap - 1) / cap);
   }
   l.cap = (int)cap;
-  l.big_logits = large_tiles(f32, a->classes, cap);
-  l.wcols = l.big_logits ? 128 : 64;
-  l.pieces = (int)(up(a->classes, l.big_logits ? 256 : 128) / l.wcols);
+  l.bt_logits = tile_for(f32, a->classes, cap, 1);
+  l.wcols = l.bt_logits / 2;                                 // a wave's share of a tile
+  l.pieces = (int)(up(a->classes, l.bt_logits) / l.wcols);
   l.head = take(at, 64);
   l.index = take(at, (size_t)a->rows * 4);
   l.pos = take(at, (size_t)a->rows * 4);
@@ -639,13 +648,15 @@ int layout_of(const mr3d_linear_ce *a, Layout &l) {
   if (train) l.g = take(at, (size_t)(cap * l.ldg));
   if (a->want_dx) {
     // parts over the classes until two workgroups a CU have work; a part keeps 16 k-steps
-    const long long tiles = ((a->hidden + 127) / 128) * ((cap + 127) / 128), steps = l.ldg / 128;
-    long long z = tiles >= 512 ? 1 : 512 / tiles;
-    if (large_tiles(f32, a->hidden, cap)) z = 1;
-    if (z > steps / 16) z = steps / 16;
-    l.z = (int)(z < 1 ? 1 : z);
+    const long long steps = l.ldg / 128, most = steps / 16 > 1 ? steps / 16 : 1;
+    l.bt_dx = tile_for(f32, a->hidden, cap, most);
+    const long long tiles = tiles_of(a->hidden, cap, l.bt_dx);
+    long long z = l.bt_dx == 256 || tiles >= 512 ? 1 : 512 / tiles;
+    if (z > most) z = most;
+    l.z = (int)z;
     l.part = take(at, (size_t)l.z * cap * up(a->hidden, 4) * 4);
   }
+  l.bt_dw = tile_for(f32, a->hidden, a->classes, 1);
   if (a->want_dweight && !f32 && l.chunks > 1) l.dwacc = take(at, (size_t)a->classes * a->hidden * 4);
   if (a->want_dbias) {
     l.db_slices = (int)(l.chunks * ((cap + kDbRows - 1) / kDbRows));
@@ -681,6 +692,10 @@ template <class T> int launch_dw(const Ce &c, int row0, int mode, hipStream_t q)
   return MR3D_OK;
 }
 
+template <class TT, class F> int pick(int bt, F f) {
+  return bt == 256 ? f(typename TT::Large()) : bt == 128 ? f(typename TT::Small()) : f(typename TT::Tiny());
+}
+
 template <bool F32> int run_ce(const mr3d_linear_ce *a, const Layout &l, Ce &c, hipStream_t q) {
   const bool train = a->want_dx || a->want_dweight || a->want_dbias;
   typedef Tiles<false, false, F32> TL;
@@ -696,28 +711,27 @@ template <bool F32> int run_ce(const mr3d_linear_ce *a, const Layout &l, Ce &c, 
     const int row0 = k * l.cap;
     int e = MR3D_OK;
     if (train) {
-      e = l.big_logits ? launch_logits<typename TL::Large, true>(c, row0, q) : launch_logits<typename TL::Small, true>(c, row0, q);
+      e = pick<TL>(l.bt_logits, [&](auto t) { return launch_logits<decltype(t), true>(c, row0, q); });
       ce_grad_kernel<F32, true><<<l.cap, 256, 0, q>>>(c, row0, l.wcols);
     } else {
-      e = l.big_logits ? launch_logits<typename TL::Large, false>(c, row0, q) : launch_logits<typename TL::Small, false>(c, row0, q);
+      e = pick<TL>(l.bt_logits, [&](auto t) { return launch_logits<decltype(t), false>(c, row0, q); });
       ce_grad_kernel<F32, false><<<l.cap, 256, 0, q>>>(c, row0, l.wcols);
     }
     if (e) return e;
     if (a->want_dx) {
-      e = large_tiles(F32, a->hidden, l.cap) ? launch_dx<typename TX::Large>(c, row0, q) : launch_dx<typename TX::Small>(c, row0, q);
+      e = pick<TX>(l.bt_dx, [&](auto t) { return launch_dx<decltype(t)>(c, row0, q); });
       if (e) return e;
       ce_dx_rows_kernel<F32><<<a->rows, 256, 0, q>>>(c, row0);
     }
     if (a->want_dweight) {
       const int mode = k ? 2 : (l.chunks > 1 ? 1 : 0);
-      e = large_tiles(F32, a->hidden, a->classes) ? launch_dw<typename TW::Large>(c, row0, mode, q) : launch_dw<typename TW::Small>(c, row0, mode, q);
+      e = pick<TW>(l.bt_dw, [&](auto t) { return launch_dw<decltype(t)>(c, row0, mode, q); });
       if (e) return e;
     }
     if (a->want_dbias) ce_db_kernel<F32><<<dim3((a->classes + 255) / 256, (l.cap + kDbRows - 1) / kDbRows), 256, 0, q>>>(c, row0);
   }
   if (a->want_dweight && l.dwacc) ce_dw_round_kernel<<<2048, 256, 0, q>>>(c.dwacc, (bf16 *)c.dw, (long long)a->classes * a->hidden);
-  if (a->want_dbias) ce_db_sum_kernel<<<(a->classes + 63) / 64, 256, 0, q>>>(c, l.db_slices);
-  ce_loss_kernel<<<1, 256, 0, q>>>(c);
+  ce_finish_kernel<<<1 + (a->want_dbias ? (a->classes + 63) / 64 : 0), 256, 0, q>>>(c, l.db_slices);
   return mr3d_launch_status();
 }
 

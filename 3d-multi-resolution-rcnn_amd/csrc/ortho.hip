@@ -25,8 +25,8 @@ constexpr float kSX = 4096.f, kSA = 4096.f, kSP = 1024.f;
 constexpr int kSmall = 64;                                  // rows of the small path
 constexpr int kThreads = 256;
 
-// 128 x 128 with two tiles in LDS, or 64 x 64 with four, two workgroups a CU each
-template <int BT, bool APPLY, bool FINE> struct Pick { typedef Tile<BT, BT, 2, 2, APPLY, false, true, 128, BT == 128 ? 2 : 4, FINE> T; };
+// 128 x 128 with two tiles in LDS, two workgroups a CU, or 64 x 64 with three and as many workgroups
+template <int BT, bool APPLY, bool FINE> struct Pick { typedef Tile<BT, BT, 2, 2, APPLY, false, true, 128, BT == 128 ? 2 : 3, FINE> T; };
 
 enum Stage { kNorm, kPack, kGram, kGramJoin, kSquare, kSquareJoin, kApply, kApplyJoin, kSmallGram, kSmallPoly, kSmallApply, kStages };
 enum Buf { kA, kP, kX0, kX1, kBufs };
@@ -39,7 +39,7 @@ struct Mat {
   long long in_i, in_j, out_i, out_j;                       // element strides along n (i) and m (j)
   long long buf[kBufs];                                     // planes
   long long part;                                           // parts of split tiles, [tile - whole][z][BT * BT] floats
-  long long norm;                                           // doubles; small path: parts of A, [z][mp][mp], then Q
+  long long norm;                                           // doubles; small path: parts of A, [z][mp][64], then Q
   int m, n, ldx, lda;                                       // ld in bytes
   int bf16, norm_blocks;
   Split gram, square, apply;
@@ -395,14 +395,14 @@ __global__ __launch_bounds__(kThreads) void ortho_small_gram_kernel(char *ws, co
           acc[b] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)t[bi[b] * 16 + r][k + kq], (double)t[bj[b] * 16 + r][k + kq], acc[b], 0, 0, 0);
     }
   }
-  double *o = at<double>(ws, p->norm) + (long long)zi * mp * mp;
+  double *o = at<double>(ws, p->norm) + zi * mp * kSmall;
 #pragma unroll
   for (int b = 0; b < 3; ++b)
     if (wave + 4 * b < blocks)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = bi[b] * 16 + 4 * e + kq, j = bj[b] * 16 + r;
-        if (i >= j) o[i * mp + j] = acc[b][e];
+        if (i >= j) o[i * kSmall + j] = acc[b][e];
       }
 }
 
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(kPolyThreads) void ortho_small_poly_kernel(char *ws
   double *a = mats4[0];
   double s[4] = {0, 0, 0, 0};                               // 4 elements a thread, 32 loads in flight
   const double *part = at<double>(ws, p->norm);
-  const int size = mp * mp;
+  const int size = mp * kSmall;                             // rows of 64: no divisions
   for (int z0 = 0; z0 < z; z0 += 8) {
     double v[8][4];
 #pragma unroll
@@ -480,7 +480,7 @@ __global__ __launch_bounds__(kPolyThreads) void ortho_small_poly_kernel(char *ws
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int e = threadIdx.x + k * kPolyThreads;
-        v[y][k] = e < size && z0 + y < z ? part[(z0 + y) * size + e] : 0.;
+        v[y][k] = e < size && e / kSmall >= e % kSmall && z0 + y < z ? part[(z0 + y) * size + e] : 0.;
       }
 #pragma unroll
     for (int y = 0; y < 8; ++y)
@@ -489,7 +489,7 @@ __global__ __launch_bounds__(kPolyThreads) void ortho_small_poly_kernel(char *ws
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const int e = threadIdx.x + k * kPolyThreads, i = e / mp, j = e % mp;
+    const int e = threadIdx.x + k * kPolyThreads, i = e / kSmall, j = e % kSmall;
     if (e < size && i >= j) a[i * kLdd + j] = a[j * kLdd + i] = s[k];
   }
   __syncthreads();
@@ -501,7 +501,8 @@ __global__ __launch_bounds__(kPolyThreads) void ortho_small_poly_kernel(char *ws
   }
   __syncthreads();
   const double inv = 1. / (sqrt(trace) + (double)eps);
-  for (int k = threadIdx.x; k < size; k += kPolyThreads) a[k / mp * kLdd + k % mp] *= inv * inv;
+  for (int k = threadIdx.x; k < size; k += kPolyThreads)
+    if (k % kSmall < mp) a[k / kSmall * kLdd + k % kSmall] *= inv * inv;
   int q;
   switch (mp / 16) {
     case 1: q = small_steps<1>(mats4, steps, ca, cb, cc); break;
@@ -509,8 +510,9 @@ __global__ __launch_bounds__(kPolyThreads) void ortho_small_poly_kernel(char *ws
     case 3: q = small_steps<3>(mats4, steps, ca, cb, cc); break;
     default: q = small_steps<4>(mats4, steps, ca, cb, cc);
   }
-  double *o = at<double>(ws, p->norm) + (long long)z * size;
-  for (int k = threadIdx.x; k < size; k += kPolyThreads) o[k] = mats4[q][k / mp * kLdd + k % mp] * inv;
+  double *o = at<double>(ws, p->norm) + z * size;
+  for (int k = threadIdx.x; k < size; k += kPolyThreads)
+    if (k % kSmall < mp) o[k] = mats4[q][k / kSmall * kLdd + k % kSmall] * inv;
 }
 
 // out = Q G, 64 columns a workgroup, in double too: Q reaches a^steps in the directions of small singular values, and its rounding to fp32 would show in
@@ -520,11 +522,11 @@ __global__ __launch_bounds__(kThreads) void ortho_small_apply_kernel(char *ws, c
   __shared__ double q[kSmall][kSmall + 2];
   const Mat *__restrict__ p = mats + map[blockIdx.x];
   const int m = p->m, n = p->n, mp = pad16(m), nb = mp / 16, i0 = (blockIdx.x - p->first[kSmallApply]) * kChunk;
-  const double *qs = at<double>(ws, p->norm) + (long long)p->gram.z * mp * mp;
+  const double *qs = at<double>(ws, p->norm) + p->gram.z * mp * kSmall;
 #pragma unroll
   for (int k = 0; k < kSmall * kSmall / kThreads; ++k) {
     const int e = threadIdx.x + k * kThreads;
-    if (e < mp * mp) q[e / mp][e % mp] = qs[e];
+    if (e / kSmall < mp && e % kSmall < mp) q[e / kSmall][e % kSmall] = qs[e];
   }
   load_tile(ws, p, i0, 0, t);
   __syncthreads();
@@ -549,8 +551,9 @@ __global__ __launch_bounds__(kThreads) void ortho_small_apply_kernel(char *ws, c
   const long long oi = p->out_i, oj = p->out_j;
   const int f32 = !p->bf16;
   char *out = ws + p->out;
-  for (int k = threadIdx.x; k < mp * kChunk; k += kThreads) {
-    const int c = wide ? k % kChunk : k / mp, j = wide ? k / kChunk : k % mp;
+#pragma unroll 4
+  for (int k = threadIdx.x; k < kSmall * kChunk; k += kThreads) {
+    const int c = wide ? k % 64 : k / 64, j = wide ? k / 64 : k % 64;
     if (j >= m || i0 + c >= n) continue;
     const long long e = j * oj + (i0 + c) * oi;
     if (f32) ((float *)out)[e] = t[j][c];
@@ -564,25 +567,26 @@ size_t take(size_t &at, size_t bytes) {
   return here;
 }
 
-// Splitting.  512 workgroups are resident (two a CU).  Fewer tiles than that in the whole list: each is split so that the chip is full, as long as a part
-// keeps 16 k-steps (a part costs a trip of its tile through memory).  More: what is left over after whole rounds would leave most of the chip idle for a
-// round; those tiles are split, down to 4 k-steps (4096 x 4096: 528 tiles on and below the diagonal, 238 -> 140 us a product).
-constexpr int kResident = 512;
-Split split_for(long long tiles, long long list_tiles, bool carries_rest, int steps) {
-  long long whole = tiles, z = 1;
-  if (list_tiles < kResident) {
-    z = kResident / list_tiles;
-    if (z > steps / 16) z = steps / 16;
-    if (z > 1) whole = 0;
-  } else if (carries_rest) {
-    const long long rest = list_tiles % kResident;
-    if (rest && rest <= tiles) {
-      z = kResident / rest;
-      if (z > steps / 4) z = steps / 4;
-      if (z > 1) whole = tiles - rest;
+// Splitting.  `resident` workgroups run at a time (512 of the 128-wide tiles, 768 of the 64-wide ones); what is left over after whole rounds of them leaves
+// most of the chip idle for a round.  Those tiles -- all tiles of a list that does not fill one round, else tiles of the list's largest matrix -- are
+// computed by z workgroups each, for the z with the least estimated time: a round of z-th parts takes 1.45 us a k-step (64-wide: 0.5) over z,
+// the parts travel through memory and back at 4 TB/s, their join is a launch of 6 us (4096 x 4096: 528 tiles on and below the diagonal, 238 -> 215 us).
+Split split_for(long long tiles, long long list_tiles, bool carries_rest, int steps, int bt) {
+  const long long resident = bt == 128 ? 512 : 768, rest = list_tiles < resident ? list_tiles : list_tiles % resident;
+  const bool all = list_tiles < resident;
+  Split s{(int)tiles, (int)tiles, 1};
+  if (!rest || (!all && (!carries_rest || rest > tiles))) return s;
+  const double tile_us = steps * (bt == 128 ? 1.45 : 0.5), part_us = bt * bt * 8. / 4e6;
+  double best = tile_us;
+  for (int z = 2; z <= 32 && z <= steps / 4; ++z) {
+    const double us = tile_us * (double)((rest * z + resident - 1) / resident) / z + part_us * (double)rest * z + 6.;
+    if (us < best) {
+      best = us;
+      s.z = z;
+      s.whole = (int)(all ? 0 : tiles - rest);
     }
   }
-  return {(int)tiles, (int)whole, (int)(z < 1 ? 1 : z)};
+  return s;
 }
 int split_blocks(const Split &s) { return s.whole + (s.tiles - s.whole) * s.z; }
 
@@ -637,7 +641,7 @@ int plan_list(const mr3d_matrix *in, int count, char *base, Plan &plan, Mat *mat
       // a share of A takes at least 64 columns, at most 32 shares (one workgroup adds them up)
       const int chunks = (p.n + kChunk - 1) / kChunk, mp = (p.m + 15) / 16 * 16;
       p.gram.z = chunks < 32 ? chunks : 32;
-      p.norm = take(at, ((size_t)p.gram.z + 1) * mp * mp * 8);
+      p.norm = take(at, ((size_t)p.gram.z + 1) * mp * kSmall * 8);
       need[kSmallGram] = p.gram.z;
       need[kSmallPoly] = 1;
       need[kSmallApply] = chunks;
@@ -647,9 +651,9 @@ int plan_list(const mr3d_matrix *in, int count, char *base, Plan &plan, Mat *mat
       const long long tg = (p.m + plan.bt_gram - 1) / plan.bt_gram, ts = (p.m + plan.bt_square - 1) / plan.bt_square, tm = (p.m + plan.bt_apply - 1) / plan.bt_apply, tn = (p.n + plan.bt_apply - 1) / plan.bt_apply;
       const int ksm = (p.m + 31) / 32, ksn = (p.n + 31) / 32, qg = plan.bt_gram == 128 ? 4 : 1, qs = plan.bt_square == 128 ? 4 : 1, qa = plan.bt_apply == 128 ? 4 : 1;
       if (ts * (ts + 1) / 2 > 0x3fffffff || tg * (tg + 1) / 2 > 0x3fffffff || tm * tn > 0x3fffffff) return MR3D_ERR_UNSUPPORTED;
-      p.gram = split_for(tg * (tg + 1) / 2, list_gram, k == sum.carrier, ksn);
-      p.square = split_for(ts * (ts + 1) / 2, list_sym, k == sum.carrier, ksm);
-      p.apply = split_for(tm * tn, list_apply, k == sum.carrier, ksm);
+      p.gram = split_for(tg * (tg + 1) / 2, list_gram, k == sum.carrier, ksn, plan.bt_gram);
+      p.square = split_for(ts * (ts + 1) / 2, list_sym, k == sum.carrier, ksm, plan.bt_square);
+      p.apply = split_for(tm * tn, list_apply, k == sum.carrier, ksm, plan.bt_apply);
       const long long numel = (long long)p.m * p.n;
       p.norm_blocks = (int)((numel + 8191) / 8192 > 1024 ? 1024 : (numel + 8191) / 8192);
       for (int b = 0; b < kBufs; ++b) {
