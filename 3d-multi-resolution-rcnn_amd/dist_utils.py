@@ -245,6 +245,16 @@ class DetectorArena:
             out += [(base + lo, base + hi) for (lo, hi), t in zip(self.heads.ranges, self.heads.touched) if not t]
         return out
 
+    def matrices(self):
+        """[(offset, shape)] in flat_params of every trainable tensor with two or more axes (a convolution counts as [Cout, Cin * taps])"""
+        out, base = [], 0
+        if self.engine is not None:
+            out = [(self.engine.rel_offsets[name], shape) for name, shape in self.engine._arena_entries()[0] if len(shape) > 1]
+            base = self.engine.num_trainable
+        if self.heads is not None:
+            out += [(base + lo, tuple(p.shape)) for p, (lo, _) in zip(self.heads.params, self.heads.ranges) if p.dim() > 1]
+        return out
+
     def touch_version(self):
         return (self.heads.version if self.heads is not None else 0,
                 bool(getattr(self.engine, 'grads_touched', True)) if self.engine is not None else True)
@@ -315,6 +325,48 @@ class ArenaSGD:
     def load_state_dict(self, sd):
         self.momentum_buffer.copy_(sd['momentum_buffer'])
         self.param_groups[0].update(sd['param_groups'][0])
+
+
+class ArenaMuon(ArenaSGD):
+    """Orthogonalised updates for the weight matrices of a DetectorArena, SGD with momentum for everything else (biases, normalisation, and
+    matrices with fewer than `min_rows` rows or columns: score and delta layers).  With v = momentum v + grad and d = grad + momentum v (Nesterov):
+        matrix [m, n]:  W -= lr (sqrt(max(1, m / n)) orthogonalize(d) + weight_decay W)
+        others:         w -= lr (other_lr d + weight_decay w)
+    All matrices go through core.orthogonalize as one list (csrc/ortho.hip: one launch per stage), in place in one flat buffer.  Same interface
+    and the same treatment of parameters that have never received a gradient as ArenaSGD (no decay, no update until the first one)."""
+
+    def __init__(self, arena, lr, momentum=0.95, weight_decay=0.0, other_lr=0.05, min_rows=16, steps=5):
+        super().__init__(arena, lr, momentum, weight_decay)
+        self.steps = steps
+        self._gain = torch.full_like(arena.flat_params, other_lr)
+        self._mats = []
+        for off, shape in arena.matrices():
+            rows = shape[0]
+            n = 1
+            for v in shape:
+                n *= v
+            if min(rows, n // rows) < min_rows:
+                continue
+            self._gain[off:off + n] = max(1.0, rows * rows / n) ** 0.5
+            self._mats.append(self._d[off:off + n].view(rows, n // rows))
+
+    @torch.no_grad()
+    def step(self):
+        from .core.orthogonalize import orthogonalize
+        g = self.param_groups[0]
+        p, grad, buf, d = self.arena.flat_params, self.arena.flat_grads, self.momentum_buffer, self._d
+        buf.mul_(g['momentum']).add_(grad)
+        torch.add(grad, buf, alpha=g['momentum'], out=d)
+        orthogonalize(self._mats, steps=self.steps, out=self._mats)
+        mask = self._active_mask()
+        if g['weight_decay'] != 0:
+            if mask is None:
+                p.mul_(1 - g['lr'] * g['weight_decay'])
+            else:
+                p.addcmul_(p, mask, value=-g['lr'] * g['weight_decay'])
+        if mask is not None:
+            d.mul_(mask)                                            # never touched: a zero gradient, but also after a foreign write to it
+        p.addcmul_(d, self._gain, value=-g['lr'])
 
 
 def _allreduce_coalesced(tensors, world_size, bucket_size_mb=-1, group=None):

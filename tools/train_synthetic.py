@@ -23,7 +23,7 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 import mr3d_amd  # noqa: E402
 from mr3d_amd.datasets import prepare_volume  # noqa: E402
 from mr3d_amd.detector import TwoStageDetector3D2Scales  # noqa: E402
-from mr3d_amd.dist_utils import ArenaSGD, DetectorArena, broadcast_params, train_step  # noqa: E402
+from mr3d_amd.dist_utils import ArenaMuon, ArenaSGD, DetectorArena, broadcast_params, train_step  # noqa: E402
 
 
 def synthetic_sample(rng, D, H, W, dev, n_gt=6):
@@ -49,6 +49,7 @@ def main():
     ap.add_argument('--lr', type=float, default=0.001)          # configs/...py:235 (SGD lr 0.001, momentum 0.9, wd 1e-4)
     ap.add_argument('--bf16', action='store_true', help='BASELINE configs[4]: bf16 activation storage')
     ap.add_argument('--dcn-neck', action='store_true', help='BASELINE configs[4]: DeformConv3d neck')
+    ap.add_argument('--optimizer', choices=('sgd', 'muon'), default='sgd', help='muon: orthogonalised updates of the weight matrices (ArenaMuon)')
     a = ap.parse_args()
     D, H, W = (int(v) for v in a.vol.split(','))
     rank, local, world = (int(os.environ.get(k, d)) for k, d in (('RANK', 0), ('LOCAL_RANK', 0), ('WORLD_SIZE', 1)))
@@ -62,7 +63,7 @@ def main():
     det.extract.init_weights()
     arena = DetectorArena(det)
     broadcast_params(arena.flat_params)                          # identical initial weights (mmcv DDP init)
-    opt = ArenaSGD(arena, lr=a.lr, momentum=0.9, weight_decay=1e-4)
+    opt = ArenaSGD(arena, lr=a.lr, momentum=0.9, weight_decay=1e-4) if a.optimizer == 'sgd' else ArenaMuon(arena, lr=a.lr, weight_decay=1e-4)
     rng = np.random.default_rng(100 + rank)                      # every rank draws its own volumes (DistributedSampler)
     t0 = time.perf_counter()
     for it in range(a.iters):
