@@ -10,11 +10,14 @@
 //
 // Split products are hi*hi + hi*lo + lo*hi in fp32 accumulators: what is dropped (lo*lo and the 23rd bit) is 2^-22 of a product, below the
 // rounding of an fp32 sum, for three passes of the fp16 pipe -- whose rate is 16 times the fp32 pipe's.
-// The matrix instruction aligns its 16 products and the accumulator to the largest of them and drops what lies 2 bits below that one's last place (16
+// The matrix instruction aligns its products and the accumulator to the largest of them and drops what lies 2 bits below that one's last place (16
 // products of 1/16 ulp of the accumulator add nothing), so a long sum of one sign drifts: 1e-5 of a sum of 3456 squares, 4e-5 of 9408.  Split
 // products therefore add the accumulators up in fp32 every 128 k and start again from zero: 3e-7 at any length, less than plain fp32 sums lose.
-// FINE ones do so every 16 k (6e-8; 10 % slower on the 128 x 128 tile: 16 additions for 3 products).
+// FINE ones do so every 32 k (1e-7; 10 % slower on the 128 x 128 tile).
 // bf16 products leave it at that: their results are rounded to 2^-9.
+//
+// v_mfma_f32_16x16x32 rather than 32x32x16: the chip is bound by power under such products, and the smaller shape sustains 1656 TFLOP/s from registers where
+// the larger one does 1510 (random operands).  8192^3, bf16, 256 x 256 tiles: 1330 TFLOP/s in all three operand orientations (1260 with 32x32x16).
 //
 // Tiles go from global memory to LDS with direct loads (16 bytes a lane, no register stop), double buffered, one barrier a k-step.
 // Such a load writes lane l to base + 16 l, so the bank swizzle is applied to the SOURCE address: in a KC tile the 16-byte chunk c of
@@ -25,7 +28,7 @@
 
 namespace gemm16 {
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
@@ -43,16 +46,16 @@ template <int BI_, int BJ_, int NWI_, int NWJ_, bool IKS_, bool JKS_, bool SPLIT
   static constexpr int BI = BI_, BJ = BJ_, NWI = NWI_, NWJ = NWJ_, NW = NWI * NWJ, THREADS = NW * 64;
   static constexpr bool IKS = IKS_, JKS = JKS_, SPLIT = SPLIT_, FINE = FINE_;
   static constexpr int RB = RB_, STAGES = STAGES_;                          // bytes of a KC row per k-step, tiles in LDS
-  static constexpr int TI = BI / NWI / 32, TJ = BJ / NWJ / 32;              // 32 x 32 blocks of a wave
+  static constexpr int TI = BI / NWI / 16, TJ = BJ / NWJ / 16;              // 16 x 16 blocks of a wave
   static constexpr int IBYTES = BI * RB, JBYTES = BJ * RB, STAGE = IBYTES + JBYTES, LDS_BYTES = STAGES * STAGE;
   static constexpr int KK = SPLIT ? RB / 4 : RB / 2;                        // k of a k-step
   static constexpr int NLI = IBYTES / 1024 / NW, NLJ = JBYTES / 1024 / NW;  // 1 KB loads of a wave per k-step
   static constexpr int RESTART = !SPLIT || FINE ? 0 : 128 / KK;// k-steps between two restarts of the accumulators (0: never)
   static_assert(SPLIT || !FINE, "");
-  static_assert(!SPLIT || TI * TJ <= 4, "accumulators and their sums fit the registers");
+  static_assert(!SPLIT || TI * TJ <= 16, "accumulators and their sums fit the registers");
   static_assert(IBYTES % (1024 * NW) == 0 && JBYTES % (1024 * NW) == 0, "whole 1 KB loads per wave");
   static_assert(RB == 128 || (RB == 64 && !SPLIT), "a split row's group is 128 bytes");
-  static_assert(KK % 32 == 0, "fragment buffers alternate");
+  static_assert(KK % 32 == 0, "whole matrix instructions");
 };
 
 // KC: rows [row0, rows) of `row_bytes` bytes (padding to the k-step included), from k-step kstep0 on
@@ -68,8 +71,12 @@ __device__ __forceinline__ Side side_ks(const void *p, long long ldb, long long 
   return {(const char *)p + off, (krows - 1) * ldb + row_bytes - off, T::KK * ldb, (unsigned)ldb};
 }
 
-// the same for the 64-byte units of a KS row of ROWB bytes: four k-rows of a unit lie in four different bank groups
-template <int ROWB> __device__ __forceinline__ int unit_swizzle(int kr) { return ROWB >= 256 ? kr & 3 : (kr >> 1) & 1; }
+// the same for the 16-byte chunk c of k-row kr in a KS tile with rows of ROWB bytes: four k-rows of a 64-byte unit lie in four different bank
+// groups, and k-rows 8 apart in the two halves of one
+template <int ROWB> __device__ __forceinline__ int place(int kr, int c) {
+  const int u = ROWB >= 256 ? kr & 3 : (kr >> 1) & 1;
+  return c ^ (u << 2) ^ (((kr >> 3) & 1) << 1);
+}
 template <int RB> __device__ __forceinline__ int swizzle(int row) { return RB == 128 ? (row >> 1) & 7 : (row >> 2) & 3; }
 
 // source byte offset of this lane in load q of the wave (BT = tile extent, NL loads per wave)
@@ -83,7 +90,7 @@ __device__ __forceinline__ unsigned source_offset(int wave, int lane, int q, uns
   } else {
     constexpr int ROWB = BT * (T::SPLIT ? 4 : 2), CPR = ROWB / 16;
     const int kr = pos / CPR, c = pos % CPR;
-    return kr * ldb + ((((c >> 2) ^ unit_swizzle<ROWB>(kr)) << 6) | ((c & 3) << 4));
+    return kr * ldb + (place<ROWB>(kr, c) << 4);
   }
 }
 
@@ -110,45 +117,38 @@ __device__ __forceinline__ void stage_load(const Side &s, const unsigned (&off)[
   for (int q = 0; q < NL; ++q) load_to_lds(rsrc, off[q], lds + q * 1024);
 }
 
-// fragment of 32 rows (block `b` of the tile) x 16 k (substep ks, plane p): lane l holds row l % 32, k = 8 (l / 32) + 0..7
+// fragment of 16 rows (block `b` of the tile) x 32 k (substep ks, plane p): lane l holds row l % 16, k = 8 (l / 16) + 0..7
 template <class T, int BT, bool KS>
 __device__ __forceinline__ i16x8 fragment(const char *lds, int b, int ks, int p, int lane) {
   if constexpr (!KS) {
-    const int row = lane & 31, chunk = (T::SPLIT ? p * 4 : 0) + ks * 2 + (lane >> 5);
-    return *reinterpret_cast<const i16x8 *>(lds + b * 32 * T::RB + row * T::RB + ((chunk ^ swizzle<T::RB>(row)) << 4));
+    const int row = b * 16 + (lane & 15), chunk = (T::SPLIT ? p * 4 : 0) + ks * 4 + (lane >> 4);
+    return *reinterpret_cast<const i16x8 *>(lds + row * T::RB + ((chunk ^ swizzle<T::RB>(row)) << 4));
   } else {
     constexpr int ROWB = BT * (T::SPLIT ? 4 : 2);
-    const int s = lane & 15, j = s >> 2, unit = T::SPLIT ? b * 2 + p : b;
-    const char *a = lds + (ks * 16 + (lane >> 5) * 8 + j) * ROWB + ((unit ^ unit_swizzle<ROWB>(j)) << 6) + ((lane >> 4) & 1) * 32 + (s & 3) * 8;
-    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4 *)a);
-    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4 *)(a + 4 * ROWB));
+    const int s = lane & 15, kr = ks * 32 + (lane >> 4) * 8 + (s >> 2);
+    // 16 columns: half a unit; split: the unit pairs of a group of 32 columns are its hi and its lo
+    const int chunk = (T::SPLIT ? (b >> 1) * 8 + p * 4 : (b >> 1) * 4) + (b & 1) * 2 + ((s & 3) >> 1);
+    const char *a = lds + kr * ROWB + (s & 1) * 8;
+    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4 *)(a + (place<ROWB>(kr, chunk) << 4)));
+    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4 *)(a + 4 * ROWB + (place<ROWB>(kr + 4, chunk) << 4)));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 }
 
 template <bool SPLIT>
-__device__ __forceinline__ f32x16 mfma(i16x8 a, i16x8 b, f32x16 c) {
-  if constexpr (SPLIT) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+__device__ __forceinline__ f32x4 mfma(i16x8 a, i16x8 b, f32x4 c) {
+  if constexpr (SPLIT) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-template <class T> __device__ __forceinline__ void interleave() {
-  constexpr int M = T::TI * T::TJ * (T::SPLIT ? 3 : 1), R = (T::TI * (T::IKS ? 2 : 1) + T::TJ * (T::JKS ? 2 : 1)) * (T::SPLIT ? 2 : 1);
-  constexpr int PER = (R + M - 1) / M;
-#pragma unroll
-  for (int k = 0; k < M; ++k) {
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
-  }
-}
-
-// acc[ti][tj][e] of wave (wi, wj), lane l:  i = (wi TI + ti) 32 + 8 (e / 4) + 4 (l / 32) + e % 4,  j = (wj TJ + tj) 32 + l % 32
+// acc[ti][tj][e] of wave (wi, wj), lane l:  i = (wi TI + ti) 16 + 4 (l / 16) + e,  j = (wj TJ + tj) 16 + l % 16
 //
 // STAGES - 1 k-steps are on their way while one is multiplied (a trip to L2 or HBM is longer than a k-step of 0.3 - 0.9 us).  Loads past the
 // last k-step are issued with an empty range (zeros into a tile nobody reads), so that the count of outstanding loads is the same in every step.
-// A wave reads the fragments of the next 16 k before it multiplies the current ones, across the barrier of a k-step too.
+// A wave keeps the J fragments of the current 32 k and the next in registers and passes its I fragments by, AHEAD of them read in advance,
+// across the barrier of a k-step too; the reads go between the products (a wave that queues LDS reads issues nothing else).
 template <class T>
-__device__ __forceinline__ void run(char *lds, Side si, Side sj, int nsteps, f32x16 (&acc)[T::TI][T::TJ]) {
+__device__ __forceinline__ void run(char *lds, Side si, Side sj, int nsteps, f32x4 (&acc)[T::TI][T::TJ]) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave % T::NWI, wj = wave / T::NWI;
   unsigned oi[T::NLI], oj[T::NLJ];
@@ -156,12 +156,11 @@ __device__ __forceinline__ void run(char *lds, Side si, Side sj, int nsteps, f32
   for (int q = 0; q < T::NLI; ++q) oi[q] = source_offset<T, T::BI, T::NLI, T::IKS>(wave, lane, q, si.ldb);
 #pragma unroll
   for (int q = 0; q < T::NLJ; ++q) oj[q] = source_offset<T, T::BJ, T::NLJ, T::JKS>(wave, lane, q, sj.ldb);
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int a = 0; a < T::TI; ++a)
 #pragma unroll
-    for (int b = 0; b < T::TJ; ++b)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.f;
+    for (int b = 0; b < T::TJ; ++b) acc[a][b] = zero;
   if (nsteps <= 0) return;
   int to_load = nsteps;
   const unsigned lds0 = __builtin_amdgcn_readfirstlane((int)(uintptr_t)(__attribute__((address_space(3))) char *)lds);
@@ -172,82 +171,93 @@ __device__ __forceinline__ void run(char *lds, Side si, Side sj, int nsteps, f32
     si.base += si.step; si.left -= si.step;
     sj.base += sj.step; sj.left -= sj.step;
   };
-  constexpr int NP = T::SPLIT ? 2 : 1, KS = T::KK / 16;
-  i16x8 fi[2][T::TI][NP], fj[2][T::TJ][NP];
-  auto fetch = [&](int which, int buf, int ks) {
-    const char *li = lds + buf * T::STAGE, *lj = li + T::IBYTES;
+  constexpr int NP = T::SPLIT ? 2 : 1, KS = T::KK / 32, POS = KS * T::TI;   // positions of a k-step: (substep, I block)
+  constexpr int AHEAD = T::TI < 3 ? T::TI : 3;
+  i16x8 fi[AHEAD + 1][NP], fj[2][T::TJ][NP];
+  auto fetch_i = [&](int slot, int buf, int pos) {
 #pragma unroll
-    for (int p = 0; p < NP; ++p) {
+    for (int p = 0; p < NP; ++p) fi[slot][p] = fragment<T, T::BI, T::IKS>(lds + buf * T::STAGE, wi * T::TI + pos % T::TI, pos / T::TI, p, lane);
+  };
+  auto fetch_j = [&](int which, int buf, int ks, int b) {
 #pragma unroll
-      for (int b = 0; b < T::TJ; ++b) fj[which][b][p] = fragment<T, T::BJ, T::JKS>(lj, wj * T::TJ + b, ks, p, lane);
-#pragma unroll
-      for (int a = 0; a < T::TI; ++a) fi[which][a][p] = fragment<T, T::BI, T::IKS>(li, wi * T::TI + a, ks, p, lane);
-    }
+    for (int p = 0; p < NP; ++p) fj[which][b][p] = fragment<T, T::BJ, T::JKS>(lds + buf * T::STAGE + T::IBYTES, wj * T::TJ + b, ks, p, lane);
   };
 #pragma unroll
   for (int k = 0; k < T::STAGES - 1; ++k) load(k);
   // outstanding loads that may remain when stage s + 1 is needed: those of stages s + 2 .. s + STAGES - 1
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"((T::STAGES - 2) * (T::NLI + T::NLJ)) : "memory");
   __builtin_amdgcn_s_barrier();
-  if constexpr (T::STAGES == 2) load(1);
-  else load(T::STAGES - 1);
-  fetch(0, 0, 0);
+  load(T::STAGES - 1);
+#pragma unroll
+  for (int b = 0; b < T::TJ; ++b) fetch_j(0, 0, 0, b);
+#pragma unroll
+  for (int x = 0; x < AHEAD; ++x) fetch_i(x, 0, x);
   int buf = 0;
-  f32x16 sum[T::TI][T::TJ];
+  f32x4 sum[T::TI][T::TJ];
   if constexpr (T::RESTART) {
 #pragma unroll
     for (int a = 0; a < T::TI; ++a)
 #pragma unroll
-      for (int b = 0; b < T::TJ; ++b) sum[a][b] = acc[a][b];
+      for (int b = 0; b < T::TJ; ++b) sum[a][b] = zero;
   }
-  for (int s = 0; s < nsteps; ++s) {
-    const int next = buf + 1 == T::STAGES ? 0 : buf + 1;
+  // registers have no index: a k-step is unrolled as often as it takes for its fragments to sit in the same registers again
+  constexpr int RING = POS % (AHEAD + 1) == 0 ? 1 : (2 * POS) % (AHEAD + 1) == 0 ? 2 : AHEAD + 1;
+  constexpr int UNR = RING * KS % 2 == 0 ? RING : 2 * RING;
+  for (int s0 = 0; s0 < nsteps; s0 += UNR) {
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      if (ks + 1 < KS) {
-        fetch((ks + 1) & 1, buf, ks + 1);
-      } else {
-        // this wave's last fragments of stage s are in registers and its loads of stage s + 1 have landed: behind the barrier both hold for
-        // every wave, stage s's tile is free
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((T::STAGES - 2) * (T::NLI + T::NLJ)) : "memory");
-        __builtin_amdgcn_s_barrier();
-        load(buf);
-        fetch(0, next, 0);
-      }
-      const int w = ks & 1;
+    for (int u = 0; u < UNR; ++u) {
+      if (UNR > 1 && s0 + u >= nsteps) break;
+      const int next = buf + 1 == T::STAGES ? 0 : buf + 1;
 #pragma unroll
-      for (int a = 0; a < T::TI; ++a)
+      for (int pos = 0; pos < POS; ++pos) {
+        const int g = u * POS + pos, ahead = pos + AHEAD, ks = pos / T::TI, a = pos % T::TI, w = (u * KS + ks) & 1, slot = g % (AHEAD + 1);
+        if (ahead == POS) {
+          // this wave's last fragments of the step are in registers and its loads of the next stage have landed: behind the barrier both hold for
+          // every wave, the step's tile is free
+          asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((T::STAGES - 2) * (T::NLI + T::NLJ)) : "memory");
+          __builtin_amdgcn_s_barrier();
+          load(buf);
+        }
+        const bool over = ahead >= POS;
+        fetch_i((g + AHEAD) % (AHEAD + 1), over ? next : buf, over ? ahead - POS : ahead);
+        // the J fragments of the next substep, a share per position; those of the next k-step behind the barrier
+        const bool last_ks = ks == KS - 1;
+        const int from = last_ks ? T::TI - AHEAD : 0, share = (T::TJ + T::TI - from - 1) / (T::TI - from);
+        if (a >= from) {
+#pragma unroll
+          for (int b = 0; b < T::TJ; ++b)
+            if (b / share == a - from) fetch_j(w ^ 1, last_ks ? next : buf, last_ks ? 0 : ks + 1, b);
+        }
 #pragma unroll
         for (int b = 0; b < T::TJ; ++b) {
-          f32x16 t = acc[a][b];
-          if constexpr (T::FINE) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) t[e] = 0.f;
-          }
+          f32x4 t = T::FINE ? zero : acc[a][b];
           if constexpr (T::SPLIT) {                        // small terms first: one rounding at the size of the result instead of three
-            t = mfma<true>(fi[w][a][0], fj[w][b][1], t);
-            t = mfma<true>(fi[w][a][1], fj[w][b][0], t);
+            t = mfma<true>(fi[slot][0], fj[w][b][1], t);
+            t = mfma<true>(fi[slot][1], fj[w][b][0], t);
           }
-          t = mfma<T::SPLIT>(fi[w][a][0], fj[w][b][0], t);
+          t = mfma<T::SPLIT>(fi[slot][0], fj[w][b][0], t);
           if constexpr (T::FINE) acc[a][b] += t;
           else acc[a][b] = t;
         }
-      // the reads go between the products, not in front of them: a wave that queues LDS reads issues nothing else
-      interleave<T>();
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    buf = next;
-    if constexpr (T::RESTART) {
-      if ((s + 1) % T::RESTART == 0) {
+        constexpr int M = T::TJ * (T::SPLIT ? 3 : 1);
 #pragma unroll
-        for (int a = 0; a < T::TI; ++a)
+        for (int m = 0; m < M; ++m) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      buf = next;
+      if constexpr (T::RESTART) {
+        if ((s0 + u + 1) % T::RESTART == 0) {
 #pragma unroll
-          for (int b = 0; b < T::TJ; ++b)
+          for (int a = 0; a < T::TI; ++a)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              sum[a][b][e] += acc[a][b][e];
-              acc[a][b][e] = 0.f;
+            for (int b = 0; b < T::TJ; ++b) {
+              sum[a][b] += acc[a][b];
+              acc[a][b] = zero;
             }
+        }
       }
     }
   }
@@ -255,9 +265,7 @@ __device__ __forceinline__ void run(char *lds, Side si, Side sj, int nsteps, f32
 #pragma unroll
     for (int a = 0; a < T::TI; ++a)
 #pragma unroll
-      for (int b = 0; b < T::TJ; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[a][b][e] += sum[a][b][e];
+      for (int b = 0; b < T::TJ; ++b) acc[a][b] += sum[a][b];
   }
   // the fragments read last belong to no k-step; the loads of empty ranges must not land in what LDS holds next
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");

@@ -203,84 +203,79 @@ __global__ __launch_bounds__(T::THREADS, 2) void ce_logits_kernel(Ce c, int row0
   if ((int)blockIdx.x >= nti * ntj) return;
   int ti, tj;
   tile_of(blockIdx.x, nti * ntj, nti, ntj, ti, tj);
-  f32x16 acc[T::TI][T::TJ];
+  f32x4 acc[T::TI][T::TJ];
   run<T>(lds, side_kc<T>(c.wp, c.ldw, c.classes, c.ldx, ti * T::BI, 0), side_kc<T>(c.xp + row0 * c.ldx, c.ldx, live, c.ldx, tj * T::BJ, 0),
          (int)(c.ldx / 128), acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave % T::NWI, wj = wave / T::NWI;
   const float rsw = T::SPLIT ? kLog2e / scale_of(c, 2) : kLog2e;
   const int vpad = (int)(c.ldg / (T::SPLIT ? 4 : 2));
-  constexpr int WI = T::TI * 32;
+  constexpr int WI = T::TI * 16;
   static_assert(kStatCols % WI == 0, "a wave's classes lie in one pair");
   const bool ragged = (ti + 1) * T::BI > c.classes;
 #pragma unroll
   for (int b = 0; b < T::TJ; ++b) {
-    const int jl = (wj * T::TJ + b) * 32 + (lane & 31), j = tj * T::BJ + jl;
+    const int jl = (wj * T::TJ + b) * 16 + (lane & 15), j = tj * T::BJ + jl;
     const float rs = T::SPLIT ? rsw / scale_for(j < live ? c.xmax[row0 + j] : 0.f) : rsw;
-    const int iw = ti * T::BI + wi * WI + (lane >> 5) * 4;
+    const int iw = ti * T::BI + wi * WI + (lane >> 4) * 4;
     // z log2 e: exponentials and sums are taken to base 2, one instruction each
     if (c.bias) {
 #pragma unroll
       for (int a = 0; a < T::TI; ++a)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int i = min(iw + a * 32 + (e / 4) * 8 + (e & 3), c.classes - 1);
+        for (int e = 0; e < 4; ++e) {
+          const int i = min(iw + a * 16 + e, c.classes - 1);
           acc[a][b][e] = fmaf(acc[a][b][e], rs, kLog2e * (c.bias_f32 ? ((const float *)c.bias)[i] : (float)((const bf16 *)c.bias)[i]));
         }
     } else {
 #pragma unroll
       for (int a = 0; a < T::TI; ++a)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[a][b][e] *= rs;
+        for (int e = 0; e < 4; ++e) acc[a][b][e] *= rs;
     }
     if (ragged) {
 #pragma unroll
       for (int a = 0; a < T::TI; ++a)
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (iw + a * 32 + (e / 4) * 8 + (e & 3) >= c.classes) acc[a][b][e] = -INFINITY;
+        for (int e = 0; e < 4; ++e)
+          if (iw + a * 16 + e >= c.classes) acc[a][b][e] = -INFINITY;
     }
     float m = -INFINITY;
 #pragma unroll
     for (int a = 0; a < T::TI; ++a)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) m = fmaxf(m, acc[a][b][e]);
+      for (int e = 0; e < 4; ++e) m = fmaxf(m, acc[a][b][e]);
+    m = fmaxf(m, __shfl_xor(m, 16));
     m = fmaxf(m, __shfl_xor(m, 32));
     const float ms = m == -INFINITY ? 0.f : m;
     float s = 0.f;
 #pragma unroll
     for (int a = 0; a < T::TI; ++a)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
+      for (int e = 0; e < 4; ++e) {
         const float p = __builtin_amdgcn_exp2f(acc[a][b][e] - ms);
         s += p;
         acc[a][b][e] = p;
       }
+    s += __shfl_xor(s, 16);
     s += __shfl_xor(s, 32);
-    if (lane < 32 && j < live) c.stats[(long long)j * c.pieces + (ti * T::BI + wi * WI) / WI] = make_float2(m, s);
+    if (lane < 16 && j < live) c.stats[(long long)j * c.pieces + (ti * T::BI + wi * WI) / WI] = make_float2(m, s);
     if constexpr (TRAIN && T::SPLIT) {
       if (j < live) {
         char *row = c.g + j * c.ldg;
 #pragma unroll
         for (int a = 0; a < T::TI; ++a)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int i = iw + a * 32 + q * 8;
-            if (i < vpad)
-              *reinterpret_cast<float4 *>(row + i * 4) = make_float4(acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]);
-          }
+          if (iw + a * 16 < vpad) *reinterpret_cast<f32x4 *>(row + (iw + a * 16) * 4) = acc[a][b];
       }
     } else if constexpr (TRAIN) {
       // through LDS, so that a row leaves in whole 16-byte pieces side by side; piece u of row jl sits at u ^ jl (a lane is a row)
 #pragma unroll
-      for (int a = 0; a < T::TI; ++a)
+      for (int a = 0; a < T::TI; ++a) {
+        const int u = ((wi * WI + a * 16) >> 3) + (lane >> 5);
+        _Float16 t[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int u = (wi * WI + a * 32 + q * 8) >> 3;
-          _Float16 t[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) t[e] = (_Float16)acc[a][b][4 * q + e];
-          *reinterpret_cast<uint2 *>(lds + jl * (T::BI * 2) + ((u ^ (jl & (T::BI / 8 - 1))) << 4) + (lane >> 5) * 8) = *reinterpret_cast<uint2 *>(t);
-        }
+        for (int e = 0; e < 4; ++e) t[e] = (_Float16)acc[a][b][e];
+        *reinterpret_cast<uint2 *>(lds + jl * (T::BI * 2) + ((u ^ (jl & (T::BI / 8 - 1))) << 4) + ((lane >> 4) & 1) * 8) = *reinterpret_cast<uint2 *>(t);
+      }
     }
   }
   if constexpr (TRAIN && !T::SPLIT) {
@@ -385,23 +380,21 @@ __global__ __launch_bounds__(T::THREADS, 2) void ce_dx_kernel(Ce c, int row0) {
   const int ti = blockIdx.x / c.z % nti, tj = blockIdx.x / c.z / nti;
   const int total = (c.classes + T::KK - 1) / T::KK;
   const int s0 = (int)((long long)total * zi / c.z), s1 = (int)((long long)total * (zi + 1) / c.z);
-  f32x16 acc[T::TI][T::TJ];
+  f32x4 acc[T::TI][T::TJ];
   run<T>(lds, side_ks<T>(c.wp, c.ldw, c.classes, c.ldx, ti * T::BI * (T::SPLIT ? 4 : 2), s0), side_kc<T>(c.g, c.ldg, live, c.ldg, tj * T::BJ, s0),
          s1 - s0, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave % T::NWI, wj = wave / T::NWI;
   const int hp = (c.hidden + 3) / 4 * 4;
 #pragma unroll
   for (int b = 0; b < T::TJ; ++b) {
-    const int j = tj * T::BJ + (wj * T::TJ + b) * 32 + (lane & 31);
+    const int j = tj * T::BJ + (wj * T::TJ + b) * 16 + (lane & 15);
     if (j >= live) continue;
     float *row = c.part + ((long long)zi * c.cap + j) * hp;
 #pragma unroll
-    for (int a = 0; a < T::TI; ++a)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int i = ti * T::BI + (wi * T::TI + a) * 32 + q * 8 + (lane >> 5) * 4;
-        if (i < hp) *reinterpret_cast<float4 *>(row + i) = make_float4(acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]);
-      }
+    for (int a = 0; a < T::TI; ++a) {
+      const int i = ti * T::BI + (wi * T::TI + a) * 16 + (lane >> 4) * 4;
+      if (i < hp) *reinterpret_cast<f32x4 *>(row + i) = acc[a][b];
+    }
   }
 }
 
@@ -449,7 +442,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void ce_dw_kernel(Ce c, int row0, in
   int ti, tj;
   tile_of(blockIdx.x, nti * ntj, nti, ntj, ti, tj);
   constexpr int E = T::SPLIT ? 4 : 2;
-  f32x16 acc[T::TI][T::TJ];
+  f32x4 acc[T::TI][T::TJ];
   const char *x = (T::SPLIT ? c.xwp : c.xp) + row0 * c.ldx;
   run<T>(lds, side_ks<T>(x, c.ldx, live, c.ldx, ti * T::BI * E, 0), side_ks<T>(c.g, c.ldg, live, c.ldg, (long long)tj * T::BJ * E, 0),
          (live + T::KK - 1) / T::KK, acc);
@@ -457,40 +450,38 @@ __global__ __launch_bounds__(T::THREADS, 2) void ce_dw_kernel(Ce c, int row0, in
   const float f = T::SPLIT ? 1.f / (kSG * ((const float *)c.head)[1] * scale_of(c, 3)) : 1.f;
 #pragma unroll
   for (int b = 0; b < T::TJ; ++b) {
-    const int j = tj * T::BJ + (wj * T::TJ + b) * 32 + (lane & 31);
+    const int j = tj * T::BJ + (wj * T::TJ + b) * 16 + (lane & 15);
     if (j >= c.classes) continue;
 #pragma unroll
-    for (int a = 0; a < T::TI; ++a)
+    for (int a = 0; a < T::TI; ++a) {
+      const int i = ti * T::BI + (wi * T::TI + a) * 16 + (lane >> 4) * 4;
+      float v[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int i = ti * T::BI + (wi * T::TI + a) * 32 + q * 8 + (lane >> 5) * 4;
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = T::SPLIT ? acc[a][b][4 * q + e] * f : acc[a][b][4 * q + e];
-        const long long at = (long long)j * c.hidden + i;
-        const bool whole = i + 4 <= c.hidden;
-        if (T::SPLIT || mode) {
-          float *d = (T::SPLIT ? (float *)c.dw : c.dwacc) + at;
-          if (whole) {
-            vf4 t = {v[0], v[1], v[2], v[3]};
-            if (mode == 2) t += *reinterpret_cast<const vf4 *>(d);
-            *reinterpret_cast<vf4 *>(d) = t;
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (i + e < c.hidden) d[e] = mode == 2 ? d[e] + v[e] : v[e];
-          }
+      for (int e = 0; e < 4; ++e) v[e] = T::SPLIT ? acc[a][b][e] * f : acc[a][b][e];
+      const long long at = (long long)j * c.hidden + i;
+      const bool whole = i + 4 <= c.hidden;
+      if (T::SPLIT || mode) {
+        float *d = (T::SPLIT ? (float *)c.dw : c.dwacc) + at;
+        if (whole) {
+          vf4 t = {v[0], v[1], v[2], v[3]};
+          if (mode == 2) t += *reinterpret_cast<const vf4 *>(d);
+          *reinterpret_cast<vf4 *>(d) = t;
         } else {
-          bf16 *d = (bf16 *)c.dw + at;
-          if (whole) {
-            *reinterpret_cast<vb4 *>(d) = vb4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
-          } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (i + e < c.hidden) d[e] = (bf16)v[e];
-          }
+          for (int e = 0; e < 4; ++e)
+            if (i + e < c.hidden) d[e] = mode == 2 ? d[e] + v[e] : v[e];
+        }
+      } else {
+        bf16 *d = (bf16 *)c.dw + at;
+        if (whole) {
+          *reinterpret_cast<vb4 *>(d) = vb4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (i + e < c.hidden) d[e] = (bf16)v[e];
         }
       }
+    }
   }
 }
 

@@ -214,61 +214,52 @@ struct Op {
   int last;
 };
 
-// 32 x 32 block (bi, bj) of tile (ti, tj), one accumulator of a wave
+// 16 x 16 block (bi, bj) of tile (ti, tj), one accumulator of a wave
 template <int KIND, int BT>
-__device__ __forceinline__ void finish_block(char *ws, const Mat *__restrict__ mat, const Op &op, int ti, int tj, int bi, int bj, const f32x16 &acc) {
+__device__ __forceinline__ void finish_block(char *ws, const Mat *__restrict__ mat, const Op &op, int ti, int tj, int bi, int bj, const f32x4 &acc) {
   const int lane = threadIdx.x & 63, m = mat->m;
-  const int j = tj * BT + bj * 32 + (lane & 31);
+  const int j = tj * BT + bj * 16 + (lane & 15), i = ti * BT + bi * 16 + (lane >> 4) * 4;
+  float v[4];
   if constexpr (KIND < 2) {
     const int mp = (m + 31) / 32 * 32, lda = mat->lda;
     char *dst = ws + mat->buf[KIND == 0 ? kA : kP];
+    if constexpr (KIND == 0) {
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int i = ti * BT + bi * 32 + g * 8 + (lane >> 5) * 4;
-      float v[4];
-      if constexpr (KIND == 0) {
+      for (int e = 0; e < 4; ++e) v[e] = op.alpha * acc[e];
+    } else {
+      float f[4] = {0.f, 0.f, 0.f, 0.f};
+      if (j < m && i < mp) load_planes(ws + mat->buf[kA] + (long long)j * lda, i, f);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = op.alpha * acc[g * 4 + e];
-      } else {
-        float f[4] = {0.f, 0.f, 0.f, 0.f};
-        if (j < m && i < mp) load_planes(ws + mat->buf[kA] + (long long)j * lda, i, f);
+      for (int e = 0; e < 4; ++e) v[e] = op.alpha * acc[e] + op.beta * f[e] + (i + e == j ? op.gamma : 0.f);
+    }
+    if (j < m && i < mp) store_planes(dst + (long long)j * lda, i, v);
+    if (ti != tj && j < mp) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = op.alpha * acc[g * 4 + e] + op.beta * f[e] + (i + e == j ? op.gamma : 0.f);
-      }
-      if (j < m && i < mp) store_planes(dst + (long long)j * lda, i, v);
-      if (ti != tj && j < mp) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (i + e < m) {
-            _Float16 h, l;
-            split16(v[e], h, l);
-            _Float16 *d = reinterpret_cast<_Float16 *>(dst + (long long)(i + e) * lda + (j >> 5) * 128) + (j & 31);
-            d[0] = h;
-            d[32] = l;
-          }
-      }
+      for (int e = 0; e < 4; ++e)
+        if (i + e < m) {
+          _Float16 h, l;
+          split16(v[e], h, l);
+          _Float16 *d = reinterpret_cast<_Float16 *>(dst + (long long)(i + e) * lda + (j >> 5) * 128) + (j & 31);
+          d[0] = h;
+          d[32] = l;
+        }
     }
   } else {
     if (j >= m) return;
     const int n = mat->n, np = (n + 31) / 32 * 32;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int i = ti * BT + bi * 32 + g * 8 + (lane >> 5) * 4;
-      float v[4];
+    for (int e = 0; e < 4; ++e) v[e] = acc[e] * op.alpha;
+    if (!op.last) {
+      if (i < np) store_planes(ws + mat->buf[op.x == kX0 ? kX1 : kX0] + (long long)j * mat->ldx, i, v);
+    } else {
+      const long long oj = mat->out_j, oi = mat->out_i;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = acc[g * 4 + e] * op.alpha;
-      if (!op.last) {
-        if (i < np) store_planes(ws + mat->buf[op.x == kX0 ? kX1 : kX0] + (long long)j * mat->ldx, i, v);
-      } else {
-        const long long oj = mat->out_j, oi = mat->out_i;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (i + e < n) {
-            const long long k = j * oj + (i + e) * oi;
-            if (mat->bf16) at<__bf16>(ws, mat->out)[k] = (__bf16)v[e];
-            else at<float>(ws, mat->out)[k] = v[e];
-          }
-      }
+      for (int e = 0; e < 4; ++e)
+        if (i + e < n) {
+          const long long k = j * oj + (i + e) * oi;
+          if (mat->bf16) at<__bf16>(ws, mat->out)[k] = (__bf16)v[e];
+          else at<float>(ws, mat->out)[k] = v[e];
+        }
     }
   }
 }
@@ -307,7 +298,7 @@ __global__ __launch_bounds__(kThreads, 2) void ortho_product_kernel(char *ws, co
   const int s0 = (int)((long long)total * zi / z), s1 = (int)((long long)total * (zi + 1) / z);
   const int ldl = KIND == 1 ? mat->lda : mat->ldx, ldr = KIND == 0 ? mat->ldx : mat->lda;
   const char *l = ws + mat->buf[KIND == 1 ? kA : op.x], *r = ws + mat->buf[KIND == 0 ? op.x : KIND == 1 ? kA : kP];
-  f32x16 acc[T::TI][T::TJ];
+  f32x4 acc[T::TI][T::TJ];
   if constexpr (KIND == 2) run<T>(lds, side_ks<T>(l, ldl, m, ldl, (long long)ti * BT * 4, s0), side_kc<T>(r, ldr, m, ldr, tj * BT, s0), s1 - s0, acc);
   else run<T>(lds, side_kc<T>(l, ldl, m, ldl, ti * BT, s0), side_kc<T>(r, ldr, m, ldr, tj * BT, s0), s1 - s0, acc);
   const int wave = threadIdx.x >> 6, wi = wave % T::NWI, wj = wave / T::NWI;
@@ -317,49 +308,49 @@ __global__ __launch_bounds__(kThreads, 2) void ortho_product_kernel(char *ws, co
 #pragma unroll
       for (int y = 0; y < T::TJ; ++y) finish_block<KIND, BT>(ws, mat, op, ti, tj, wi * T::TI + x, wj * T::TJ + y, acc[x][y]);
   } else {
-    float *d = at<float>(ws, mat->part) + ((long long)(t - sp.whole) * z + zi) * (BT * BT) + threadIdx.x;
+    f32x4 *d = at<f32x4>(ws, mat->part) + ((long long)(t - sp.whole) * z + zi) * (BT * BT / 4) + threadIdx.x;
 #pragma unroll
     for (int x = 0; x < T::TI; ++x)
 #pragma unroll
-      for (int y = 0; y < T::TJ; ++y)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) d[((x * T::TJ + y) * 16 + e) * kThreads] = acc[x][y][e];
+      for (int y = 0; y < T::TJ; ++y) d[(x * T::TJ + y) * kThreads] = acc[x][y];
   }
 }
 
-// the parts of split tiles, added in a fixed order; a workgroup takes one 32 x 32 block of every wave
+// the parts of split tiles, added in a fixed order; a workgroup takes four 16 x 16 blocks of every wave
 template <int KIND, int BT>
 __global__ __launch_bounds__(kThreads) void ortho_join_kernel(char *ws, const Mat *__restrict__ mats, const int *__restrict__ map, Op op) {
   typedef typename Pick<BT, KIND == 2, false>::T T;
-  constexpr int kFirst = KIND == 0 ? kGramJoin : KIND == 1 ? kSquareJoin : kApplyJoin, Q = T::TI * T::TJ;
+  constexpr int kFirst = KIND == 0 ? kGramJoin : KIND == 1 ? kSquareJoin : kApplyJoin, Q = T::TI * T::TJ / 4;
   const int b = blockIdx.x;
   const Mat *__restrict__ mat = mats + map[b];
   const Split sp = split_of<KIND>(mat);
   const int local = b - mat->first[kFirst], u = local / Q, q = local % Q;
   int ti, tj;
   tile_at<KIND, BT>(mat, sp.whole + u, ti, tj);
-  const float *s = at<float>(ws, mat->part) + (long long)u * sp.z * (BT * BT) + q * 16 * kThreads + threadIdx.x;
-  f32x16 acc;
+  const f32x4 *s = at<const f32x4>(ws, mat->part) + (long long)u * sp.z * (BT * BT / 4) + q * 4 * kThreads + threadIdx.x;
+  f32x4 acc[4];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) acc[e] = s[e * kThreads];
-  for (int zi = 1; zi < sp.z; zi += 2) {                    // 32 loads in flight
-    const float *s1 = s + (long long)zi * (BT * BT);
+  for (int k = 0; k < 4; ++k) acc[k] = s[k * kThreads];
+  for (int zi = 1; zi < sp.z; zi += 2) {                    // 8 loads of 16 bytes in flight
+    const f32x4 *s1 = s + (long long)zi * (BT * BT / 4);
     const bool two = zi + 1 < sp.z;
-    const float *s2 = two ? s1 + BT * BT : s1;
-    float x[16], y[16];
+    const f32x4 *s2 = two ? s1 + BT * BT / 4 : s1;
+    f32x4 x[4], y[4];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      x[e] = s1[e * kThreads];
-      y[e] = s2[e * kThreads];
+    for (int k = 0; k < 4; ++k) {
+      x[k] = s1[k * kThreads];
+      y[k] = s2[k * kThreads];
     }
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      acc[e] += x[e];
-      if (two) acc[e] += y[e];
+    for (int k = 0; k < 4; ++k) {
+      acc[k] += x[k];
+      if (two) acc[k] += y[k];
     }
   }
   const int wave = threadIdx.x >> 6, wi = wave % T::NWI, wj = wave / T::NWI;
-  finish_block<KIND, BT>(ws, mat, op, ti, tj, wi * T::TI + q / T::TJ, wj * T::TJ + q % T::TJ, acc);
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    finish_block<KIND, BT>(ws, mat, op, ti, tj, wi * T::TI + (q * 4 + k) / T::TJ, wj * T::TJ + (q * 4 + k) % T::TJ, acc[k]);
 }
 
 // ------------------------------------------------------------------------------------------------ small path
