@@ -613,13 +613,16 @@ int layout_of(const mr3d_linear_ce *a, Layout &l) {
   size_t at = 0;
   l.ldx = up(a->hidden, f32 ? 32 : 64) * (f32 ? 4 : 2);
   l.ldg = up(a->classes, f32 ? 32 : 64) * (f32 ? 4 : 2);
-  // bf16 weights are read where they are when a row is whole 128-byte k-steps on 16-byte boundaries
-  l.pack_w = f32 || a->hidden % 64 || a->weight_stride % 8 || ((uintptr_t)a->weight & 15);
+  // bf16 weights are read where they are when a row is whole 128-byte k-steps on 16-byte boundaries, and 256 rows lie within the 32-bit
+  // offsets of a tile's loads
+  l.pack_w = f32 || a->hidden % 64 || a->weight_stride % 8 || a->weight_stride > 1 << 21 || ((uintptr_t)a->weight & 15);
   l.ldw = l.pack_w ? l.ldx : a->weight_stride * 2;
   l.chunks = 1;
+  // bytes a row of a piece needs: its exponentials, or only its (max, sum) pairs (one for 32 classes at most)
+  const long long row_bytes = train ? l.ldg : up(a->classes, 64) / 32 * 8;
   long long cap = a->rows;
-  if (train && cap * l.ldg > kPiece) {
-    cap = kPiece / l.ldg / 256 * 256;
+  if (cap * row_bytes > kPiece) {
+    cap = kPiece / row_bytes / 256 * 256;
     if (cap < 256) cap = 256;
     l.chunks = (int)((a->rows + cap - 1) / cap);
   }

@@ -1,15 +1,17 @@
 """linear_cross_entropy (csrc/linear_ce.hip) against the formulas in 64 bits.
 
 Tolerances, norm-wise per row or matrix.  u = 2^-24.
-  logits   fp32: each factor carries 22 bits (error 2^-23 of the value at most), lo * lo (2^-22 of a term) is dropped, and the K products are
-           summed in fp32 with at most K / 16 + 16 roundings (16 products an instruction): |dz| <= (2^-21 + (K / 16 + 16) u) |x| |W_c|.
-           bf16: factors are exact, |dz| <= (K / 16 + 16) u |x| |W_c|.  Adding the bias and subtracting the maximum: 2 u |z| more.  Call the row's
+  products One matrix instruction adds 32 products; each of them and the accumulator is cut 2 bits below the last place of the largest (2^-25 of
+           it), and the sum is rounded: 32 * 2^-25 + 2^-24 = 17 u of |x| |W_c|.  bf16: K / 32 of them, 17 K / 32 u.  fp32: factors carry 22 bits (error
+           2^-23 of the value at most), lo * lo (2^-22 of a term) is dropped; three passes over 128 k (204 u of that part's |x| |W_c|, whose
+           sum over the parts is at most |x| |W_c| by Cauchy-Schwarz) are added in fp32, K / 128 u: together 2^-21 + (204 + K / 128) u.
+  logits   |dz| <= that times |x| |W_c|, bf16 factors being exact.  Adding the bias and subtracting the maximum: 2 u |z| more.  Call the row's
            largest Z.  Exponential and sums: 2^-20 relative in all (the hardware exponential is good to a few u; sums are short).
   loss     |d ce_i| <= 2 Z + 2^-20, and the weighted mean over rows; stored in fp32.
   g        relative to softmax: E = 2 Z + 2^-19; the label's entry is computed apart, absolute error E.  fp32: two planes of 14 + 22 bits
            (2^-21 of the value and 2^-38 absolute); bf16: 2^-8 for the stored exponential and 2^-8 for g.
            So |dg_i| <= (E + r) |g_i| + E p_label w with r = 2^-20 (fp32), 2^-7 (bf16), taken entry by entry below.
-  dx, dW   the error of g through |W| and |x|, entry by entry, plus (2^-20 + (n / 16 + 20) u) sum |g| |W| for the product (n its length), plus
+  dx, dW   the error of g through |W| and |x|, entry by entry, plus the product's own error (n its length) on sum |g| |W|, plus
            half a step of the stored type."""
 import pytest
 import torch
@@ -39,12 +41,12 @@ def _reference(x, w, b, label, rw, ignore=-100, valid=None, avg=None):
     g = p.clone()
     g[at, ll] -= 1
     s = (rl / avg)[:, None]
-    zerr = ((2.0 ** -21 if f32 else 0) + (k / 16 + 16) * U) * xl.norm(dim=1, keepdim=True) * w.norm(dim=1).max() + 2 * U * z.abs().amax(1, keepdim=True)
+    prod = lambda m: 2.0 ** -21 + (204 + m / 128) * U if f32 else (17 * (m // 32 + 1)) * U
+    zerr = prod(k) * xl.norm(dim=1, keepdim=True) * w.norm(dim=1).max() + 2 * U * z.abs().amax(1, keepdim=True)
     e = 2 * zerr + 2.0 ** -19
     eg = (e + (2.0 ** -20 if f32 else 2.0 ** -7)) * g.abs() + (2.0 ** -36 if f32 else 0)
     eg[at, ll] += e.squeeze(1) * torch.ones(len(rows))
     g, eg = g * s, eg * s.abs()
-    prod = lambda m: (2.0 ** -20 if f32 else 0) + (m / 16 + 20) * U
     dx, ex = torch.zeros_like(x), torch.zeros_like(x)
     dx[rows] = g @ w
     ex[rows] = eg @ w.abs() + prod(v) * (g.abs() @ w.abs())
@@ -292,6 +294,54 @@ def test_same_bits_every_run_on_another_stream_and_in_a_graph():
             graph.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(p, q) for p, q in zip(held, both())), k
+
+
+@pytest.mark.gpu
+def test_large_tiles_in_a_replayed_graph():
+    from mr3d_amd.core import linear_cross_entropy
+    x, w, _, label, rw = (None if t is None else t.cuda() for t in _inputs(3500, 64, 3600, torch.bfloat16, bias=False))
+
+    def both():
+        leaves = [t.detach().requires_grad_(True) for t in (x, w)]
+        loss = linear_cross_entropy(leaves[0], leaves[1], label, rw)
+        return (loss.detach(),) + torch.autograd.grad(loss, leaves)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = both()
+    for k in range(3):
+        x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(k)).to(x.dtype))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(held, both())), k
+
+
+@pytest.mark.gpu
+def test_weight_rows_far_apart():
+    """rows of the weight 6 MB apart (a slice of a wide buffer): 256 of them pass 32 bits of byte offsets"""
+    x, w, _, label, rw = _inputs(70, 64, 300, torch.bfloat16, bias=False)
+    wide = torch.zeros(300, 3 << 20, dtype=torch.bfloat16, device='cuda')
+    wide[:, 64:128] = w.cuda()
+    from mr3d_amd.core import linear_cross_entropy
+    ref, bound = _reference(x, w, None, label, rw)
+    leaves = [x.cuda().requires_grad_(True), wide[:, 64:128].detach().requires_grad_(True)]
+    loss = linear_cross_entropy(leaves[0], leaves[1], label.cuda(), rw.cuda())
+    for name, t in zip(('loss', 'dx', 'dw'), (loss,) + torch.autograd.grad(loss, leaves)):
+        _check(t, ref[name], bound[name], (name,))
+
+
+@pytest.mark.gpu
+def test_forward_alone_in_pieces():
+    """20000 rows against 2^20 classes need 5 GB of (max, sum) pairs: three pieces of rows, compared with the halves called alone"""
+    from mr3d_amd.core import linear_cross_entropy
+    g = torch.Generator(device='cuda').manual_seed(0)
+    x = torch.randn(20000, 8, generator=g, device='cuda').bfloat16()
+    w = torch.randn(1 << 20, 8, generator=g, device='cuda').bfloat16()
+    label = torch.randint(0, 1 << 20, (20000,), generator=g, device='cuda')
+    with torch.no_grad():
+        whole = float(linear_cross_entropy(x, w, label))
+        halves = [float(linear_cross_entropy(x[s], w, label[s], avg_factor=20000.0)) for s in (slice(0, 10000), slice(10000, None))]
+    assert abs(whole - sum(halves)) <= 4 * U * whole
 
 
 @pytest.mark.gpu
