@@ -5,6 +5,7 @@
 
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include <algorithm>
 #include <vector>
 
 namespace {
@@ -265,6 +266,28 @@ std::vector<at::Tensor> orthogonalize(const std::vector<at::Tensor> &mats, int64
       TORCH_CHECK_VALUE(outs[i].sizes() == mats[i].sizes() && outs[i].scalar_type() == mats[i].scalar_type() && outs[i].device() == mats[i].device() &&
                             outs[i].is_contiguous(),
                         "orthogonalize: an out is contiguous and has its matrix's shape, type and device");
+    // No out may lie on another matrix or out: some are written while others are still read.  A matrix that is its own out counts once.
+    struct Span {
+      const char *from, *to;
+      bool written;
+    };
+    std::vector<Span> spans;
+    for (size_t i = 0; i < mats.size(); ++i) {
+      const at::Tensor &m = flat[i];
+      if (!m.numel()) continue;
+      const char *o = (const char *)outs[i].data_ptr(), *in = (const char *)m.data_ptr();
+      spans.push_back({o, o + outs[i].nbytes(), true});
+      if (in == o && m.is_contiguous()) continue;
+      spans.push_back({in, in + ((m.size(0) - 1) * m.stride(0) + (m.size(1) - 1) * m.stride(1) + 1) * m.element_size(), false});
+    }
+    std::sort(spans.begin(), spans.end(), [](const Span &p, const Span &q) { return p.from < q.from; });
+    const char *read = nullptr, *written = nullptr;
+    for (const Span &s : spans) {
+      TORCH_CHECK_VALUE(s.from >= written && (!s.written || s.from >= read),
+                        "orthogonalize: an out overlaps another out or a matrix that is not its own, contiguous one");
+      const char *&end = s.written ? written : read;
+      end = std::max(end, s.to);
+    }
   } else {
     // one buffer per type; every result starts on its own 256 bytes
     outs.resize(mats.size());
@@ -302,6 +325,9 @@ std::vector<at::Tensor> orthogonalize(const std::vector<at::Tensor> &mats, int64
   mr3d_check_status(mr3d_orthogonalize(table.data(), (int)table.size(), (int)steps, (float)a, (float)b, (float)c, (float)eps, p, need,
                                        mr3d_current_stream(mats[0])),
                     "mr3d_orthogonalize");
+  if (out)
+    for (const at::Tensor &t : outs)
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();  // a graph that saved it says so
   return outs;
 }
 

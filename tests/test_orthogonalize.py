@@ -1,10 +1,11 @@
 """orthogonalize (csrc/ortho.hip) against the same iteration in 64 bits.
 
-Tolerance.  The factors carry 22 bits: rounding each of them is at most 2^-23 of the value, and a product drops lo * lo, at most 2^-22 of
-a term; fp32 accumulation adds at most 2^-24 per term.  One step therefore perturbs X by at most about d = 2^-20 |X|_F in norm (three products
-of factors with spectral norms below 1.3, 4.8 and 1.3, errors taken at their worst in the norm over all entries: 2^-22 * (1 + b + c + 1)).  The map's
-slope is largest at 0 (a = 3.4445), so an error of step k is amplified by a^(steps-1-k) at most while |X|_F itself grows towards sqrt(m):
-|error| <= d sum_k a^(steps-1-k) |X_k|_F, with the norms of the iterates taken from the reference.  Random errors stay far below that.
+Tolerance.  Up to 64 rows the iteration is in double.  Above: the factors carry 22 bits (rounding 2^-23 of the value at most, lo * lo of at most 2^-22 of a
+term is dropped), and a matrix instruction cuts each of its 32 products 2 bits below the last place of the largest.  Taken as independent, these
+errors perturb a product by 2^-23 of the product of its factors' norms or less, and one step -- three products of factors with spectral norms
+below 1.3, weighted 1, b = 4.8, c = 2 and 1 -- perturbs X by at most about d = 2^-20 |X|_F.  The map's slope is largest at 0 (a = 3.4445), so an
+error of step k is amplified by a^(steps-1-k) at most while |X|_F itself grows towards sqrt(m):
+|error| <= d sum_k a^(steps-1-k) |X_k|_F, with the norms of the iterates taken from the reference.
 Results in bf16 add half a step, 2^-8 of each value."""
 import pytest
 import torch
@@ -99,12 +100,14 @@ def test_scales_of_the_input():
 @pytest.mark.gpu
 def test_nan_and_infinity_stay_in_their_matrix():
     from mr3d_amd.core import orthogonalize
-    mats = [_gauss(40, 60), _gauss(64, 64), _gauss(130, 50), _gauss(40, 60, 5)]
-    mats[1][3, 5], mats[2][0, 0] = float('nan'), float('inf')
+    mats = [_gauss(40, 60), _gauss(64, 64), _gauss(130, 50), _gauss(40, 60, 5), _gauss(200, 300), _gauss(300, 100), _gauss(150, 150), _gauss(200, 300, 6)]
+    for i, v in ((1, 'nan'), (2, 'inf'), (5, 'inf'), (6, 'nan')):
+        mats[i][3, 5] = float(v)
     out = orthogonalize(mats)
-    _check(out[0], mats[0])
-    _check(out[3], mats[3])
-    assert torch.isnan(out[1]).all() and not torch.isfinite(out[2]).any()
+    for i in (0, 3, 4, 7):
+        _check(out[i], mats[i])
+    for i in (1, 2, 5, 6):
+        assert torch.isnan(out[i]).all(), i
 
 
 @pytest.mark.gpu
@@ -120,6 +123,24 @@ def test_strided_inputs_and_given_outputs():
     h = g.clone()
     orthogonalize(h, out=h)
     assert torch.equal(h, ref)
+    big = _gauss(200, 300)
+    ref = orthogonalize(big)
+    orthogonalize(big, out=big)
+    assert torch.equal(big, ref)
+    with pytest.raises(ValueError, match='overlaps'):
+        orthogonalize([g, g], out=[o[:70], o[:70]])
+    with pytest.raises(ValueError, match='overlaps'):
+        orthogonalize([h, g], out=[o[:70], h])
+    saved = _gauss(70, 140).requires_grad_(True)
+    kept = (saved * o[:70]).sum()
+    orthogonalize(g, out=o[:70])
+    with pytest.raises(RuntimeError, match='inplace'):
+        kept.backward()
+    sq = _gauss(64, 64)
+    with pytest.raises(ValueError, match='overlaps'):
+        orthogonalize(sq.t(), out=sq)
+    with pytest.raises(ValueError, match='contiguous'):
+        orthogonalize(g, out=torch.empty(140, 70, device='cuda').t())
 
 
 @pytest.mark.gpu
