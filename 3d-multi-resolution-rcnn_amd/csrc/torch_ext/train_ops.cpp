@@ -135,7 +135,14 @@ struct CeArgs {
   int64_t ignore_index;
 };
 
-// The forward call leaves the gradients too; backward multiplies them by the incoming one, in place and once
+bool capturing(const at::Tensor &t) {
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  TORCH_CHECK(hipStreamIsCapturing((hipStream_t)mr3d_current_stream(t), &st) == hipSuccess, "hipStreamIsCapturing failed");
+  return st != hipStreamCaptureStatusNone;
+}
+
+// The forward call leaves the gradients too; backward multiplies them by the incoming one, in place and once: a graph that holds only one of the two
+// would multiply again at every replay, or hand out memory that the next replay overwrites, so they are captured together or not at all
 struct LinearCe : torch::autograd::Function<LinearCe> {
   static at::Tensor compute(const at::Tensor &x, const at::Tensor &w, const at::Tensor &bias, const CeArgs &c, int want, at::Tensor (&grads)[3]) {
     const int64_t k = w.size(1), classes = w.size(0);
@@ -172,6 +179,7 @@ struct LinearCe : torch::autograd::Function<LinearCe> {
   static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &w, const std::optional<at::Tensor> &bias, const CeArgs &c) {
     const at::Tensor b = or_none(bias);
     at::Tensor grads[3];
+    ctx->saved_data["captured"] = capturing(x);
     at::Tensor loss = compute(x, w, b, c, wants(x) | wants(w) << 1 | wants(b) << 2, grads);
     for (int i = 0; i < 3; ++i)
       if (grads[i].defined()) ctx->saved_data["g" + std::to_string(i)] = i == 0 && x.dim() != 2 ? grads[i].view(x.sizes()) : grads[i];
@@ -181,6 +189,8 @@ struct LinearCe : torch::autograd::Function<LinearCe> {
   static variable_list backward(AutogradContext *ctx, variable_list g) {
     TORCH_CHECK(!ctx->saved_data.count("used"), "linear_cross_entropy: a second backward through the same loss (its gradients were handed over by the "
                                                 "first); call linear_cross_entropy again");
+    TORCH_CHECK(ctx->saved_data["captured"].toBool() == capturing(g[0]),
+                "linear_cross_entropy: the call and its backward are captured into graphs together or not at all");
     ctx->saved_data["used"] = true;
     variable_list out(4);
     {

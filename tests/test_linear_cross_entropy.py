@@ -317,6 +317,68 @@ def test_large_tiles_in_a_replayed_graph():
 
 
 @pytest.mark.gpu
+def test_backward_belongs_to_the_graph_of_its_call():
+    from mr3d_amd.core import linear_cross_entropy
+    x, w, b, label, rw = (t.cuda() for t in _inputs(40, 32, 50, torch.float32))
+    x.requires_grad_(True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = linear_cross_entropy(x, w, label, rw, b)
+    graph.replay()
+    with pytest.raises(RuntimeError, match='together or not at all'):
+        torch.autograd.grad(loss, x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_graphed_callable(dtype):
+    """forward and backward in two graphs; the incoming gradient is not 1, replays alternate with eager calls"""
+    from mr3d_amd.core import linear_cross_entropy
+    x, w, b, label, rw = (t.cuda() for t in _inputs(100, 48, 300, dtype))
+
+    class Head(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.w, self.b = torch.nn.Parameter(w.clone()), torch.nn.Parameter(b.clone())
+
+        def forward(self, x):
+            return linear_cross_entropy(x, self.w, label, rw, self.b)
+
+    head = Head()
+    graphed = torch.cuda.make_graphed_callables(Head(), (x.clone().requires_grad_(True),))
+    for k in range(4):
+        v = torch.randn(x.shape, generator=torch.Generator().manual_seed(k)).to(dtype).cuda()
+        res = []
+        for m in (graphed, head):
+            leaf = v.clone().requires_grad_(True)
+            res.append([t.clone() for t in torch.autograd.grad(3.0 * m(leaf), [leaf, *m.parameters()])])
+            torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(*res)), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('low', [float('-inf'), torch.finfo(torch.float32).min])
+def test_classes_masked_by_the_bias(dtype, low):
+    """a bias of minus infinity or the lowest value takes classes out: whole tiles of them, single ones, all but one of a tile"""
+    x, w, b, label, rw = _inputs(90, 40, 700, dtype)
+    keep = torch.ones(700, dtype=torch.bool)
+    keep[128:512], keep[5], keep[600:640] = False, False, False
+    keep[620] = True
+    kept = keep.nonzero().squeeze(1)
+    label = kept[torch.arange(90) * 7 % len(kept)]
+    ref, bound = _reference(x, w[kept], b.float()[kept], torch.searchsorted(kept, label), rw)
+    masked = b.float().masked_fill(~keep, low)
+    from mr3d_amd.core import linear_cross_entropy
+    leaves = [x.cuda().requires_grad_(True), w.cuda().requires_grad_(True), masked.cuda().requires_grad_(True)]
+    loss = linear_cross_entropy(leaves[0], leaves[1], label.cuda(), rw.cuda(), leaves[2])
+    dx, dw, db = torch.autograd.grad(loss, leaves)
+    assert not dw[~keep].any() and not db[~keep].any()
+    for name, t in zip(('loss', 'dx', 'dw', 'db'), (loss, dx, dw[keep], db[keep])):
+        _check(t, ref[name], bound[name], (name,))
+
+
+@pytest.mark.gpu
 def test_weight_rows_far_apart():
     """rows of the weight 6 MB apart (a slice of a wide buffer): 256 of them pass 32 bits of byte offsets"""
     x, w, _, label, rw = _inputs(70, 64, 300, torch.bfloat16, bias=False)
