@@ -369,15 +369,13 @@ __global__ __launch_bounds__(256) void ce_grad_kernel(Ce c, int row0, int wcols)
 }
 
 // part z of dx: live rows x hidden, summed over the z-th share of the classes
-template <class T>
-__global__ __launch_bounds__(T::THREADS, 2) void ce_dx_kernel(Ce c, int row0) {
-  extern __shared__ __attribute__((aligned(1024))) char lds[];
+template <class T> __device__ __forceinline__ void dx_tile(const Ce &c, int row0, int bid, char *lds) {
   const int live = min(c.head[0] - row0, c.cap);
   if (live <= 0) return;
   const int nti = (c.hidden + T::BI - 1) / T::BI, ntj = (live + T::BJ - 1) / T::BJ;
-  if ((int)blockIdx.x >= nti * ntj * c.z) return;
-  const int zi = blockIdx.x % c.z;
-  const int ti = blockIdx.x / c.z % nti, tj = blockIdx.x / c.z / nti;
+  if (bid >= nti * ntj * c.z) return;
+  const int zi = bid % c.z;
+  const int ti = bid / c.z % nti, tj = bid / c.z / nti;
   const int total = (c.classes + T::KK - 1) / T::KK;
   const int s0 = (int)((long long)total * zi / c.z), s1 = (int)((long long)total * (zi + 1) / c.z);
   f32x4 acc[T::TI][T::TJ];
@@ -433,14 +431,12 @@ __global__ __launch_bounds__(256) void ce_dx_rows_kernel(Ce c, int row0) {
 }
 
 // dW tile: classes x hidden, summed over the piece's live rows.  mode 0: store in the caller's type, 1: store to / 2: add to an fp32 accumulator
-template <class T>
-__global__ __launch_bounds__(T::THREADS, 2) void ce_dw_kernel(Ce c, int row0, int mode) {
-  extern __shared__ __attribute__((aligned(1024))) char lds[];
+template <class T> __device__ __forceinline__ void dw_tile(const Ce &c, int row0, int mode, int bid, char *lds) {
   const int live = max(min(c.head[0] - row0, c.cap), 0);
   if (live == 0 && row0) return;
   const int nti = (c.hidden + T::BI - 1) / T::BI, ntj = (c.classes + T::BJ - 1) / T::BJ;
   int ti, tj;
-  tile_of(blockIdx.x, nti * ntj, nti, ntj, ti, tj);
+  tile_of(bid, nti * ntj, nti, ntj, ti, tj);
   constexpr int E = T::SPLIT ? 4 : 2;
   f32x4 acc[T::TI][T::TJ];
   const char *x = (T::SPLIT ? c.xwp : c.xp) + row0 * c.ldx;
@@ -492,12 +488,11 @@ __global__ __launch_bounds__(256) void ce_dw_round_kernel(const float *__restric
 // db: column sums of g.  A workgroup adds kDbRows rows of 256 columns: 8 columns (16 bytes, split: of each plane) a thread and 8 rows side
 // by side, which meet in LDS; the parts are added in order afterwards
 constexpr int kDbRows = 64;
-template <bool F32>
-__global__ __launch_bounds__(256) void ce_db_kernel(Ce c, int row0) {
-  __shared__ float sum[8][256];
+template <bool F32> __device__ __forceinline__ void db_part(const Ce &c, int row0, int bx, int slice, char *lds) {
+  float (*sum)[256] = reinterpret_cast<float (*)[256]>(lds);
   const int live = min(c.head[0] - row0, c.cap);
-  const int slice = blockIdx.y, j0 = slice * kDbRows, j1 = min(j0 + kDbRows, live);
-  const int col = (threadIdx.x & 31) * 8, i = blockIdx.x * 256 + col, sub = threadIdx.x >> 5;
+  const int j0 = slice * kDbRows, j1 = min(j0 + kDbRows, live);
+  const int col = (threadIdx.x & 31) * 8, i = bx * 256 + col, sub = threadIdx.x >> 5;
   float s[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) s[e] = 0.f;
@@ -521,13 +516,38 @@ __global__ __launch_bounds__(256) void ce_db_kernel(Ce c, int row0) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) sum[sub][col + e] = s[e];
   __syncthreads();
-  const int o = blockIdx.x * 256 + threadIdx.x;
+  const int o = bx * 256 + threadIdx.x;
   if (o >= c.classes) return;
   float t = 0.f;
 #pragma unroll
   for (int k = 0; k < 8; ++k) t += sum[k][threadIdx.x];
   c.dbpart[(long long)(row0 / kDbRows + slice) * c.classes + o] = F32 ? t / (kSG * ((const float *)c.head)[1]) : t;
 }
+
+// The gradients' launches.  Tiles of 64 and 128 (one workgroup shape) share one launch with db's sums: each of the three alone leaves CUs idle
+template <class TX, class TW, bool F32>
+__global__ __launch_bounds__(256, 2) void ce_gradients_kernel(Ce c, int row0, int mode, int dx_blocks, int dw_blocks, int db_blocks) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  int b = blockIdx.x;
+  if (b < dx_blocks) return dx_tile<TX>(c, row0, b, lds);
+  b -= dx_blocks;
+  if (b < dw_blocks) return dw_tile<TW>(c, row0, mode, b, lds);
+  b -= dw_blocks;
+  db_part<F32>(c, row0, b % db_blocks, b / db_blocks, lds);
+}
+template <class T> __global__ __launch_bounds__(T::THREADS, 2) void ce_dx_kernel(Ce c, int row0) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  dx_tile<T>(c, row0, blockIdx.x, lds);
+}
+template <class T> __global__ __launch_bounds__(T::THREADS, 2) void ce_dw_kernel(Ce c, int row0, int mode) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  dw_tile<T>(c, row0, mode, blockIdx.x, lds);
+}
+template <bool F32> __global__ __launch_bounds__(256) void ce_db_kernel(Ce c, int row0) {
+  __shared__ __attribute__((aligned(16))) char lds[8 * 256 * 4];
+  db_part<F32>(c, row0, blockIdx.x, blockIdx.y, lds);
+}
+
 // The last launch.  Workgroup 0: the loss, row by row in order; the others (want_db): db, 64 columns each, the slices four side by side
 __global__ __launch_bounds__(256) void ce_finish_kernel(Ce c, int slices) {
   __shared__ double sum[4][64];
@@ -671,19 +691,26 @@ template <class T, bool TRAIN> int launch_logits(const Ce &c, int row0, hipStrea
   ce_logits_kernel<T, TRAIN><<<(unsigned)n, T::THREADS, T::LDS_BYTES, q>>>(c, row0);
   return MR3D_OK;
 }
+template <class T> int dx_blocks(const Ce &c) { return (c.hidden + T::BI - 1) / T::BI * ((c.cap + T::BJ - 1) / T::BJ) * c.z; }
+template <class T> int dw_blocks(const Ce &c) { return (c.hidden + T::BI - 1) / T::BI * ((c.classes + T::BJ - 1) / T::BJ); }
 template <class T> int launch_dx(const Ce &c, int row0, hipStream_t q) {
   if (T::LDS_BYTES > 65536)
     if (const int e = allow_lds(ce_dx_kernel<T>, T::LDS_BYTES)) return e;
-  const long long n = (long long)((c.hidden + T::BI - 1) / T::BI) * ((c.cap + T::BJ - 1) / T::BJ) * c.z;
-  ce_dx_kernel<T><<<(unsigned)n, T::THREADS, T::LDS_BYTES, q>>>(c, row0);
+  ce_dx_kernel<T><<<dx_blocks<T>(c), T::THREADS, T::LDS_BYTES, q>>>(c, row0);
   return MR3D_OK;
 }
 template <class T> int launch_dw(const Ce &c, int row0, int mode, hipStream_t q) {
   if (T::LDS_BYTES > 65536)
     if (const int e = allow_lds(ce_dw_kernel<T>, T::LDS_BYTES)) return e;
-  const long long n = (long long)((c.hidden + T::BI - 1) / T::BI) * ((c.classes + T::BJ - 1) / T::BJ);
-  ce_dw_kernel<T><<<(unsigned)n, T::THREADS, T::LDS_BYTES, q>>>(c, row0, mode);
+  ce_dw_kernel<T><<<dw_blocks<T>(c), T::THREADS, T::LDS_BYTES, q>>>(c, row0, mode);
   return MR3D_OK;
+}
+template <class TX, class TW, bool F32> void launch_gradients(const mr3d_linear_ce *a, const Ce &c, int row0, int mode, hipStream_t q) {
+  constexpr int lds = TX::LDS_BYTES > TW::LDS_BYTES ? TX::LDS_BYTES : TW::LDS_BYTES;
+  static_assert(lds <= 65536 && lds >= 8192 && TX::THREADS == 256 && TW::THREADS == 256, "");
+  const int nx = a->want_dx ? dx_blocks<TX>(c) : 0, nw = a->want_dweight ? dw_blocks<TW>(c) : 0, nb = (a->classes + 255) / 256;
+  const int n = nx + nw + (a->want_dbias ? nb * ((c.cap + kDbRows - 1) / kDbRows) : 0);
+  ce_gradients_kernel<TX, TW, F32><<<n, 256, lds, q>>>(c, row0, mode, nx, nw, nb);
 }
 
 template <class TT, class F> int pick(int bt, F f) {
@@ -712,17 +739,21 @@ template <bool F32> int run_ce(const mr3d_linear_ce *a, const Layout &l, Ce &c, 
       ce_grad_kernel<F32, false><<<l.cap, 256, 0, q>>>(c, row0, l.wcols);
     }
     if (e) return e;
-    if (a->want_dx) {
-      e = pick<TX>(l.bt_dx, [&](auto t) { return launch_dx<decltype(t)>(c, row0, q); });
+    const int mode = k ? 2 : (l.chunks > 1 ? 1 : 0);
+    if (!train) continue;
+    if ((!a->want_dx || l.bt_dx < 256) && (!a->want_dweight || l.bt_dw < 256)) {
+      if (l.bt_dx == 128 && l.bt_dw == 128) launch_gradients<typename TX::Small, typename TW::Small, F32>(a, c, row0, mode, q);
+      else if (l.bt_dx == 128) launch_gradients<typename TX::Small, typename TW::Tiny, F32>(a, c, row0, mode, q);
+      else if (l.bt_dw == 128) launch_gradients<typename TX::Tiny, typename TW::Small, F32>(a, c, row0, mode, q);
+      else launch_gradients<typename TX::Tiny, typename TW::Tiny, F32>(a, c, row0, mode, q);
+    } else {
+      if (a->want_dx) e = pick<TX>(l.bt_dx, [&](auto t) { return launch_dx<decltype(t)>(c, row0, q); });
       if (e) return e;
-      ce_dx_rows_kernel<F32><<<a->rows, 256, 0, q>>>(c, row0);
-    }
-    if (a->want_dweight) {
-      const int mode = k ? 2 : (l.chunks > 1 ? 1 : 0);
-      e = pick<TW>(l.bt_dw, [&](auto t) { return launch_dw<decltype(t)>(c, row0, mode, q); });
+      if (a->want_dweight) e = pick<TW>(l.bt_dw, [&](auto t) { return launch_dw<decltype(t)>(c, row0, mode, q); });
       if (e) return e;
+      if (a->want_dbias) ce_db_kernel<F32><<<dim3((a->classes + 255) / 256, (l.cap + kDbRows - 1) / kDbRows), 256, 0, q>>>(c, row0);
     }
-    if (a->want_dbias) ce_db_kernel<F32><<<dim3((a->classes + 255) / 256, (l.cap + kDbRows - 1) / kDbRows), 256, 0, q>>>(c, row0);
+    if (a->want_dx) ce_dx_rows_kernel<F32><<<a->rows, 256, 0, q>>>(c, row0);
   }
   if (a->want_dweight && l.dwacc) ce_dw_round_kernel<<<2048, 256, 0, q>>>(c.dwacc, (bf16 *)c.dw, (long long)a->classes * a->hidden);
   ce_finish_kernel<<<1 + (a->want_dbias ? (a->classes + 63) / 64 : 0), 256, 0, q>>>(c, l.db_slices);
