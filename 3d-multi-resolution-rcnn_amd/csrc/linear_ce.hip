@@ -112,41 +112,64 @@ __device__ __forceinline__ float block_max(float v, float *lds) {
   return fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
 }
 
-// largest |p[k]| of a row, by one wave: 16 bytes a load with the alignment of a float (odd strides)
-__device__ __forceinline__ float row_max(const float *p, int n) {
-  typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
-  float m = 0.f;
-  int k = (threadIdx.x & 63) * 4;
-#pragma unroll 4
-  for (; k + 4 <= n; k += 256) {
-    const f4 t = *reinterpret_cast<const f4 *>(p + k);
-    m = fmaxf(fmaxf(fmaxf(m, fabsf(t[0])), fabsf(t[1])), fmaxf(fabsf(t[2]), fabsf(t[3])));
-  }
-  for (; k < n; ++k) m = fmaxf(m, fabsf(p[k]));            // the last, partial group: one lane's
+// largest |p[k]| of each of kMaxRows rows as far as this lane sees it: 16 bytes a load with the alignment of a float (odd strides), the rows side
+// by side so that a short one does not leave the wave waiting.  Rows that do not exist repeat the first
+constexpr int kMaxRows = 4;
+__device__ __forceinline__ void rows_max(const float *const (&p)[kMaxRows], int n, float (&m)[kMaxRows]) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  return m;
+  for (int r = 0; r < kMaxRows; ++r) m[r] = 0.f;
+  int k = (threadIdx.x & 63) * 4;
+#pragma unroll 2
+  for (; k + 4 <= n; k += 256)
+#pragma unroll
+    for (int r = 0; r < kMaxRows; ++r) {
+      const vf4 t = *reinterpret_cast<const vf4 *>(p[r] + k);
+      m[r] = fmaxf(fmaxf(fmaxf(m[r], fabsf(t[0])), fabsf(t[1])), fmaxf(fabsf(t[2]), fabsf(t[3])));
+    }
+  for (; k < n; ++k)                                        // the last, partial group: one lane's
+#pragma unroll
+    for (int r = 0; r < kMaxRows; ++r) m[r] = fmaxf(m[r], fabsf(p[r][k]));
 }
 
-// fp32: the largest |x| of each live row and |x w| of all, the largest |W|; a wave per row, the first `xblocks` workgroups take x, the rest W.
+// fp32: the largest |x| of each live row and |x w| of all, the largest |W|; four rows a wave, the first `xblocks` workgroups take x, the rest W.
 // The maximum of positive floats is the maximum of their bits: an integer atomic, whose order does not matter -- one per workgroup, because
 // a thousand of them on one address take 15 us
 __global__ __launch_bounds__(256) void ce_max_kernel(Ce c, int xblocks, int wblocks) {
   __shared__ float lds[4];
-  float m = 0.f;
+  float m = 0.f, v[kMaxRows];
+  const float *p[kMaxRows];
   const int wave = threadIdx.x >> 6;
   const bool is_x = (int)blockIdx.x < xblocks;
   if (is_x) {
     const int live = c.head[0];
-    for (int j = blockIdx.x * 4 + wave; j < live; j += xblocks * 4) {
-      const int r = c.index[j];
-      const float v = row_max((const float *)c.x + r * c.x_stride, c.hidden);
-      if ((threadIdx.x & 63) == 0) c.xmax[j] = v;
-      const float w = v * fabsf(c.row_weight ? c.row_weight[r] : 1.f);
-      m = fmaxf(m, w < 3.0e38f ? w : INFINITY);             // a NaN weight counts as infinite: the scale falls back to 1
+    for (int j = (blockIdx.x * 4 + wave) * kMaxRows; j < live; j += xblocks * 4 * kMaxRows) {
+      int row[kMaxRows];
+#pragma unroll
+      for (int r = 0; r < kMaxRows; ++r) {
+        row[r] = c.index[j + r < live ? j + r : j];
+        p[r] = (const float *)c.x + row[r] * c.x_stride;
+      }
+      rows_max(p, c.hidden, v);
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1)
+#pragma unroll
+        for (int r = 0; r < kMaxRows; ++r) v[r] = fmaxf(v[r], __shfl_xor(v[r], o));
+#pragma unroll
+      for (int r = 0; r < kMaxRows; ++r) {
+        if (j + r >= live) break;
+        if ((threadIdx.x & 63) == 0) c.xmax[j + r] = v[r];
+        const float w = v[r] * fabsf(c.row_weight ? c.row_weight[row[r]] : 1.f);
+        m = fmaxf(m, w < 3.0e38f ? w : INFINITY);           // a NaN weight counts as infinite: the scale falls back to 1
+      }
     }
   } else {
-    for (int v = (blockIdx.x - xblocks) * 4 + wave; v < c.classes; v += wblocks * 4) m = fmaxf(m, row_max((const float *)c.w + v * c.w_stride, c.hidden));
+    for (int j = ((blockIdx.x - xblocks) * 4 + wave) * kMaxRows; j < c.classes; j += wblocks * 4 * kMaxRows) {
+#pragma unroll
+      for (int r = 0; r < kMaxRows; ++r) p[r] = (const float *)c.w + (j + r < c.classes ? j + r : j) * c.w_stride;
+      rows_max(p, c.hidden, v);
+#pragma unroll
+      for (int r = 0; r < kMaxRows; ++r) m = fmaxf(m, v[r]);
+    }
   }
   m = block_max(m, lds);
   if (threadIdx.x == 0 && m > 0.f) atomicMax(&c.head[is_x ? 3 : 2], __float_as_int(m));
@@ -724,7 +747,7 @@ template <bool F32> int run_ce(const mr3d_linear_ce *a, const Layout &l, Ce &c, 
   typedef Tiles<true, true, F32> TW;
   ce_rows_kernel<<<1, 1024, 0, q>>>(c);
   if (F32) {
-    const int xb = a->rows < 512 ? (a->rows + 3) / 4 : 128, wb = a->classes < 2048 ? (a->classes + 3) / 4 : 512;
+    const int per = 4 * kMaxRows, xb = a->rows < 128 * per ? (a->rows + per - 1) / per : 128, wb = a->classes < 512 * per ? (a->classes + per - 1) / per : 512;
     ce_max_kernel<<<xb + wb, 256, 0, q>>>(c, xb, wb);
   }
   ce_pack_kernel<F32><<<a->rows + (l.pack_w ? a->classes : 0), 256, 0, q>>>(c, a->want_dweight);
