@@ -420,12 +420,11 @@ template <class T> __device__ __forceinline__ void dx_tile(const Ce &c, int row0
 }
 
 // dx rows of the caller: the parts of a live row added up, zeros for the others
-template <bool F32>
-__global__ __launch_bounds__(256) void ce_dx_rows_kernel(Ce c, int row0) {
+template <bool F32> __device__ __forceinline__ void dx_row(const Ce &c, int row0, int r) {
   const int live = min(c.head[0] - row0, c.cap);
   const int hp = (c.hidden + 3) / 4 * 4;
   const float avg = ((const float *)c.head)[1], rsw = F32 ? 1.f / scale_of(c, 2) : 1.f;
-  const int r = blockIdx.x, p = c.pos[r];
+  const int p = c.pos[r];
   if (p < 0 ? row0 != 0 : (p < row0 || p >= row0 + live)) return;            // another piece's row
   const float f = F32 ? (c.row_weight ? c.row_weight[r] : 1.f) / avg * (rsw / kSG) : 1.f;
   for (int k = threadIdx.x * 4; k < c.hidden; k += 1024) {
@@ -571,9 +570,14 @@ template <bool F32> __global__ __launch_bounds__(256) void ce_db_kernel(Ce c, in
   db_part<F32>(c, row0, blockIdx.x, blockIdx.y, lds);
 }
 
-// The last launch.  Workgroup 0: the loss, row by row in order; the others (want_db): db, 64 columns each, the slices four side by side
-__global__ __launch_bounds__(256) void ce_finish_kernel(Ce c, int slices) {
+// rows of dx of all pieces but the last
+template <bool F32> __global__ __launch_bounds__(256) void ce_dx_rows_kernel(Ce c, int row0) { dx_row<F32>(c, row0, blockIdx.x); }
+
+// The last launch.  Workgroup 0: the loss, row by row in order; the next db_blocks: db, 64 columns each, the slices four side by side; the others:
+// the rows of dx of the last piece (from row0 on)
+template <bool F32> __global__ __launch_bounds__(256) void ce_finish_kernel(Ce c, int slices, int db_blocks, int row0) {
   __shared__ double sum[4][64];
+  if ((int)blockIdx.x > db_blocks) return dx_row<F32>(c, row0, blockIdx.x - 1 - db_blocks);
   if (blockIdx.x == 0) {
     double s = 0;
     const int live = c.head[0];
@@ -776,10 +780,11 @@ template <bool F32> int run_ce(const mr3d_linear_ce *a, const Layout &l, Ce &c, 
       if (e) return e;
       if (a->want_dbias) ce_db_kernel<F32><<<dim3((a->classes + 255) / 256, (l.cap + kDbRows - 1) / kDbRows), 256, 0, q>>>(c, row0);
     }
-    if (a->want_dx) ce_dx_rows_kernel<F32><<<a->rows, 256, 0, q>>>(c, row0);
+    if (a->want_dx && k + 1 < l.chunks) ce_dx_rows_kernel<F32><<<a->rows, 256, 0, q>>>(c, row0);
   }
   if (a->want_dweight && l.dwacc) ce_dw_round_kernel<<<2048, 256, 0, q>>>(c.dwacc, (bf16 *)c.dw, (long long)a->classes * a->hidden);
-  ce_finish_kernel<<<1 + (a->want_dbias ? (a->classes + 63) / 64 : 0), 256, 0, q>>>(c, l.db_slices);
+  const int db_blocks = a->want_dbias ? (a->classes + 63) / 64 : 0;
+  ce_finish_kernel<F32><<<1 + db_blocks + (a->want_dx ? a->rows : 0), 256, 0, q>>>(c, l.db_slices, db_blocks, (l.chunks - 1) * l.cap);
   return mr3d_launch_status();
 }
 
