@@ -10,9 +10,13 @@
 // of the 16-bit matrix pipe, fp32 accumulators.  Plain bf16 or fp16 factors would lose 2e-2 / 2e-3 of the result over five steps (p's slope at 0
 // is a = 3.4: rounding errors of the first steps are amplified a few hundred times).  Symmetric results: only the tiles on and below the diagonal are
 // computed and stored twice.  Iterating on A here too, in rounds of two or three steps between looks at X, was measured: 1.6 to 2.4 times fewer
-// products at n = 9 m, but no less time (940 us for the 64 matrices of a detector either way: the m x m products are short) and A's noise, amplified,
+// products at n = 9 m, but no less time for the 64 matrices of a detector (the m x m products are short), and A's noise, amplified,
 // takes the result from 1.0e-6 to 2.5e-6 (two steps) or 5e-6 (three) where plain fp32 loses 1.6e-6.
+// In bf16 lists the last two steps with the hi planes alone were measured too: 4096 x 4096 3.92 -> 3.52 ms (such tiles wait for their loads: half of every
+// cache line is unused), the error against 64 bits 1.12 times that of rounding the result: not taken.
 // MFMA-bound on large matrices; on small ones the dependent launches are what counts, hence the list and the small path.
+// Measured: 64 x 1728 75 us (A 9, the iteration 46: 17 products of 1.3 us of the double matrix pipe each and their barriers; Q G 15), 777 x 2311 and
+// 333 x 1301 295 us (15 products of 13 to 22 us), the 64 matrices of a detector (179 GFLOP) 1.02 ms, 4096 x 4096 bf16 3.8 to 3.9 ms (1.06 PFLOP/s of passes).
 #include "gemm16.h"
 #include <new>
 
@@ -561,7 +565,7 @@ size_t take(size_t &at, size_t bytes) {
 // Splitting.  `resident` workgroups run at a time (512 of the 128-wide tiles, 768 of the 64-wide ones); what is left over after whole rounds of them leaves
 // most of the chip idle for a round.  Those tiles -- all tiles of a list that does not fill one round, else tiles of the list's largest matrix -- are
 // computed by z workgroups each, for the z with the least estimated time: a round of z-th parts takes 1.45 us a k-step (64-wide: 0.5) over z,
-// the parts travel through memory and back at 4 TB/s, their join is a launch of 6 us (4096 x 4096: 528 tiles on and below the diagonal, 238 -> 215 us).
+// the parts travel through memory and back at 4 TB/s, their join is a launch of 6 us (4096 x 4096: 528 tiles on and below the diagonal, 240 -> 202 us).
 Split split_for(long long tiles, long long list_tiles, bool carries_rest, int steps, int bt) {
   const long long resident = bt == 128 ? 512 : 768, rest = list_tiles < resident ? list_tiles : list_tiles % resident;
   const bool all = list_tiles < resident;
@@ -694,7 +698,7 @@ struct Launcher {
     ortho_product_kernel<KIND, BT, FINE><<<plan.blocks[stage], kThreads, Pick<BT, KIND == 2, FINE>::T::LDS_BYTES, q>>>(ws, mats, maps.map[stage], op);
     if (plan.blocks[stage + 1]) ortho_join_kernel<KIND, BT><<<plan.blocks[stage + 1], kThreads, 0, q>>>(ws, mats, maps.map[stage + 1], op);
   }
-  // fp32 results: sums restarted every 16 k (2e-6 -> 1e-6 of the result); bf16 ones are rounded to 2^-9 anyway
+  // fp32 results: sums restarted every 32 k instead of 128 (2e-6 -> 1.2e-6 of the result, 10 % slower); bf16 ones are rounded to 2^-9 anyway
   template <int KIND> void product(const Op &op, int stage, int bt) const {
     if (bt == 128) plan.fine ? tiles<KIND, 128, true>(op, stage) : tiles<KIND, 128, false>(op, stage);
     else plan.fine ? tiles<KIND, 64, true>(op, stage) : tiles<KIND, 64, false>(op, stage);
