@@ -326,15 +326,41 @@ __device__ __forceinline__ double block_sum(double v, double *lds) {
   return lds[0] + lds[1] + lds[2] + lds[3];
 }
 
+// two sums at once, the same in every thread
+__device__ __forceinline__ void block_sum(double &a, double &b, double (*lds)[4]) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    a += __shfl_xor(a, o);
+    b += __shfl_xor(b, o);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    lds[0][threadIdx.x >> 6] = a;
+    lds[1][threadIdx.x >> 6] = b;
+  }
+  __syncthreads();
+  a = lds[0][0] + lds[0][1] + lds[0][2] + lds[0][3];
+  b = lds[1][0] + lds[1][1] + lds[1][2] + lds[1][3];
+}
+
 // one live row: log-sum-exp, loss, and (TRAIN) the exponentials become g.  `wcols`: classes of a (max, sum) pair
 template <bool F32, bool TRAIN>
 __global__ __launch_bounds__(256) void ce_grad_kernel(Ce c, int row0, int wcols) {
-  __shared__ double lds[4];
+  __shared__ double lds[2][4];
   __shared__ float ldm[4];
   const int j = blockIdx.x;
   if (j >= min(c.head[0] - row0, c.cap)) return;
   const int r = c.index[row0 + j];
   const float2 *st = c.stats + (long long)j * c.pieces;
+  // the label's logit first: its loads wait for row and label, the pairs' do not
+  const long long label = c.labels[r];
+  const bool known = label >= 0 && label < c.classes;        // else: the loss and this row's gradient are NaN
+  double dot = 0;
+  if (known) {
+#pragma unroll 4
+    for (int k = threadIdx.x; k < c.hidden; k += 256)
+      dot += (double)elem<F32>(c.x, r * c.x_stride + k) * (double)elem<F32>(c.w, label * c.w_stride + k);
+    if (threadIdx.x == 0 && c.bias) dot += c.bias_f32 ? (double)((const float *)c.bias)[label] : (double)(float)((const bf16 *)c.bias)[label];
+  }
   float m = -INFINITY;
   bool nan = false;
   for (int k = threadIdx.x; k < c.pieces; k += 256) {
@@ -342,21 +368,12 @@ __global__ __launch_bounds__(256) void ce_grad_kernel(Ce c, int row0, int wcols)
     nan |= v != v || st[k].y != st[k].y;                     // fmaxf drops a NaN
     m = fmaxf(m, v);
   }
-  m = block_max(m, ldm);
-  nan = __syncthreads_or(nan);
+  m = block_max(nan ? INFINITY : m, ldm);                    // infinity less infinity: the row's sums become NaN
   const float ms = m == -INFINITY ? 0.f : m;
   double s = 0;
   for (int k = threadIdx.x; k < c.pieces; k += 256) s += (double)st[k].y * (double)__builtin_amdgcn_exp2f(st[k].x - ms);
-  s = block_sum(s, lds);
-  const long long label = c.labels[r];
-  const bool known = label >= 0 && label < c.classes;        // else: the loss and this row's gradient are NaN
-  double dot = 0;
-  if (known)
-    for (int k = threadIdx.x; k < c.hidden; k += 256)
-      dot += (double)elem<F32>(c.x, r * c.x_stride + k) * (double)elem<F32>(c.w, label * c.w_stride + k);
-  dot = block_sum(dot, lds);
-  if (known && c.bias) dot += c.bias_f32 ? (double)((const float *)c.bias)[label] : (double)(float)((const bf16 *)c.bias)[label];
-  const double lse2 = known && !nan ? (double)m + log2(s) : (double)NAN, lse = lse2 * 0.69314718055994530942;
+  block_sum(s, dot, lds);
+  const double lse2 = known ? (double)m + log2(s) : (double)NAN, lse = lse2 * 0.69314718055994530942;
   const float w = c.row_weight ? c.row_weight[r] : 1.f;
   if (threadIdx.x == 0) c.row_loss[row0 + j] = (lse - dot) * (double)w;
   if constexpr (TRAIN) {
