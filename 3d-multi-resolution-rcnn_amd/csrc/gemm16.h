@@ -12,8 +12,8 @@
 // rounding of an fp32 sum, for three passes of the fp16 pipe -- whose rate is 16 times the fp32 pipe's.
 // The matrix instruction aligns its products and the accumulator to the largest of them and drops what lies 2 bits below that one's last place (16
 // products of 1/16 ulp of the accumulator add nothing), so a long sum of one sign drifts: 1e-5 of a sum of 3456 squares, 4e-5 of 9408.  Split
-// products therefore add the accumulators up in fp32 every 128 k and start again from zero: 3e-7 at any length, less than plain fp32 sums lose.
-// FINE ones do so every 32 k (1e-7; 10 % slower on the 128 x 128 tile).
+// products therefore add the accumulators up in fp32 every 128 k and start again from zero: 3e-7 at any length, less than plain fp32 sums lose
+// (every 32 k: 1e-7, and 10 % slower on the 128 x 128 tile).
 // bf16 products leave it at that: their results are rounded to 2^-9.
 //
 // v_mfma_f32_16x16x32 rather than 32x32x16: the chip is bound by power under such products, and the smaller shape sustains 1656 TFLOP/s from registers where
@@ -42,16 +42,15 @@ struct Side {
   unsigned ldb;
 };
 
-template <int BI_, int BJ_, int NWI_, int NWJ_, bool IKS_, bool JKS_, bool SPLIT_, int RB_, int STAGES_, bool FINE_ = false> struct Tile {
+template <int BI_, int BJ_, int NWI_, int NWJ_, bool IKS_, bool JKS_, bool SPLIT_, int RB_, int STAGES_> struct Tile {
   static constexpr int BI = BI_, BJ = BJ_, NWI = NWI_, NWJ = NWJ_, NW = NWI * NWJ, THREADS = NW * 64;
-  static constexpr bool IKS = IKS_, JKS = JKS_, SPLIT = SPLIT_, FINE = FINE_;
+  static constexpr bool IKS = IKS_, JKS = JKS_, SPLIT = SPLIT_;
   static constexpr int RB = RB_, STAGES = STAGES_;                          // bytes of a KC row per k-step, tiles in LDS
   static constexpr int TI = BI / NWI / 16, TJ = BJ / NWJ / 16;              // 16 x 16 blocks of a wave
   static constexpr int IBYTES = BI * RB, JBYTES = BJ * RB, STAGE = IBYTES + JBYTES, LDS_BYTES = STAGES * STAGE;
   static constexpr int KK = SPLIT ? RB / 4 : RB / 2;                        // k of a k-step
   static constexpr int NLI = IBYTES / 1024 / NW, NLJ = JBYTES / 1024 / NW;  // 1 KB loads of a wave per k-step
-  static constexpr int RESTART = !SPLIT || FINE ? 0 : 128 / KK;// k-steps between two restarts of the accumulators (0: never)
-  static_assert(SPLIT || !FINE, "");
+  static constexpr int RESTART = SPLIT ? 128 / KK : 0;                     // k-steps between two restarts of the accumulators (0: never)
   static_assert(!SPLIT || TI * TJ <= 16, "accumulators and their sums fit the registers");
   static_assert(IBYTES % (1024 * NW) == 0 && JBYTES % (1024 * NW) == 0, "whole 1 KB loads per wave");
   static_assert(RB == 128 || (RB == 64 && !SPLIT), "a split row's group is 128 bytes");
@@ -230,14 +229,13 @@ __device__ __forceinline__ void run(char *lds, Side si, Side sj, int nsteps, f32
         }
 #pragma unroll
         for (int b = 0; b < T::TJ; ++b) {
-          f32x4 t = T::FINE ? zero : acc[a][b];
+          f32x4 t = acc[a][b];
           if constexpr (T::SPLIT) {                        // small terms first: one rounding at the size of the result instead of three
             t = mfma<true>(fi[slot][0], fj[w][b][1], t);
             t = mfma<true>(fi[slot][1], fj[w][b][0], t);
           }
           t = mfma<T::SPLIT>(fi[slot][0], fj[w][b][0], t);
-          if constexpr (T::FINE) acc[a][b] += t;
-          else acc[a][b] = t;
+          acc[a][b] = t;
         }
         constexpr int M = T::TJ * (T::SPLIT ? 3 : 1);
 #pragma unroll

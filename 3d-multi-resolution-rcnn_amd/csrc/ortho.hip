@@ -16,7 +16,7 @@
 // cache line is unused), the error against 64 bits 1.12 times that of rounding the result: not taken.
 // MFMA-bound on large matrices; on small ones the dependent launches are what counts, hence the list and the small path.
 // Measured: 64 x 1728 75 us (A 9, the iteration 46: 17 products of 1.3 us of the double matrix pipe each and their barriers; Q G 15), 777 x 2311 and
-// 333 x 1301 295 us (15 products of 13 to 22 us), the 64 matrices of a detector (179 GFLOP) 1.02 ms, 4096 x 4096 bf16 3.8 to 3.9 ms (1.06 PFLOP/s of passes).
+// 333 x 1301 287 us (15 products of 13 to 22 us), the 64 matrices of a detector (179 GFLOP) 0.95 ms, 4096 x 4096 bf16 3.8 to 3.9 ms (1.06 PFLOP/s of passes).
 #include "gemm16.h"
 #include <new>
 
@@ -30,7 +30,7 @@ constexpr int kSmall = 64;                                  // rows of the small
 constexpr int kThreads = 256;
 
 // 128 x 128 with two tiles in LDS, two workgroups a CU, or 64 x 64 with three and as many workgroups
-template <int BT, bool APPLY, bool FINE> struct Pick { typedef Tile<BT, BT, 2, 2, APPLY, false, true, 128, BT == 128 ? 2 : 3, FINE> T; };
+template <int BT, bool APPLY> struct Pick { typedef Tile<BT, BT, 2, 2, APPLY, false, true, 128, BT == 128 ? 2 : 3> T; };
 
 enum Stage { kNorm, kPack, kGram, kGramJoin, kSquare, kSquareJoin, kApply, kApplyJoin, kSmallGram, kSmallPoly, kSmallApply, kStages };
 enum Buf { kA, kP, kX0, kX1, kBufs };
@@ -54,7 +54,6 @@ static_assert(sizeof(Mat) <= 240, "sixteen of them are kernel arguments");
 struct Plan {
   int blocks[kStages];
   int bt_square, bt_gram, bt_apply;
-  bool fine;
   size_t bytes, mats_off, map_off[kStages];
 };
 
@@ -80,15 +79,15 @@ __global__ __launch_bounds__(64) void ortho_table_kernel(MatBatch batch, int cou
 // workgroup -> matrix, per stage
 struct Maps { int *map[kStages]; int blocks[kStages]; };
 __global__ __launch_bounds__(256) void ortho_map_kernel(const Mat *__restrict__ mats, int count, Maps maps) {
-  for (int s = 0; s < kStages; ++s)
-    for (int b = blockIdx.x * 256 + threadIdx.x; b < maps.blocks[s]; b += gridDim.x * 256) {
-      int lo = 0, hi = count - 1;
-      while (lo < hi) {                                     // the last matrix whose first workgroup is <= b
-        const int mid = (lo + hi + 1) / 2;
-        if (mats[mid].first[s] <= b) lo = mid; else hi = mid - 1;
-      }
-      maps.map[s][b] = lo;
+  const int s = blockIdx.y;
+  for (int b = blockIdx.x * 256 + threadIdx.x; b < maps.blocks[s]; b += gridDim.x * 256) {
+    int lo = 0, hi = count - 1;
+    while (lo < hi) {                                       // the last matrix whose first workgroup is <= b
+      const int mid = (lo + hi + 1) / 2;
+      if (mats[mid].first[s] <= b) lo = mid; else hi = mid - 1;
     }
+    maps.map[s][b] = lo;
+  }
 }
 
 __device__ __forceinline__ float read_in(char *ws, const Mat &p, long long off) {
@@ -281,9 +280,9 @@ __device__ __forceinline__ void tile_at(const Mat *__restrict__ mat, int t, int 
   }
 }
 
-template <int KIND, int BT, bool FINE>
+template <int KIND, int BT>
 __global__ __launch_bounds__(kThreads, 2) void ortho_product_kernel(char *ws, const Mat *__restrict__ mats, const int *__restrict__ map, Op op) {
-  typedef typename Pick<BT, KIND == 2, FINE>::T T;
+  typedef typename Pick<BT, KIND == 2>::T T;
   constexpr int kFirst = KIND == 0 ? kGram : KIND == 1 ? kSquare : kApply;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int b = blockIdx.x;
@@ -323,7 +322,7 @@ __global__ __launch_bounds__(kThreads, 2) void ortho_product_kernel(char *ws, co
 // the parts of split tiles, added in a fixed order; a workgroup takes four 16 x 16 blocks of every wave
 template <int KIND, int BT>
 __global__ __launch_bounds__(kThreads) void ortho_join_kernel(char *ws, const Mat *__restrict__ mats, const int *__restrict__ map, Op op) {
-  typedef typename Pick<BT, KIND == 2, false>::T T;
+  typedef typename Pick<BT, KIND == 2>::T T;
   constexpr int kFirst = KIND == 0 ? kGramJoin : KIND == 1 ? kSquareJoin : kApplyJoin, Q = T::TI * T::TJ / 4;
   const int b = blockIdx.x;
   const Mat *__restrict__ mat = mats + map[b];
@@ -599,7 +598,6 @@ int plan_list(const mr3d_matrix *in, int count, char *base, Plan &plan, Mat *mat
     if (g.dtype != MR3D_DTYPE_F32 && g.dtype != MR3D_DTYPE_BF16) return MR3D_ERR_UNSUPPORTED;
     const long long m = g.rows < g.cols ? g.rows : g.cols, n = g.rows < g.cols ? g.cols : g.rows;
     if (m <= kSmall) continue;
-    plan.fine |= g.dtype == MR3D_DTYPE_F32;
     for (int b = 0; b < 2; ++b) {
       const long long bt = b ? 128 : 64, tm = (m + bt - 1) / bt, tn = (n + bt - 1) / bt;
       sum.sym[b] += tm * (tm + 1) / 2;
@@ -694,15 +692,11 @@ struct Launcher {
   const Maps &maps;
   hipStream_t q;
 
-  template <int KIND, int BT, bool FINE> void tiles(const Op &op, int stage) const {
-    ortho_product_kernel<KIND, BT, FINE><<<plan.blocks[stage], kThreads, Pick<BT, KIND == 2, FINE>::T::LDS_BYTES, q>>>(ws, mats, maps.map[stage], op);
+  template <int KIND, int BT> void tiles(const Op &op, int stage) const {
+    ortho_product_kernel<KIND, BT><<<plan.blocks[stage], kThreads, Pick<BT, KIND == 2>::T::LDS_BYTES, q>>>(ws, mats, maps.map[stage], op);
     if (plan.blocks[stage + 1]) ortho_join_kernel<KIND, BT><<<plan.blocks[stage + 1], kThreads, 0, q>>>(ws, mats, maps.map[stage + 1], op);
   }
-  // fp32 results: sums restarted every 32 k instead of 128 (2e-6 -> 1.2e-6 of the result, 10 % slower); bf16 ones are rounded to 2^-9 anyway
-  template <int KIND> void product(const Op &op, int stage, int bt) const {
-    if (bt == 128) plan.fine ? tiles<KIND, 128, true>(op, stage) : tiles<KIND, 128, false>(op, stage);
-    else plan.fine ? tiles<KIND, 64, true>(op, stage) : tiles<KIND, 64, false>(op, stage);
-  }
+  template <int KIND> void product(const Op &op, int stage, int bt) const { bt == 128 ? tiles<KIND, 128>(op, stage) : tiles<KIND, 64>(op, stage); }
   void step(int x, bool last, float ca, float cb, float cc) const {
     product<0>(Op{x, kSA / (kSX * kSX), 0.f, 0.f, 0}, kGram, plan.bt_gram);
     product<1>(Op{x, cc * kSP / (kSA * kSA), cb * kSP / kSA, ca * kSP, 0}, kSquare, plan.bt_square);
@@ -754,7 +748,7 @@ extern "C" int mr3d_orthogonalize(const mr3d_matrix *mats_host, int count, int s
     most = plan.blocks[k] > most ? plan.blocks[k] : most;
   }
   const int mb = (most + 255) / 256;
-  ortho_map_kernel<<<mb < 256 ? mb : 256, 256, 0, q>>>(mats, count, maps);
+  ortho_map_kernel<<<dim3(mb < 256 ? mb : 256, kStages), 256, 0, q>>>(mats, count, maps);
   if (plan.blocks[kSmallPoly]) {
     ortho_small_gram_kernel<<<plan.blocks[kSmallGram], kThreads, 0, q>>>(base, mats, maps.map[kSmallGram]);
     ortho_small_poly_kernel<<<plan.blocks[kSmallPoly], kPolyThreads, kPolyLds, q>>>(base, mats, maps.map[kSmallPoly], steps, ca, cb, cc, eps);
