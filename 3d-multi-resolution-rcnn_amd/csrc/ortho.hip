@@ -15,8 +15,8 @@
 // In bf16 lists the last two steps with the hi planes alone were measured too: 4096 x 4096 3.92 -> 3.52 ms (such tiles wait for their loads: half of every
 // cache line is unused), the error against 64 bits 1.12 times that of rounding the result: not taken.
 // MFMA-bound on large matrices; on small ones the dependent launches are what counts, hence the list and the small path.
-// Measured: 64 x 1728 75 us (A 9, the iteration 46: 17 products of 1.3 us of the double matrix pipe each and their barriers; Q G 15), 777 x 2311 and
-// 333 x 1301 287 us (15 products of 13 to 22 us), the 64 matrices of a detector (179 GFLOP) 0.95 ms, 4096 x 4096 bf16 3.8 to 3.9 ms (1.06 PFLOP/s of passes).
+// Measured: 64 x 1728 70 us (A 9, the iteration 46: 17 products of 1.3 us of the double matrix pipe each and their barriers; Q G 12), 777 x 2311 and
+// 333 x 1301 287 us (15 products of 13 to 22 us), the 64 matrices of a detector (179 GFLOP) 0.96 ms, 4096 x 4096 bf16 3.8 to 3.9 ms (1.06 PFLOP/s of passes).
 #include "gemm16.h"
 #include <new>
 
@@ -49,7 +49,7 @@ struct Mat {
   Split gram, square, apply;
   int first[kStages];                                       // first workgroup of this matrix in each stage
 };
-static_assert(sizeof(Mat) <= 240, "sixteen of them are kernel arguments");
+static_assert(sizeof(Mat) <= 240, "fifteen of them, and the maps, are kernel arguments (4 KB)");
 
 struct Plan {
   int blocks[kStages];
@@ -57,7 +57,7 @@ struct Plan {
   size_t bytes, mats_off, map_off[kStages];
 };
 
-constexpr int kBatch = 16;
+constexpr int kBatch = 15;
 struct MatBatch { Mat m[kBatch]; };
 
 // Places are stored as distances from the workspace, a kernel argument: a pointer read from the table would count as generic, and generic (flat)
@@ -72,21 +72,16 @@ __device__ __forceinline__ int triangle(int t, int &ti) {
   return tj;
 }
 
-__global__ __launch_bounds__(64) void ortho_table_kernel(MatBatch batch, int count, int at, Mat *__restrict__ mats) {
-  if ((int)threadIdx.x < count) mats[at + threadIdx.x] = batch.m[threadIdx.x];
-}
-
-// workgroup -> matrix, per stage
-struct Maps { int *map[kStages]; int blocks[kStages]; };
-__global__ __launch_bounds__(256) void ortho_map_kernel(const Mat *__restrict__ mats, int count, Maps maps) {
+// The table in memory and, per stage, workgroup -> matrix.  A launch takes a batch of matrices as arguments and fills in both for its own: workgroups
+// from its first matrix's first one to `end`
+struct Maps { int *map[kStages]; int end[kStages]; };
+__global__ __launch_bounds__(256) void ortho_table_kernel(MatBatch batch, int count, int at, Mat *__restrict__ mats, Maps maps) {
   const int s = blockIdx.y;
-  for (int b = blockIdx.x * 256 + threadIdx.x; b < maps.blocks[s]; b += gridDim.x * 256) {
-    int lo = 0, hi = count - 1;
-    while (lo < hi) {                                       // the last matrix whose first workgroup is <= b
-      const int mid = (lo + hi + 1) / 2;
-      if (mats[mid].first[s] <= b) lo = mid; else hi = mid - 1;
-    }
-    maps.map[s][b] = lo;
+  if (s == 0 && blockIdx.x == 0 && (int)threadIdx.x < count) mats[at + threadIdx.x] = batch.m[threadIdx.x];
+  for (int b = batch.m[0].first[s] + blockIdx.x * 256 + threadIdx.x; b < maps.end[s]; b += gridDim.x * 256) {
+    int k = 0;                                              // the last matrix whose first workgroup is <= b
+    for (int i = 1; i < count; ++i) k = batch.m[i].first[s] <= b ? i : k;
+    maps.map[s][b] = at + k;
   }
 }
 
@@ -509,6 +504,19 @@ __global__ __launch_bounds__(kPolyThreads) void ortho_small_poly_kernel(char *ws
     if (k % kSmall < mp) o[k] = mats4[q][k / kSmall * kLdd + k % kSmall] * inv;
 }
 
+// acc = Q t for the 16 columns from c0 on
+template <int NB> __device__ __forceinline__ void small_apply(double (*q)[kSmall + 2], float (*t)[kChunk + 1], int c0, f64x4 (&acc)[4]) {
+  const int r = threadIdx.x & 15, kq = (threadIdx.x >> 4) & 3;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) acc[b] = f64x4{0, 0, 0, 0};
+#pragma unroll
+  for (int k = 0; k < NB * 16; k += 4) {
+    const double x = (double)t[k + kq][c0 + r];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[b] = __builtin_amdgcn_mfma_f64_16x16x4f64(q[b * 16 + r][k + kq], x, acc[b], 0, 0, 0);
+  }
+}
+
 // out = Q G, 64 columns a workgroup, in double too: Q reaches a^steps in the directions of small singular values, and its rounding to fp32 would show in
 // the others (1e-6).  Wave w has the columns 16 w .. 16 w + 15
 __global__ __launch_bounds__(kThreads) void ortho_small_apply_kernel(char *ws, const Mat *__restrict__ mats, const int *__restrict__ map) {
@@ -526,13 +534,11 @@ __global__ __launch_bounds__(kThreads) void ortho_small_apply_kernel(char *ws, c
   __syncthreads();
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kq = lane >> 4;
   f64x4 acc[4];
-#pragma unroll
-  for (int b = 0; b < 4; ++b) acc[b] = f64x4{0, 0, 0, 0};
-  for (int k = 0; k < mp; k += 4) {
-    const double x = (double)t[k + kq][wave * 16 + r];
-#pragma unroll
-    for (int b = 0; b < 4; ++b)
-      if (b < nb) acc[b] = __builtin_amdgcn_mfma_f64_16x16x4f64(q[b * 16 + r][k + kq], x, acc[b], 0, 0, 0);
+  switch (nb) {
+    case 1: small_apply<1>(q, t, wave * 16, acc); break;
+    case 2: small_apply<2>(q, t, wave * 16, acc); break;
+    case 3: small_apply<3>(q, t, wave * 16, acc); break;
+    default: small_apply<4>(q, t, wave * 16, acc);
   }
   __syncthreads();
 #pragma unroll
@@ -733,22 +739,21 @@ extern "C" int mr3d_orthogonalize(const mr3d_matrix *mats_host, int count, int s
   }
   hipStream_t q = mr3d_stream(s);
   Mat *mats = (Mat *)(base + plan.mats_off);
+  Maps maps;
+  for (int s = 0; s < kStages; ++s) maps.map[s] = (int *)(base + plan.map_off[s]);
   for (int at = 0; at < count; at += kBatch) {
     MatBatch b;
     const int n = count - at < kBatch ? count - at : kBatch;
     for (int k = 0; k < n; ++k) b.m[k] = table[at + k];
-    ortho_table_kernel<<<1, 64, 0, q>>>(b, n, at, mats);
+    int most = 1;
+    for (int s = 0; s < kStages; ++s) {
+      maps.end[s] = at + n < count ? table[at + n].first[s] : plan.blocks[s];
+      most = maps.end[s] - b.m[0].first[s] > most ? maps.end[s] - b.m[0].first[s] : most;
+    }
+    const int mb = (most + 255) / 256;
+    ortho_table_kernel<<<dim3(mb < 256 ? mb : 256, kStages), 256, 0, q>>>(b, n, at, mats, maps);
   }
   delete[] table;
-  Maps maps;
-  int most = 0;
-  for (int k = 0; k < kStages; ++k) {
-    maps.map[k] = (int *)(base + plan.map_off[k]);
-    maps.blocks[k] = plan.blocks[k];
-    most = plan.blocks[k] > most ? plan.blocks[k] : most;
-  }
-  const int mb = (most + 255) / 256;
-  ortho_map_kernel<<<dim3(mb < 256 ? mb : 256, kStages), 256, 0, q>>>(mats, count, maps);
   if (plan.blocks[kSmallPoly]) {
     ortho_small_gram_kernel<<<plan.blocks[kSmallGram], kThreads, 0, q>>>(base, mats, maps.map[kSmallGram]);
     ortho_small_poly_kernel<<<plan.blocks[kSmallPoly], kPolyThreads, kPolyLds, q>>>(base, mats, maps.map[kSmallPoly], steps, ca, cb, cc, eps);
