@@ -12,7 +12,7 @@ def linear_cross_entropy(x, weight, label, row_weight=None, bias=None, avg_facto
     A row counts when its weight is not 0, its label is not ignore_index and it lies before valid_rows (a device int32 scalar: static
     shapes with padding).  The others take no part, whatever they hold, and get zero gradients.  avg_factor: a number, a device scalar, or None for
     max(number of counted rows with a positive weight, 1), as `weighted_cross_entropy` divides.  A counted label outside [0, C) makes the loss NaN.
-    The memory beside the gradients is bounded (2 GiB of exponentials, rows go through in pieces).  fp32: products carry 22 bits of
+    Beside copies of x and weight the memory is bounded (2 GiB of exponentials, rows go through in pieces).  fp32: products carry 22 bits of
     each factor.  One backward per call; under graph capture both are captured (as `torch.cuda.make_graphed_callables` does) or neither."""
     on_device = torch.is_tensor(avg_factor)
     return _hip.train_ops().linear_cross_entropy(x, weight, label, row_weight, bias, avg_factor if on_device else None,

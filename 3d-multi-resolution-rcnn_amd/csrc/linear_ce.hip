@@ -445,7 +445,7 @@ template <bool F32> __device__ __forceinline__ void dx_row(const Ce &c, int row0
   const int hp = (c.hidden + 3) / 4 * 4;
   const float avg = ((const float *)c.head)[1], rsw = F32 ? 1.f / scale_of(c, 2) : 1.f;
   const int p = c.pos[r];
-  if (p < 0 ? row0 != 0 : (p < row0 || p >= row0 + live)) return;            // another piece's row
+  if (p >= 0 && (p < row0 || p >= row0 + live)) return;                       // another piece's row
   const float f = F32 ? (c.row_weight ? c.row_weight[r] : 1.f) / avg * (rsw / kSG) : 1.f;
   for (int k = threadIdx.x * 4; k < c.hidden; k += 1024) {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -563,7 +563,9 @@ template <bool F32> __device__ __forceinline__ void db_part(const Ce &c, int row
   float t = 0.f;
 #pragma unroll
   for (int k = 0; k < 8; ++k) t += sum[k][threadIdx.x];
-  c.dbpart[(long long)(row0 / kDbRows + slice) * c.classes + o] = F32 ? t / (kSG * ((const float *)c.head)[1]) : t;
+  if (F32) t /= kSG * ((const float *)c.head)[1];
+  float *d = c.dbpart + (long long)slice * c.classes + o;
+  *d = row0 ? *d + t : t;                                    // pieces one after the other
 }
 
 // The gradients' launches.  Tiles of 64 and 128 (one workgroup shape) share one launch with db's sums: each of the three alone leaves CUs idle
@@ -590,11 +592,13 @@ template <bool F32> __global__ __launch_bounds__(256) void ce_db_kernel(Ce c, in
   db_part<F32>(c, row0, blockIdx.x, blockIdx.y, lds);
 }
 
-// rows of dx of all pieces but the last
-template <bool F32> __global__ __launch_bounds__(256) void ce_dx_rows_kernel(Ce c, int row0) { dx_row<F32>(c, row0, blockIdx.x); }
+// live rows of dx of a piece that is not the last
+template <bool F32> __global__ __launch_bounds__(256) void ce_dx_rows_kernel(Ce c, int row0) {
+  if (row0 + (int)blockIdx.x < c.head[0]) dx_row<F32>(c, row0, c.index[row0 + blockIdx.x]);
+}
 
 // The last launch.  Workgroup 0: the loss, row by row in order; the next db_blocks: db, 64 columns each, the slices four side by side; the others:
-// the rows of dx of the last piece (from row0 on)
+// the rows of dx of the last piece (from row0 on) and those that do not count
 template <bool F32> __global__ __launch_bounds__(256) void ce_finish_kernel(Ce c, int slices, int db_blocks, int row0) {
   __shared__ double sum[4][64];
   if ((int)blockIdx.x > db_blocks) return dx_row<F32>(c, row0, blockIdx.x - 1 - db_blocks);
@@ -720,7 +724,7 @@ int layout_of(const mr3d_linear_ce *a, Layout &l) {
   l.bt_dw = tile_for(f32, a->hidden, a->classes, 1);
   if (a->want_dweight && !f32 && l.chunks > 1) l.dwacc = take(at, (size_t)a->classes * a->hidden * 4);
   if (a->want_dbias) {
-    l.db_slices = (int)(l.chunks * ((cap + kDbRows - 1) / kDbRows));
+    l.db_slices = (int)((cap + kDbRows - 1) / kDbRows);
     l.dbpart = take(at, (size_t)l.db_slices * a->classes * 4);
   }
   l.bytes = at;
@@ -800,7 +804,7 @@ template <bool F32> int run_ce(const mr3d_linear_ce *a, const Layout &l, Ce &c, 
       if (e) return e;
       if (a->want_dbias) ce_db_kernel<F32><<<dim3((a->classes + 255) / 256, (l.cap + kDbRows - 1) / kDbRows), 256, 0, q>>>(c, row0);
     }
-    if (a->want_dx && k + 1 < l.chunks) ce_dx_rows_kernel<F32><<<a->rows, 256, 0, q>>>(c, row0);
+    if (a->want_dx && k + 1 < l.chunks) ce_dx_rows_kernel<F32><<<l.cap, 256, 0, q>>>(c, row0);
   }
   if (a->want_dweight && l.dwacc) ce_dw_round_kernel<<<2048, 256, 0, q>>>(c.dwacc, (bf16 *)c.dw, (long long)a->classes * a->hidden);
   const int db_blocks = a->want_dbias ? (a->classes + 63) / 64 : 0;

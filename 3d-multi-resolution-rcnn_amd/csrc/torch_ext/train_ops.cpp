@@ -234,7 +234,8 @@ at::Tensor linear_cross_entropy(const at::Tensor &x, const at::Tensor &weight, c
     TORCH_CHECK_NOT_IMPLEMENTED(!row_weight->requires_grad(), "linear_cross_entropy is not differentiable in row_weight");
   }
   TORCH_CHECK_VALUE(!avg_dev || (avg_dev->numel() == 1 && avg_dev->device() == x.device()), CE "avg_factor is a number or one value on the device of x");
-  TORCH_CHECK_VALUE(!avg_host || *avg_host > 0, CE "avg_factor is positive");
+  TORCH_CHECK_NOT_IMPLEMENTED(!avg_dev || !avg_dev->requires_grad(), "linear_cross_entropy is not differentiable in avg_factor");
+  TORCH_CHECK_VALUE(!avg_host || (float)*avg_host > 0, CE "avg_factor is positive in float32");
   TORCH_CHECK_VALUE(!valid_rows || (valid_rows->numel() == 1 && valid_rows->scalar_type() == at::kInt), CE "valid_rows is one int32 value on the device");
   for (const at::Tensor &t : {weight, or_none(bias), label, or_none(row_weight), or_none(valid_rows)})
     TORCH_CHECK_VALUE(!t.defined() || t.device() == x.device(), CE "all tensors are on one device");

@@ -539,7 +539,8 @@ int mr3d_layer_norm_backward(const void *x, long long x_stride, const void *dy, 
  * A counted row whose label is outside [0, classes) makes the loss, its dx row and dweight NaN.  want_*: which gradients are written.
  * fp32 products carry 22 bits of each factor, bf16 gradients of the logits are rounded to bf16 once more; sums are fp32 or wider, in a
  * fixed order.  hidden <= 65536, classes <= 2^20, rows <= 2^22.  workspace: 1024-byte aligned device memory of
- * mr3d_linear_cross_entropy_workspace_bytes (0 = refused; the exponentials in it are bounded by 2 GiB, rows go through in pieces).
+ * mr3d_linear_cross_entropy_workspace_bytes (0 = refused): x (and, fp32 or unaligned, weight) in packed form, dx in fp32, and at most about
+ * 2 GiB of exponentials, as many rows at a time as fit (256 at least).
  * mr3d_scale_by: up to 4 arrays *= *factor_dev in place, in one launch; nothing is touched when the factor is 1.
  * ---------------------------------------------------------------------------------------------- */
 typedef struct {

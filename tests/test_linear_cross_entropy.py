@@ -150,6 +150,25 @@ def test_rows_in_pieces(dtype, monkeypatch):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_bias_gradient_over_pieces(dtype):
+    """the same g, summed over pieces or over halves: 8 rows a thread, 8 threads, 16 slices of 64 rows, all fp32 -- 32 roundings of at most
+    sum |g| = |sum g| + 2 |g of the label|, a label's being at most max rw / avg, and one in the type of b"""
+    v = (1 << 20) - 13
+    x, w, b, label, rw = _inputs(1100, 8, v, dtype, seed=3, dead=0.1, scale=1.0)
+    b = b.float()
+    got = _run(x, w, b, label, rw, avg_factor=1000.0)
+    s = torch.zeros(v, dtype=torch.float64, device='cuda')
+    for sl in (slice(0, 600), slice(600, None)):
+        lab = torch.full_like(label, -100)
+        lab[sl] = label[sl]
+        s += _run(x, w, b, lab, rw, avg_factor=1000.0)['db'].double()
+    hits = torch.bincount(label[label >= 0], minlength=v).double().cuda()
+    assert bool(((got['db'].double() - s).abs() <= 2 * 32 * U * (s.abs() + 2 * hits * 1.25 / 1000) + 3 * U * s.abs()).all())
+    assert float((got['dx'][label == -100]).abs().max()) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 def test_rows_that_do_not_count_may_hold_anything(dtype):
     x, w, b, label, rw = _inputs(150, 64, 400, dtype)
     rw[5], rw[6], label[9] = 0.0, -0.0, -7
@@ -454,6 +473,10 @@ def test_refusals_need_no_gpu():
         ce(x, torch.zeros(1, 8).expand((1 << 20) + 1, 8), lab)
     with pytest.raises(NotImplementedError):
         ce(x, w, lab, torch.ones(4, requires_grad=True))
+    with pytest.raises(NotImplementedError, match='avg_factor'):
+        ce(x, w, lab, avg_factor=torch.ones(1, requires_grad=True))
+    with pytest.raises(ValueError):
+        ce(x, w, lab, avg_factor=1e-60)
     L = lib()
     base = dict(x=1024, weight=1024, bias=1024, labels=1024, loss=1024, dx=1024, dweight=1024, dbias=1024, x_stride=8, weight_stride=8, ignore_index=-100,
                 rows=4, hidden=8, classes=10, dtype=0, param_dtype=0, want_dx=1, want_dweight=1, want_dbias=1)
