@@ -68,6 +68,21 @@ def test_list_of_mixed_shapes_types_and_axes_equals_the_single_calls():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('count', [15, 16, 47])
+def test_long_lists(count):
+    """more matrices than one launch takes as arguments, small and large ones mixed, runs of either"""
+    from mr3d_amd.core import orthogonalize
+    g = torch.Generator().manual_seed(count)
+    mats = []
+    for k in range(count):
+        lo, hi = ((1, 64) if k % 20 < 8 else (65, 200) if k % 20 < 16 else (1, 200))
+        m, n = (int(v) for v in torch.randint(lo, hi + 1, (2,), generator=g))
+        mats.append(_gauss(m, n, k, torch.bfloat16 if k % 5 == 4 else torch.float32))
+    for got, want in zip(orthogonalize(mats), mats):
+        _check(got, want)
+
+
+@pytest.mark.gpu
 def test_spectra():
     """low rank, decaying spectrum, duplicated rows, one dominant direction, zeros"""
     from mr3d_amd.core import orthogonalize
