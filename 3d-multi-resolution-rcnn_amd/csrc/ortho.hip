@@ -567,23 +567,71 @@ size_t take(size_t &at, size_t bytes) {
   return here;
 }
 
-// Splitting.  `resident` workgroups run at a time (512 of the 128-wide tiles, 768 of the 64-wide ones); what is left over after whole rounds of them leaves
-// most of the chip idle for a round.  Those tiles -- all tiles of a list that does not fill one round, else tiles of the list's largest matrix -- are
-// computed by z workgroups each, for the z with the least estimated time: a round of z-th parts takes 1.45 us a k-step (64-wide: 0.5) over z,
-// the parts travel through memory and back at 4 TB/s, their join is a launch of 6 us (4096 x 4096: 528 tiles on and below the diagonal, 240 -> 202 us).
-Split split_for(long long tiles, long long list_tiles, bool carries_rest, int steps, int bt) {
-  const long long resident = bt == 128 ? 512 : 768, rest = list_tiles < resident ? list_tiles : list_tiles % resident;
-  const bool all = list_tiles < resident;
-  Split s{(int)tiles, (int)tiles, 1};
-  if (!rest || (!all && (!carries_rest || rest > tiles))) return s;
-  const double tile_us = steps * (bt == 128 ? 1.45 : 0.5), part_us = bt * bt * 8. / 4e6;
+// Splitting the k axis.  What a list (or its last round of workgroups) leaves idle is filled by computing tiles with z workgroups each: their parts travel
+// through memory and back at 4 TB/s and are joined by another launch of 6 us.
+//
+// A list of fewer tiles than run at a time (512 of the 128-wide ones, 768 of the 64-wide ones): parts of about `len` k-steps for every matrix, so that long
+// and short axes end together.  A k-step takes 0.7 us while a 128-wide tile has its CU alone, and as much longer as there are more on it; 64-wide tiles
+// 0.34 us alone, 0.5 for two and 0.7 for three a CU
+struct Work { long long tiles; int steps; };
+Work work_of(const mr3d_matrix &g, int kind, int bt) {
+  const long long m = g.rows < g.cols ? g.rows : g.cols, n = g.rows < g.cols ? g.cols : g.rows, tm = (m + bt - 1) / bt, tn = (n + bt - 1) / bt;
+  if (m <= kSmall) return {0, 0};
+  return {kind < 2 ? tm * (tm + 1) / 2 : tm * tn, (int)(((kind == 0 ? n : m) + 31) / 32)};
+}
+int part_length(const mr3d_matrix *in, int count, int kind, int bt) {
+  int longest = 0;
+  double total = 0;
+  for (int k = 0; k < count; ++k) {
+    const Work w = work_of(in[k], kind, bt);
+    longest = w.steps > longest ? w.steps : longest;
+    total += (double)w.tiles * w.steps;
+  }
+  const double part_us = bt * bt * 8. / 4e6;
+  double best = 1e30;
+  int best_len = longest;
+  for (const int div : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32}) {
+    const int len = (longest + div - 1) / div;
+    if (len < 4) break;
+    double us = 0;
+    for (int k = 0; k < count && div > 1; ++k) {
+      const Work w = work_of(in[k], kind, bt);
+      if (w.steps > len) us += part_us * (double)w.tiles * ((w.steps + len - 1) / len);
+    }
+    const double c = total / (256. * (double)len);          // workgroups a CU
+    const double step = bt == 128 ? 0.7 * (c > 1 ? c : 1) : c <= 1 ? 0.34 : c <= 2 ? 0.34 + 0.16 * (c - 1) : 0.5 + 0.2 * (c - 2);
+    us += (double)len * step + (div > 1 ? 6. : 0.);
+    if (us < best) {
+      best = us;
+      best_len = len;
+    }
+  }
+  return best_len;
+}
+
+// One matrix's share.  len > 0: parts of that many k-steps.  len 0 (a list that fills whole rounds of workgroups): the tiles left over after them, taken
+// from the list's largest matrix, for the z with the least estimated time (4096 x 4096: 528 tiles on and below the diagonal, 240 -> 202 us)
+Split split_for(int tiles, int steps, int len, long long list_tiles, bool carries_rest, int bt) {
+  Split s{tiles, tiles, 1};
+  if (len) {
+    int z = (steps + len - 1) / len;
+    z = z > 32 ? 32 : z;
+    if (z > 1) {
+      s.z = z;
+      s.whole = 0;
+    }
+    return s;
+  }
+  const long long resident = bt == 128 ? 512 : 768, rest = list_tiles % resident;
+  if (!rest || !carries_rest || rest > tiles) return s;
+  const double tile_us = steps * (bt == 128 ? 1.4 : 0.7), part_us = bt * bt * 8. / 4e6;
   double best = tile_us;
   for (int z = 2; z <= 32 && z <= steps / 4; ++z) {
     const double us = tile_us * (double)((rest * z + resident - 1) / resident) / z + part_us * (double)rest * z + 6.;
     if (us < best) {
       best = us;
       s.z = z;
-      s.whole = (int)(all ? 0 : tiles - rest);
+      s.whole = (int)(tiles - rest);
     }
   }
   return s;
@@ -621,6 +669,8 @@ int plan_list(const mr3d_matrix *in, int count, char *base, Plan &plan, Mat *mat
   plan.bt_gram = sum.parts >= 256 ? 128 : 64;
   plan.bt_apply = sum.apply[1] >= 192 ? 128 : 64;
   const long long list_gram = sum.sym[plan.bt_gram == 128], list_sym = sum.sym[plan.bt_square == 128], list_apply = sum.apply[plan.bt_apply == 128];
+  const auto length = [&](int kind, long long tiles, int bt) { return tiles < (bt == 128 ? 512 : 768) ? part_length(in, count, kind, bt) : 0; };
+  const int len_gram = length(0, list_gram, plan.bt_gram), len_square = length(1, list_sym, plan.bt_square), len_apply = length(2, list_apply, plan.bt_apply);
   long long blocks[kStages] = {};
   for (int k = 0; k < count; ++k) {
     const mr3d_matrix &g = in[k];
@@ -650,9 +700,9 @@ int plan_list(const mr3d_matrix *in, int count, char *base, Plan &plan, Mat *mat
       const long long tg = (p.m + plan.bt_gram - 1) / plan.bt_gram, ts = (p.m + plan.bt_square - 1) / plan.bt_square, tm = (p.m + plan.bt_apply - 1) / plan.bt_apply, tn = (p.n + plan.bt_apply - 1) / plan.bt_apply;
       const int ksm = (p.m + 31) / 32, ksn = (p.n + 31) / 32, qg = plan.bt_gram == 128 ? 4 : 1, qs = plan.bt_square == 128 ? 4 : 1, qa = plan.bt_apply == 128 ? 4 : 1;
       if (ts * (ts + 1) / 2 > 0x3fffffff || tg * (tg + 1) / 2 > 0x3fffffff || tm * tn > 0x3fffffff) return MR3D_ERR_UNSUPPORTED;
-      p.gram = split_for(tg * (tg + 1) / 2, list_gram, k == sum.carrier, ksn, plan.bt_gram);
-      p.square = split_for(ts * (ts + 1) / 2, list_sym, k == sum.carrier, ksm, plan.bt_square);
-      p.apply = split_for(tm * tn, list_apply, k == sum.carrier, ksm, plan.bt_apply);
+      p.gram = split_for((int)(tg * (tg + 1) / 2), ksn, len_gram, list_gram, k == sum.carrier, plan.bt_gram);
+      p.square = split_for((int)(ts * (ts + 1) / 2), ksm, len_square, list_sym, k == sum.carrier, plan.bt_square);
+      p.apply = split_for((int)(tm * tn), ksm, len_apply, list_apply, k == sum.carrier, plan.bt_apply);
       const long long numel = (long long)p.m * p.n;
       p.norm_blocks = (int)((numel + 8191) / 8192 > 1024 ? 1024 : (numel + 8191) / 8192);
       for (int b = 0; b < kBufs; ++b) {
