@@ -579,7 +579,7 @@ Work work_of(const mr3d_matrix &g, int kind, int bt) {
   if (m <= kSmall) return {0, 0};
   return {kind < 2 ? tm * (tm + 1) / 2 : tm * tn, (int)(((kind == 0 ? n : m) + 31) / 32)};
 }
-int part_length(const mr3d_matrix *in, int count, int kind, int bt) {
+int part_length(const mr3d_matrix *in, int count, int kind, int bt, double &best) {
   int longest = 0;
   double total = 0;
   for (int k = 0; k < count; ++k) {
@@ -588,7 +588,7 @@ int part_length(const mr3d_matrix *in, int count, int kind, int bt) {
     total += (double)w.tiles * w.steps;
   }
   const double part_us = bt * bt * 8. / 4e6;
-  double best = 1e30;
+  best = 1e30;
   int best_len = longest;
   for (const int div : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32}) {
     const int len = (longest + div - 1) / div;
@@ -644,7 +644,7 @@ int plan_list(const mr3d_matrix *in, int count, char *base, Plan &plan, Mat *mat
   plan = Plan{};
   size_t at = 0;
   plan.mats_off = take(at, (size_t)count * sizeof(Mat));
-  struct { long long sym[2], apply[2], parts, most; int carrier; } sum{};
+  struct { long long sym[2], apply[2], most; int carrier; } sum{};
   sum.carrier = -1;
   for (int k = 0; k < count; ++k) {
     const mr3d_matrix &g = in[k];
@@ -656,21 +656,27 @@ int plan_list(const mr3d_matrix *in, int count, char *base, Plan &plan, Mat *mat
       const long long bt = b ? 128 : 64, tm = (m + bt - 1) / bt, tn = (n + bt - 1) / bt;
       sum.sym[b] += tm * (tm + 1) / 2;
       sum.apply[b] += tm * tn;
-      if (b) sum.parts += tm * (tm + 1) / 2 * ((n + 511) / 512);
     }
     if (m * n > sum.most) {
       sum.most = m * n;
       sum.carrier = k;
     }
   }
-  // 64-wide tiles where 128-wide ones would leave CUs without one
-  plan.bt_square = sum.sym[1] >= 192 ? 128 : 64;
-  // X X^T has the long axis to split: 128-wide tiles as long as 16 k-steps a part make 256 workgroups of them
-  plan.bt_gram = sum.parts >= 256 ? 128 : 64;
-  plan.bt_apply = sum.apply[1] >= 192 ? 128 : 64;
-  const long long list_gram = sum.sym[plan.bt_gram == 128], list_sym = sum.sym[plan.bt_square == 128], list_apply = sum.apply[plan.bt_apply == 128];
-  const auto length = [&](int kind, long long tiles, int bt) { return tiles < (bt == 128 ? 512 : 768) ? part_length(in, count, kind, bt) : 0; };
-  const int len_gram = length(0, list_gram, plan.bt_gram), len_square = length(1, list_sym, plan.bt_square), len_apply = length(2, list_apply, plan.bt_apply);
+  // tile width and part length of each product: the pair with the least estimated time; 128 once 64-wide tiles fill a round
+  int bt[3], len[3];
+  long long list[3];
+  for (int kind = 0; kind < 3; ++kind) {
+    const long long n64 = kind < 2 ? sum.sym[0] : sum.apply[0], n128 = kind < 2 ? sum.sym[1] : sum.apply[1];
+    double us64 = 1e30, us128 = 1e30;
+    const int l64 = n64 < 768 ? part_length(in, count, kind, 64, us64) : 0, l128 = n128 < 512 ? part_length(in, count, kind, 128, us128) : 0;
+    const bool wide = n64 >= 768 || us128 < us64;
+    bt[kind] = wide ? 128 : 64;
+    len[kind] = wide ? l128 : l64;
+    list[kind] = wide ? n128 : n64;
+  }
+  plan.bt_gram = bt[0];
+  plan.bt_square = bt[1];
+  plan.bt_apply = bt[2];
   long long blocks[kStages] = {};
   for (int k = 0; k < count; ++k) {
     const mr3d_matrix &g = in[k];
@@ -700,9 +706,9 @@ int plan_list(const mr3d_matrix *in, int count, char *base, Plan &plan, Mat *mat
       const long long tg = (p.m + plan.bt_gram - 1) / plan.bt_gram, ts = (p.m + plan.bt_square - 1) / plan.bt_square, tm = (p.m + plan.bt_apply - 1) / plan.bt_apply, tn = (p.n + plan.bt_apply - 1) / plan.bt_apply;
       const int ksm = (p.m + 31) / 32, ksn = (p.n + 31) / 32, qg = plan.bt_gram == 128 ? 4 : 1, qs = plan.bt_square == 128 ? 4 : 1, qa = plan.bt_apply == 128 ? 4 : 1;
       if (ts * (ts + 1) / 2 > 0x3fffffff || tg * (tg + 1) / 2 > 0x3fffffff || tm * tn > 0x3fffffff) return MR3D_ERR_UNSUPPORTED;
-      p.gram = split_for((int)(tg * (tg + 1) / 2), ksn, len_gram, list_gram, k == sum.carrier, plan.bt_gram);
-      p.square = split_for((int)(ts * (ts + 1) / 2), ksm, len_square, list_sym, k == sum.carrier, plan.bt_square);
-      p.apply = split_for((int)(tm * tn), ksm, len_apply, list_apply, k == sum.carrier, plan.bt_apply);
+      p.gram = split_for((int)(tg * (tg + 1) / 2), ksn, len[0], list[0], k == sum.carrier, plan.bt_gram);
+      p.square = split_for((int)(ts * (ts + 1) / 2), ksm, len[1], list[1], k == sum.carrier, plan.bt_square);
+      p.apply = split_for((int)(tm * tn), ksm, len[2], list[2], k == sum.carrier, plan.bt_apply);
       const long long numel = (long long)p.m * p.n;
       p.norm_blocks = (int)((numel + 8191) / 8192 > 1024 ? 1024 : (numel + 8191) / 8192);
       for (int b = 0; b < kBufs; ++b) {
