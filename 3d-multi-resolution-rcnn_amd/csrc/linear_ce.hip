@@ -52,9 +52,10 @@ struct Ce {
   int db_f32;
 };
 
-// four values at any element's alignment
+// four or eight values at any element's alignment
 typedef float vf4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef bf16 vb4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef bf16 vb8 __attribute__((ext_vector_type(8), aligned(2)));
 
 template <bool F32> __device__ __forceinline__ float elem(const char *p, long long i) {
   return F32 ? ((const float *)p)[i] : (float)((const bf16 *)p)[i];
@@ -184,18 +185,22 @@ template <bool F32> __device__ __forceinline__ void pack_row(const char *src, ch
     const float *s = (const float *)src;
     for (int k = threadIdx.x * 4; k < ld / 4; k += 1024) {
       _Float16 h[4], l[4];
+      float t[4];
+      if (k + 4 <= cols) *reinterpret_cast<vf4 *>(t) = *reinterpret_cast<const vf4 *>(s + k);
+      else
 #pragma unroll
-      for (int e = 0; e < 4; ++e) split16(k + e < cols ? s[k + e] * factor * scale : 0.f, h[e], l[e]);
+        for (int e = 0; e < 4; ++e) t[e] = k + e < cols ? s[k + e] : 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) split16(t[e] * factor * scale, h[e], l[e]);
       char *d = dst + (k >> 5) * 128 + (k & 31) * 2;
       *reinterpret_cast<uint2 *>(d) = *reinterpret_cast<uint2 *>(h);
       *reinterpret_cast<uint2 *>(d + 64) = *reinterpret_cast<uint2 *>(l);
     }
   } else {
     const bf16 *s = (const bf16 *)src;
-    const bool vec = (((uintptr_t)src) & 15) == 0;
     for (int k = threadIdx.x * 8; k < ld / 2; k += 2048) {
       bf16 t[8];
-      if (vec && k + 8 <= cols) *reinterpret_cast<uint4 *>(t) = *reinterpret_cast<const uint4 *>(s + k);
+      if (k + 8 <= cols) *reinterpret_cast<vb8 *>(t) = *reinterpret_cast<const vb8 *>(s + k);
       else
 #pragma unroll
         for (int e = 0; e < 8; ++e) t[e] = k + e < cols ? s[k + e] : (bf16)0.f;
