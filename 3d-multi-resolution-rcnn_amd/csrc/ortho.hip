@@ -16,7 +16,7 @@
 // cache line is unused), the error against 64 bits 1.12 times that of rounding the result: not taken.
 // MFMA-bound on large matrices; on small ones the dependent launches are what counts, hence the list and the small path.
 // Measured: 64 x 1728 70 us (A 9, the iteration 46: 17 products of 1.3 us of the double matrix pipe each and their barriers; Q G 12), 777 x 2311 and
-// 333 x 1301 287 us (15 products of 13 to 22 us), the 64 matrices of a detector (179 GFLOP) 0.96 ms, 4096 x 4096 bf16 3.8 to 3.9 ms (1.06 PFLOP/s of passes).
+// 333 x 1301 277 us (15 products of 13 to 22 us), the 64 matrices of a detector (179 GFLOP) 0.96 ms, 4096 x 4096 bf16 3.8 to 3.9 ms (1.06 PFLOP/s of passes).
 #include "gemm16.h"
 #include <new>
 
