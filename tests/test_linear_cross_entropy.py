@@ -316,6 +316,13 @@ def test_same_bits_every_run_on_another_stream_and_in_a_graph():
 
 
 @pytest.mark.gpu
+def test_large_tiles_over_parts_of_the_classes():
+    """dx of 6 x 8 large tiles, five parts of the classes each"""
+    x, w, b, label, rw = _inputs(1500, 2000, 5200, torch.bfloat16, seed=6)
+    _compare(x, w, b, label, rw, ())
+
+
+@pytest.mark.gpu
 def test_large_tiles_in_a_replayed_graph():
     from mr3d_amd.core import linear_cross_entropy
     x, w, _, label, rw = (None if t is None else t.cuda() for t in _inputs(3500, 64, 3600, torch.bfloat16, bias=False))
