@@ -5,10 +5,13 @@
 //   rows     live rows (weight not 0, label not ignored, row < valid_rows) are numbered; the others cost nothing further, take no part
 //            in any product (NaN in them stays there) and get a zero row of dx
 //   pack     live rows of x (and W, where its storage is not what the products read) into gemm16.h's operand form
-//   logits   z tile by tile; a wave holds 128 classes of a row: it leaves exp(z - max of the 128) and (max, sum).  The exponentials take the place
-//            of the logits: for bf16 in fp16 (in [0, 1]; 2^-12 of the value, an eighth of what g's rounding to bf16 loses), else fp32
-//   grad     per row: lse from the (max, sum) pairs, the label's logit once more as a dot product, loss; exponentials -> g in place
+//   logits   z tile by tile; a wave holds 128 classes of a row: it leaves exp(z - max of the 128) and (max, sum), the label's class left out: where a
+//            row is certain of its label, 1 - p of the label is a sum of small exponentials, not a difference.  The exponentials take the place
+//            of the logits: for bf16 in fp16 (in [0, 1]; 2^-11 of the value, an eighth of what g's rounding to bf16 loses), else fp32
+//   grad     per row: lse from the (max, sum) pairs and the label's logit, a dot product in double; loss; exponentials -> g in place
 //   dx, dw   g W (split over the classes, parts added in a fixed order) and g^T x
+// bf16: g is kept as t g', t = w (1 - p_label) / avg in fp32, so that the label's entry of g' is -1 and loses nothing to bf16 -- a rounding there would be
+// the same for the whole row of dx; dx rows take t at the end, dW takes bf16(t x) in the place of x, db multiplies.
 // The exponentials of at most kPiece bytes of rows exist at a time; dW accumulates over such pieces in fp32.
 // Measured, 8192 x 2048 x 131072 bf16 (7782 live rows): logits 3.9 ms (1.08 PFLOP/s, exponentials and their 2 GB of stores included), grad 0.93 (4.4 TB/s),
 // dx 3.5, dW 3.5 (1.2): the matrix pipe at the clock its power allows.  3001 x 515 x 20011 fp32 (2010 live): logits 167 us, grad 64, gradients 297,
@@ -38,7 +41,8 @@ struct Ce {
   // workspace
   int *head;                                                 // [0] live rows  [1] avg (float)  [2] max |W|  [3] max |x w| (float bits)
   int *index, *pos;                                          // live row -> row, row -> live row or -1
-  float *xmax;                                               // fp32: max |x| of a live row
+  int *label;                                                // of a live row; -1: outside the classes
+  float *xmax, *t;                                           // of a live row.  fp32: max |x|.  bf16: w (1 - p_label) / avg
   char *xp, *xwp, *wp;                                       // packed operands (wp may be the caller's W)
   long long ldx, ldw, ldg;                                   // bytes
   char *g;
@@ -97,7 +101,10 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(Ce c) {
       positive += wpos[k];
     }
     const int at = before + __popcll(bl & ((1ull << lane) - 1));
-    if (live) c.index[at] = r;
+    if (live) {
+      c.index[at] = r;
+      c.label[at] = c.labels[r] >= 0 && c.labels[r] < c.classes ? (int)c.labels[r] : -1;
+    }
     if (r < c.rows) c.pos[r] = live ? at : -1;
     __syncthreads();
   }
@@ -270,6 +277,14 @@ __global__ __launch_bounds__(T::THREADS, 2) void ce_logits_kernel(Ce c, int row0
         for (int e = 0; e < 4; ++e)
           if (iw + a * 16 + e >= c.classes) acc[a][b][e] = -INFINITY;
     }
+    const int own = (j < live ? c.label[row0 + j] : -1) - (ti * T::BI + wi * WI);
+    if (__any(own >= 0 && own < WI)) {
+#pragma unroll
+      for (int a = 0; a < T::TI; ++a)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (own == (lane >> 4) * 4 + a * 16 + e) acc[a][b][e] = -INFINITY;
+    }
     float m = -INFINITY;
 #pragma unroll
     for (int a = 0; a < T::TI; ++a)
@@ -349,7 +364,7 @@ __device__ __forceinline__ void block_sum(double &a, double &b, double (*lds)[4]
 
 // one live row: log-sum-exp, loss, and (TRAIN) the exponentials become g.  `wcols`: classes of a (max, sum) pair
 template <bool F32, bool TRAIN>
-__global__ __launch_bounds__(256) void ce_grad_kernel(Ce c, int row0, int wcols) {
+__global__ __launch_bounds__(256) void ce_grad_kernel(Ce c, int row0, int wcols, int want_dw) {
   __shared__ double lds[2][4];
   __shared__ float ldm[4];
   const int j = blockIdx.x;
@@ -357,10 +372,9 @@ __global__ __launch_bounds__(256) void ce_grad_kernel(Ce c, int row0, int wcols)
   const int r = c.index[row0 + j];
   const float2 *st = c.stats + (long long)j * c.pieces;
   // the label's logit first: its loads wait for row and label, the pairs' do not
-  const long long label = c.labels[r];
-  const bool known = label >= 0 && label < c.classes;        // else: the loss and this row's gradient are NaN
+  const int label = c.label[row0 + j];                       // -1: the loss and this row's gradient are NaN
   double dot = 0;
-  if (known) {
+  if (label >= 0) {
 #pragma unroll 4
     for (int k = threadIdx.x; k < c.hidden; k += 256)
       dot += (double)elem<F32>(c.x, r * c.x_stride + k) * (double)elem<F32>(c.w, label * c.w_stride + k);
@@ -378,14 +392,16 @@ __global__ __launch_bounds__(256) void ce_grad_kernel(Ce c, int row0, int wcols)
   double s = 0;
   for (int k = threadIdx.x; k < c.pieces; k += 256) s += (double)st[k].y * (double)__builtin_amdgcn_exp2f(st[k].x - ms);
   block_sum(s, dot, lds);
-  const double lse2 = known ? (double)m + log2(s) : (double)NAN, lse = lse2 * 0.69314718055994530942;
+  // the others' sum is s 2^m; with the label's 2^d: lse, 1 - p_label, and lse - z_label without a difference where that is small
+  const double d = label >= 0 ? dot * 1.44269504088896340736 : (double)NAN, top = fmax((double)m, d);
+  const double others = s * exp2((double)m - top), all = others + exp2(d - top), rest = others / all;
+  const double ce = ((double)m < d ? log1p(s * exp2((double)m - d)) : (top + log2(all)) * 0.69314718055994530942 - dot) + (all - all);   // NaN stays
   const float w = c.row_weight ? c.row_weight[r] : 1.f;
-  if (threadIdx.x == 0) c.row_loss[row0 + j] = (lse - dot) * (double)w;
+  if (threadIdx.x == 0) c.row_loss[row0 + j] = ce * (double)w;
   if constexpr (TRAIN) {
-    const float l = (float)lse2, avg = ((const float *)c.head)[1];
-    const float f = F32 ? kSG : w / avg;
-    const float at = (float)expm1(dot - lse);                // p - 1 of the label, without the cancellation
     char *row = c.g + j * c.ldg;
+    // exponentials relative to their pair's maximum -> p, times kSG (fp32); p / (1 - p_label) (bf16)
+    const float l = F32 ? (float)(top + log2(all)) : ms, f = F32 ? kSG : s > 0 ? (float)(1. / s) : (float)(s * 0.), at = F32 ? -(float)rest * kSG : -1.f;
     if constexpr (F32) {
       for (long long k = threadIdx.x * 4; k < c.ldg / 4; k += 1024) {
         float4 p = *reinterpret_cast<const float4 *>(row + k * 4);
@@ -393,7 +409,7 @@ __global__ __launch_bounds__(256) void ce_grad_kernel(Ce c, int row0, int wcols)
         float v[4] = {p.x * e, p.y * e, p.z * e, p.w * e};
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          if (k + q == label) v[q] = at * f;
+          if (k + q == label) v[q] = at;
         _Float16 hi[4], lo[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) split16(v[q], hi[q], lo[q]);
@@ -409,8 +425,20 @@ __global__ __launch_bounds__(256) void ce_grad_kernel(Ce c, int row0, int wcols)
         *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(row + k * 2);
         const float e = __builtin_amdgcn_exp2f(st[k / wcols].x - l) * f;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) t[q] = (bf16)(k + q == label ? at * f : (float)p[q] * e);
+        for (int q = 0; q < 8; ++q) t[q] = (bf16)(k + q == label ? at : (float)p[q] * e);
         *reinterpret_cast<uint4 *>(row + k * 2) = *reinterpret_cast<uint4 *>(t);
+      }
+      const float t = (float)(rest * (double)w / (double)((const float *)c.head)[1]);
+      if (threadIdx.x == 0) c.t[row0 + j] = t;
+      if (want_dw) {
+        const char *from = c.xp + (row0 + j) * c.ldx;
+        char *to = c.xwp + (row0 + j) * c.ldx;
+        for (long long k = threadIdx.x * 16; k < c.ldx; k += 4096) {
+          bf16x8 v = *reinterpret_cast<const bf16x8 *>(from + k);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) v[q] = (bf16)((float)v[q] * t);
+          *reinterpret_cast<bf16x8 *>(to + k) = v;
+        }
       }
     }
   }
@@ -451,7 +479,7 @@ template <bool F32> __device__ __forceinline__ void dx_row(const Ce &c, int row0
   const float avg = ((const float *)c.head)[1], rsw = F32 ? 1.f / scale_of(c, 2) : 1.f;
   const int p = c.pos[r];
   if (p >= 0 && (p < row0 || p >= row0 + live)) return;                       // another piece's row
-  const float f = F32 ? (c.row_weight ? c.row_weight[r] : 1.f) / avg * (rsw / kSG) : 1.f;
+  const float f = F32 ? (c.row_weight ? c.row_weight[r] : 1.f) / avg * (rsw / kSG) : p >= 0 ? c.t[p] : 0.f;
   for (int k = threadIdx.x * 4; k < c.hidden; k += 1024) {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (p >= 0) {
@@ -459,7 +487,7 @@ template <bool F32> __device__ __forceinline__ void dx_row(const Ce &c, int row0
         const float4 t = *reinterpret_cast<const float4 *>(c.part + ((long long)z * c.cap + p - row0) * hp + k);
         v.x += t.x; v.y += t.y; v.z += t.z; v.w += t.w;
       }
-      if constexpr (F32) { v.x *= f; v.y *= f; v.z *= f; v.w *= f; }
+      v.x *= f; v.y *= f; v.z *= f; v.w *= f;
     }
     const float o[4] = {v.x, v.y, v.z, v.w};
     const long long at = (long long)r * c.hidden + k;
@@ -486,7 +514,7 @@ template <class T> __device__ __forceinline__ void dw_tile(const Ce &c, int row0
   tile_of(bid, nti * ntj, nti, ntj, ti, tj);
   constexpr int E = T::SPLIT ? 4 : 2;
   f32x4 acc[T::TI][T::TJ];
-  const char *x = (T::SPLIT ? c.xwp : c.xp) + row0 * c.ldx;
+  const char *x = c.xwp + row0 * c.ldx;
   run<T>(lds, side_ks<T>(x, c.ldx, live, c.ldx, ti * T::BI * E, 0), side_ks<T>(c.g, c.ldg, live, c.ldg, (long long)tj * T::BJ * E, 0),
          (live + T::KK - 1) / T::KK, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave % T::NWI, wj = wave / T::NWI;
@@ -555,8 +583,9 @@ template <bool F32> __device__ __forceinline__ void db_part(const Ce &c, int row
         for (int e = 0; e < 8; ++e) s[e] += ((float)h[e] + (float)l[e]) * w;
       } else {
         const bf16x8 v = *reinterpret_cast<const bf16x8 *>(row + i * 2);
+        const float t = c.t[row0 + j];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] += (float)v[e];
+        for (int e = 0; e < 8; ++e) s[e] += (float)v[e] * t;
       }
     }
   }
@@ -665,7 +694,7 @@ int tile_for(bool f32, long long i, long long j, long long z) {
 long long up(long long v, long long a) { return (v + a - 1) / a * a; }
 
 struct Layout {
-  size_t bytes, head, index, pos, xmax, xp, xwp, wp, g, stats, part, row_loss, dwacc, dbpart;
+  size_t bytes, head, index, pos, label, xmax, xp, xwp, wp, g, stats, part, row_loss, dwacc, dbpart;
   long long ldx, ldw, ldg;
   int cap, chunks, pieces, z, wcols, db_slices;
   int bt_logits, bt_dx, bt_dw;
@@ -710,9 +739,10 @@ int layout_of(const mr3d_linear_ce *a, Layout &l) {
   l.index = take(at, (size_t)a->rows * 4);
   l.pos = take(at, (size_t)a->rows * 4);
   l.row_loss = take(at, (size_t)a->rows * 8);
+  l.label = take(at, (size_t)a->rows * 4);
   l.xmax = take(at, (size_t)a->rows * 4);
   l.xp = take(at, (size_t)(a->rows * l.ldx));
-  if (f32 && a->want_dweight) l.xwp = take(at, (size_t)(a->rows * l.ldx));
+  if (a->want_dweight) l.xwp = take(at, (size_t)(a->rows * l.ldx));
   if (l.pack_w) l.wp = take(at, (size_t)(a->classes * l.ldx));
   l.stats = take(at, (size_t)cap * l.pieces * 8);
   if (train) l.g = take(at, (size_t)(cap * l.ldg));
@@ -794,10 +824,10 @@ template <bool F32> int run_ce(const mr3d_linear_ce *a, const Layout &l, Ce &c, 
     int e = MR3D_OK;
     if (train) {
       e = pick<TL>(l.bt_logits, [&](auto t) { return launch_logits<decltype(t), true>(c, row0, q); });
-      ce_grad_kernel<F32, true><<<l.cap, 256, 0, q>>>(c, row0, l.wcols);
+      ce_grad_kernel<F32, true><<<l.cap, 256, 0, q>>>(c, row0, l.wcols, a->want_dweight);
     } else {
       e = pick<TL>(l.bt_logits, [&](auto t) { return launch_logits<decltype(t), false>(c, row0, q); });
-      ce_grad_kernel<F32, false><<<l.cap, 256, 0, q>>>(c, row0, l.wcols);
+      ce_grad_kernel<F32, false><<<l.cap, 256, 0, q>>>(c, row0, l.wcols, a->want_dweight);
     }
     if (e) return e;
     const int mode = k ? 2 : (l.chunks > 1 ? 1 : 0);
@@ -845,7 +875,8 @@ extern "C" int mr3d_linear_cross_entropy(const mr3d_linear_ce *a, void *workspac
   c.rows = a->rows; c.hidden = a->hidden; c.classes = a->classes;
   c.bias_f32 = c.db_f32 = a->param_dtype == MR3D_DTYPE_F32;
   c.head = (int *)(b + l.head); c.index = (int *)(b + l.index); c.pos = (int *)(b + l.pos);
-  c.xmax = (float *)(b + l.xmax);
+  c.label = (int *)(b + l.label);
+  c.xmax = c.t = (float *)(b + l.xmax);
   c.xp = b + l.xp; c.xwp = b + l.xwp;
   c.wp = l.pack_w ? b + l.wp : (char *)const_cast<void *>(a->weight);
   c.ldx = l.ldx; c.ldw = l.ldw; c.ldg = l.ldg;

@@ -9,8 +9,8 @@ Tolerances, norm-wise per row or matrix.  u = 2^-24.
            largest Z.  Exponential and sums: 2^-20 relative in all (the hardware exponential is good to a few u; sums are short).
   loss     |d ce_i| <= 2 Z + 2^-20, and the weighted mean over rows; stored in fp32.
   g        relative to softmax: E = 2 Z + 2^-19; the label's entry is computed apart, absolute error E.  fp32: two planes of 14 + 22 bits
-           (2^-21 of the value and 2^-38 absolute); bf16: 2^-8 for the stored exponential and 2^-8 for g.
-           So |dg_i| <= (E + r) |g_i| + E p_label w with r = 2^-20 (fp32), 2^-7 (bf16), taken entry by entry below.
+           (2^-21 of the value and 2^-38 absolute); bf16: 2^-11 for the stored exponential, 2^-8 for g and, in dW, 2^-8 for t x.
+           So |dg_i| <= (E + r) |g_i| + E p_label w with r = 2^-20 (fp32), 2^-7 + 2^-10 (bf16), taken entry by entry below.
   dx, dW   the error of g through |W| and |x|, entry by entry, plus the product's own error (n its length) on sum |g| |W|, plus
            half a step of the stored type."""
 import pytest
@@ -44,7 +44,7 @@ def _reference(x, w, b, label, rw, ignore=-100, valid=None, avg=None):
     prod = lambda m: 2.0 ** -21 + (204 + m / 128) * U if f32 else (17 * (m // 32 + 1)) * U
     zerr = prod(k) * xl.norm(dim=1, keepdim=True) * w.norm(dim=1).max() + 2 * U * z.abs().amax(1, keepdim=True)
     e = 2 * zerr + 2.0 ** -19
-    eg = (e + (2.0 ** -20 if f32 else 2.0 ** -7)) * g.abs() + (2.0 ** -36 if f32 else 0)
+    eg = (e + (2.0 ** -20 if f32 else 2.0 ** -7 + 2.0 ** -10)) * g.abs() + (2.0 ** -36 if f32 else 0)
     eg[at, ll] += e.squeeze(1) * torch.ones(len(rows))
     g, eg = g * s, eg * s.abs()
     dx, ex = torch.zeros_like(x), torch.zeros_like(x)
@@ -402,6 +402,44 @@ def test_classes_masked_by_the_bias(dtype, low):
     assert not dw[~keep].any() and not db[~keep].any()
     for name, t in zip(('loss', 'dx', 'dw', 'db'), (loss, dx, dw[keep], db[keep])):
         _check(t, ref[name], bound[name], (name,))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('margin', [8.0, 14.0, 25.0])
+def test_rows_certain_of_their_label(dtype, margin):
+    """every row gives its label all but about exp(-margin): gradients as small as that, right relative to themselves.  1 - p_label is a sum over the others
+    (relative error E), g of an other class is relative to that sum (bf16) or has two planes that end at 2^-38 (fp32: 2^-38 / exp(-25) is lost: margin
+    25 is for bf16 and the loss)."""
+    n, v = 60, 300
+    g = torch.Generator().manual_seed(1)
+    w = (0.3 * torch.randn(v, v, generator=g)).to(dtype)
+    label = torch.arange(n) * 5 % v
+    x = torch.zeros(n, v)
+    for i in range(n):                                       # x_i = a e_label: z = a W[:, label], the label's entry of W lifted
+        x[i, label[i]] = 1.0
+    w[torch.arange(v), torch.arange(v)] = (margin + 6.0)
+    x, rw = x.to(dtype), 0.25 + torch.rand(n, generator=g)
+    leaves = [x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)]
+    from mr3d_amd.core import linear_cross_entropy
+    loss = linear_cross_entropy(leaves[0], leaves[1], label.cuda(), rw.cuda())
+    dx, dw = (t.double().cpu() for t in torch.autograd.grad(loss, leaves))
+    z = x.double() @ w.double().t()
+    at = torch.arange(n)
+    others = z.masked_fill(torch.nn.functional.one_hot(label, v).bool(), float('-inf'))
+    so = torch.logsumexp(others, 1)
+    ce = torch.log1p(torch.exp(so - z[at, label]))
+    rest = torch.exp(so - torch.logaddexp(so, z[at, label]))
+    p = torch.softmax(others, 1) * rest[:, None]
+    p[at, label] = -rest
+    gg = p * rw.double()[:, None] / n
+    want = float((ce * rw.double()).sum() / n)
+    assert abs(float(loss) - want) <= 1e-5 * want
+    if dtype == torch.float32 and margin > 20:
+        return
+    rel = 1e-4 if dtype == torch.float32 else 2.0 ** -6     # fp32: E = 1e-5 and 2^-38 of exp(-14), over 300 entries; bf16: 3 roundings of 2^-8
+    for got, ref in ((dx, gg @ w.double()), (dw, gg.t() @ x.double())):
+        assert float((got - ref).norm()) <= rel * float(ref.norm())
 
 
 @pytest.mark.gpu
