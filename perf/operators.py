@@ -188,19 +188,18 @@ def run(state):
     if not own:
         with torch.no_grad():
             return {'norm': _plain_norm, 'ce': _plain_ce, 'ortho': _plain_ortho}[op](state)
+    from mr3d_amd.core import linear_cross_entropy, orthogonalize
+    from mr3d_amd.detector.layers import layer_norm
     if op == 'ortho':
-        from mr3d_amd.core import orthogonalize
         return orthogonalize(state['mats'], steps=STEPS, coefficients=COEFFICIENTS, eps=NS_EPS)
     train = state['case']['train']
     x, w, b = state['x'], state['w'], state['b']
     leaves = [t for t in (x, w, b) if t is not None]
     if op == 'norm':
-        from mr3d_amd.detector.layers import layer_norm
         y = layer_norm(x, w, b, eps=LN_EPS)
         out = {'y': y.detach()}
         grads = torch.autograd.grad(y, leaves, state['dy']) if train else ()
     else:
-        from mr3d_amd.core import linear_cross_entropy
         loss = linear_cross_entropy(x, w, state['label'], state['row_weight'], bias=b, ignore_index=IGNORE)
         out = {'loss': loss.detach()}
         grads = torch.autograd.grad(loss, leaves) if train else ()
