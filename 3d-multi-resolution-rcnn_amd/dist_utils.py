@@ -355,17 +355,19 @@ class ArenaMuon(ArenaSGD):
         from .core.orthogonalize import orthogonalize
         g = self.param_groups[0]
         p, grad, buf, d = self.arena.flat_params, self.arena.flat_grads, self.momentum_buffer, self._d
+        mask = self._active_mask()
+        if mask is not None:
+            grad = torch.mul(grad, mask, out=d)                     # a never-touched slice: its momentum stays zero, whatever lies in its gradient
         buf.mul_(g['momentum']).add_(grad)
         torch.add(grad, buf, alpha=g['momentum'], out=d)
         orthogonalize(self._mats, steps=self.steps, out=self._mats)
-        mask = self._active_mask()
         if g['weight_decay'] != 0:
             if mask is None:
                 p.mul_(1 - g['lr'] * g['weight_decay'])
             else:
                 p.addcmul_(p, mask, value=-g['lr'] * g['weight_decay'])
         if mask is not None:
-            d.mul_(mask)                                            # never touched: a zero gradient, but also after a foreign write to it
+            d.mul_(mask)                                            # momentum restored from a checkpoint waits for the first gradient too
         p.addcmul_(d, self._gain, value=-g['lr'])
 
 
