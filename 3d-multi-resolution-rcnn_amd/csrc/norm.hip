@@ -124,7 +124,15 @@ __global__ __launch_bounds__(threads_of<LPR>()) void ln_fwd_kernel(const T *__re
 #pragma unroll
     for (int e = 0; e < N; ++e) s[0] += f[e];
     row_sum<LPR, 1>(s, lds);
-    const float mean = s[0] * inv;
+    // the mean of what the first mean leaves takes out its error of some steps, which a small variance would show: a row of one value has variance 0.
+    // (A quotient, because a product would be fused with the differences below, which would then be taken from another number than `mean`)
+    float mean = s[0] / (float)cols, left[1] = {0.f};
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int e = 0; e < Vec<T>::N; ++e) left[0] += (v * LPR + lane) * Vec<T>::N + e < cols ? f[v * Vec<T>::N + e] - mean : 0.f;
+    row_sum<LPR, 1>(left, lds);
+    mean += left[0] * inv;
     float q[1] = {0.f};
 #pragma unroll
     for (int v = 0; v < NV; ++v)
