@@ -127,7 +127,13 @@ at::Tensor layer_norm(const at::Tensor &x, const std::optional<at::Tensor> &weig
 }
 
 // ------------------------------------------------------------------------------------------------ linear cross entropy
-at::Tensor packed_rows(const at::Tensor &t) { return t.stride(1) == 1 && t.stride(0) >= t.size(1) ? t : t.contiguous(); }
+// [rows, cols] as the kernels read it.  Strides of axes of one element say nothing (contiguous() lets them be): they are set to the packed ones
+at::Tensor packed_rows(const at::Tensor &t) {
+  const int64_t rows = t.size(0), cols = t.size(1);
+  const int64_t r = rows > 1 ? t.stride(0) : cols, c = cols > 1 ? t.stride(1) : 1;
+  if (c != 1 || r < cols) return t.contiguous();
+  return r == t.stride(0) && c == t.stride(1) ? t : t.as_strided({rows, cols}, {r, c});
+}
 
 struct CeArgs {
   at::Tensor label, row_weight, avg, valid;
