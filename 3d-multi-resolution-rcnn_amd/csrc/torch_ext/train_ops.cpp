@@ -4,6 +4,7 @@
 #include "common.h"
 
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
 #include <vector>
@@ -24,6 +25,21 @@ at::Tensor workspace(size_t bytes, const at::Tensor &like, size_t align, void **
   const uintptr_t a = (uintptr_t)ws.data_ptr();
   *p = (void *)((a + align - 1) / align * align);
   return ws;
+}
+
+// The operators read memory, and autograd's reverse mode is all that they take part in: a forward-mode tangent would be lost, a trace would record the
+// empty result and not the kernel, function transforms hand in wrappers, and a negated view keeps its sign outside of its memory
+void check_plain(const char *what, const std::vector<at::Tensor> &tensors) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), what, " cannot be traced (torch.jit.trace)");
+  static const c10::DispatchKeySet wrappers({c10::DispatchKey::Batched, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Functionalize,
+                                             c10::DispatchKey::Python});
+  for (const at::Tensor &t : tensors) {
+    if (!t.defined()) continue;
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.key_set().has_any(wrappers), what, " has no function transforms (torch.func, vmap, fake tensors)");
+    TORCH_CHECK_NOT_IMPLEMENTED(t.layout() == at::kStrided, what, " takes dense tensors, got ", t.layout());
+    TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), what, " has no forward-mode derivative");
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.is_neg(), what, " does not read a negated view: resolve_neg() first");
+  }
 }
 
 // The nodes below give first derivatives.  A graph through their gradients (create_graph) gets a node that says so when it is used
@@ -74,6 +90,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   }
 
   static variable_list backward(AutogradContext *ctx, variable_list g) {
+    check_plain("layer_norm's backward", g);
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &x = saved[0], &w = saved[1], &stats = saved[2];
     const int64_t want = ctx->saved_data["want"].toInt(), cols = x.size(-1);
@@ -107,6 +124,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 };
 
 at::Tensor layer_norm(const at::Tensor &x, const std::optional<at::Tensor> &weight, const std::optional<at::Tensor> &bias, double eps) {
+  check_plain("layer_norm", {x, or_none(weight), or_none(bias)});
   TORCH_CHECK_VALUE(x.dim() >= 1, "layer_norm: x is a tensor [..., C]");
   TORCH_CHECK_TYPE(stored(x), "layer_norm: x is float32 or bfloat16, got ", x.scalar_type());
   const int64_t cols = x.size(-1);
@@ -193,6 +211,7 @@ struct LinearCe : torch::autograd::Function<LinearCe> {
   }
 
   static variable_list backward(AutogradContext *ctx, variable_list g) {
+    check_plain("linear_cross_entropy's backward", g);
     TORCH_CHECK(!ctx->saved_data.count("used"), "linear_cross_entropy: a second backward through the same loss (its gradients were handed over by the "
                                                 "first); call linear_cross_entropy again");
     TORCH_CHECK(ctx->saved_data["captured"].toBool() == capturing(g[0]),
@@ -223,6 +242,7 @@ struct LinearCe : torch::autograd::Function<LinearCe> {
 at::Tensor linear_cross_entropy(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &label, const std::optional<at::Tensor> &row_weight,
                                 const std::optional<at::Tensor> &bias, const std::optional<at::Tensor> &avg_dev, std::optional<double> avg_host,
                                 const std::optional<at::Tensor> &valid_rows, int64_t ignore_index) {
+  check_plain("linear_cross_entropy", {x, weight, label, or_none(row_weight), or_none(bias), or_none(avg_dev), or_none(valid_rows)});
 #define CE "linear_cross_entropy: "
   TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && weight.size(1) == x.size(-1), CE "x is [..., K] and weight [C, K], got ", x.sizes(), " and ", weight.sizes());
   TORCH_CHECK_TYPE(stored(x) && weight.scalar_type() == x.scalar_type(), CE "x and weight are both float32 or both bfloat16, got ", x.scalar_type(), " and ",
@@ -262,6 +282,8 @@ at::Tensor linear_cross_entropy(const at::Tensor &x, const at::Tensor &weight, c
 // ------------------------------------------------------------------------------------------------ orthogonalised updates
 std::vector<at::Tensor> orthogonalize(const std::vector<at::Tensor> &mats, int64_t steps, double a, double b, double c, double eps,
                                       const std::optional<std::vector<at::Tensor>> &out) {
+  check_plain("orthogonalize", mats);
+  if (out) check_plain("orthogonalize", *out);
   at::AutoGradMode off(false);
   std::vector<at::Tensor> flat, outs;
   for (const at::Tensor &t : mats) {
