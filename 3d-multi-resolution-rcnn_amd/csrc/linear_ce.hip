@@ -7,7 +7,7 @@
 //   pack     live rows of x (and W, where its storage is not what the products read) into gemm16.h's operand form
 //   logits   z tile by tile; a wave holds 128 classes of a row: it leaves exp(z - max of the 128) and (max, sum), the label's class left out: where a
 //            row is certain of its label, 1 - p of the label is a sum of small exponentials, not a difference.  The exponentials take the place
-//            of the logits: for bf16 in fp16 (in [0, 1]; 2^-11 of the value, an eighth of what g's rounding to bf16 loses), else fp32
+//            of the logits: fp32, or for bf16 16 bits of that (pack_exp: 2^-10 of the value, a quarter of what g's rounding to bf16 loses)
 //   grad     per row: lse from the (max, sum) pairs and the label's logit, a dot product in double; loss; exponentials -> g in place
 //   dx, dw   g W (split over the classes, parts added in a fixed order) and g^T x
 // bf16: g is kept as t g', t = w (1 - p_label) / avg in fp32, so that the label's entry of g' is -1 and loses nothing to bf16 -- a rounding there would be
@@ -64,6 +64,14 @@ typedef bf16 vb8 __attribute__((ext_vector_type(8), aligned(2)));
 template <bool F32> __device__ __forceinline__ float elem(const char *p, long long i) {
   return F32 ? ((const float *)p)[i] : (float)((const bf16 *)p)[i];
 }
+
+// Two exponentials in [0, 1] as 16 bits each: of an fp32 value the sign and the upper bit of the exponent are 0 there, the next 16 bits are kept
+// (rounded).  2^-10 of the value over fp32's whole range down to 2^-126: fp16 would have 2^-11, but only above 2^-14 of the largest of the 128
+// classes, and nothing below 2^-25, where g in bf16 still has its 8 bits
+__device__ __forceinline__ unsigned pack_exp(float a, float b) {
+  return (__float_as_uint(a) + 0x2000u) >> 14 | ((__float_as_uint(b) + 0x2000u) << 2 & 0xffff0000u);
+}
+__device__ __forceinline__ float unpack_exp(unsigned short v) { return __uint_as_float((unsigned)v << 14); }
 
 // largest power of two that keeps |v| <= max below 2^14
 __device__ __forceinline__ float scale_for(float max) {
@@ -317,10 +325,8 @@ __global__ __launch_bounds__(T::THREADS, 2) void ce_logits_kernel(Ce c, int row0
 #pragma unroll
       for (int a = 0; a < T::TI; ++a) {
         const int u = ((wi * WI + a * 16) >> 3) + (lane >> 5);
-        _Float16 t[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) t[e] = (_Float16)acc[a][b][e];
-        *reinterpret_cast<uint2 *>(lds + jl * (T::BI * 2) + ((u ^ (jl & (T::BI / 8 - 1))) << 4) + ((lane >> 4) & 1) * 8) = *reinterpret_cast<uint2 *>(t);
+        *reinterpret_cast<uint2 *>(lds + jl * (T::BI * 2) + ((u ^ (jl & (T::BI / 8 - 1))) << 4) + ((lane >> 4) & 1) * 8) =
+            make_uint2(pack_exp(acc[a][b][0], acc[a][b][1]), pack_exp(acc[a][b][2], acc[a][b][3]));
       }
     }
   }
@@ -420,12 +426,12 @@ __global__ __launch_bounds__(256) void ce_grad_kernel(Ce c, int row0, int wcols,
       }
     } else {
       for (long long k = threadIdx.x * 8; k < c.ldg / 2; k += 2048) {
-        _Float16 p[8];
+        unsigned short p[8];
         bf16 t[8];
         *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(row + k * 2);
         const float e = __builtin_amdgcn_exp2f(st[k / wcols].x - l) * f;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) t[q] = (bf16)(k + q == label ? at : (float)p[q] * e);
+        for (int q = 0; q < 8; ++q) t[q] = (bf16)(k + q == label ? at : unpack_exp(p[q]) * e);
         *reinterpret_cast<uint4 *>(row + k * 2) = *reinterpret_cast<uint4 *>(t);
       }
       const float t = (float)(rest * (double)w / (double)((const float *)c.head)[1]);
