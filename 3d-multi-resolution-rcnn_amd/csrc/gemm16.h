@@ -147,8 +147,15 @@ __device__ __forceinline__ f32x4 mfma(i16x8 a, i16x8 b, f32x4 c) {
 // last k-step are issued with an empty range (zeros into a tile nobody reads), so that the count of outstanding loads is the same in every step.
 // A wave keeps the J fragments of the current 32 k and the next in registers and passes its I fragments by, AHEAD of them read in advance,
 // across the barrier of a k-step too; the reads go between the products (a wave that queues LDS reads issues nothing else).
-template <class T>
-__device__ __forceinline__ void run(char *lds, Side si, Side sj, int nsteps, f32x4 (&acc)[T::TI][T::TJ]) {
+//
+// `weight(part, b)`: a tile that restarts its accumulators may weight what each part (RESTART k-steps) adds to the sums of this lane's j of block b
+struct Unweighted {
+  __device__ float operator()(int, int) const { return 1.f; }
+};
+template <class T, class W = Unweighted>
+__device__ __forceinline__ void run(char *lds, Side si, Side sj, int nsteps, f32x4 (&acc)[T::TI][T::TJ], W weight = W()) {
+  constexpr bool WEIGHTED = !__is_same(W, Unweighted);
+  static_assert(!WEIGHTED || T::RESTART, "");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave % T::NWI, wj = wave / T::NWI;
   unsigned oi[T::NLI], oj[T::NLJ];
@@ -250,21 +257,25 @@ __device__ __forceinline__ void run(char *lds, Side si, Side sj, int nsteps, f32
       if constexpr (T::RESTART) {
         if ((s0 + u + 1) % T::RESTART == 0) {
 #pragma unroll
-          for (int a = 0; a < T::TI; ++a)
+          for (int b = 0; b < T::TJ; ++b) {
+            const float f = weight((s0 + u) / T::RESTART, b);
 #pragma unroll
-            for (int b = 0; b < T::TJ; ++b) {
-              sum[a][b] += acc[a][b];
+            for (int a = 0; a < T::TI; ++a) {
+              sum[a][b] += WEIGHTED ? acc[a][b] * f : acc[a][b];
               acc[a][b] = zero;
             }
+          }
         }
       }
     }
   }
   if constexpr (T::RESTART) {
 #pragma unroll
-    for (int a = 0; a < T::TI; ++a)
+    for (int b = 0; b < T::TJ; ++b) {
+      const float f = WEIGHTED && nsteps % T::RESTART ? weight(nsteps / T::RESTART, b) : 1.f;      // no such part: acc is zero
 #pragma unroll
-      for (int b = 0; b < T::TJ; ++b) acc[a][b] += sum[a][b];
+      for (int a = 0; a < T::TI; ++a) acc[a][b] = (WEIGHTED ? acc[a][b] * f : acc[a][b]) + sum[a][b];
+    }
   }
   // the fragments read last belong to no k-step; the loads of empty ranges must not land in what LDS holds next
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");

@@ -8,14 +8,15 @@
 //   logits   z tile by tile; a wave holds 128 classes of a row: it leaves exp(z - max of the 128) and (max, sum), the label's class left out: where a
 //            row is certain of its label, 1 - p of the label is a sum of small exponentials, not a difference.  The exponentials take the place
 //            of the logits: fp32, or for bf16 16 bits of that (pack_exp: 2^-10 of the value, a quarter of what g's rounding to bf16 loses)
-//   grad     per row: lse from the (max, sum) pairs and the label's logit, a dot product in double; loss; exponentials -> g in place
+//   grad     per row: lse from the (max, sum) pairs and the label's logit, a dot product in double; loss; exponentials -> g
 //   dx, dw   g W (split over the classes, parts added in a fixed order) and g^T x
-// bf16: g is kept as t g', t = w (1 - p_label) / avg in fp32, so that the label's entry of g' is -1 and loses nothing to bf16 -- a rounding there would be
-// the same for the whole row of dx; dx rows take t at the end, dW takes bf16(t x) in the place of x, db multiplies.
+// g is kept as t g', t = w (1 - p_label) / avg in fp32: a row certain of its label has gradients as exact as the others, and dx rows take t at the end.
+// bf16: the label's entry of g' is -1 and loses nothing to bf16 -- a rounding there would be the same for the whole row of dx; dW takes bf16(t x) in the
+// place of x, db multiplies.  fp32: dW's factor is t g' with a scale per class and 128 rows (ce_slab_kernel).
 // The exponentials of at most kPiece bytes of rows exist at a time; dW accumulates over such pieces in fp32.
 // Measured, 8192 x 2048 x 131072 bf16 (7782 live rows): logits 3.9 ms (1.08 PFLOP/s, exponentials and their 2 GB of stores included), grad 0.93 (4.4 TB/s),
-// dx 3.5, dW 3.5 (1.2): the matrix pipe at the clock its power allows.  3001 x 515 x 20011 fp32 (2010 live): logits 167 us, grad 64, gradients 297,
-// packing 40.  512 x 1024 x 1204 fp32: eight launches, 59 us in all.  One row, 1024 x 32768 bf16: logits 16 us (W at 4.2 TB/s), 10 in four small launches.
+// dx 3.5, dW 3.5 (1.2): the matrix pipe at the clock its power allows.  3001 x 515 x 20011 fp32 (2010 live): logits 162 us, losses 12, g 105, gradients
+// 305, packing 34.  512 x 1024 x 1204 fp32: nine launches, 64 us in all.  One row, 1024 x 32768 bf16: logits 16 us (W at 4.2 TB/s), 10 in four small launches.
 // Recomputing z for the gradient instead (no such buffer at all) costs 2 R V K more: 1.7 ps a logit at 1024 features against 0.8 ps for the
 // buffer's extra trip through memory.
 #include "gemm16.h"
@@ -26,9 +27,11 @@ namespace {
 
 typedef __bf16 bf16;
 constexpr float kLog2e = 1.44269504f;
-constexpr float kSG = 16384.f;                               // fp32: g without its weight, in [-1, 1], times this
+constexpr float kSG = 16384.f;                               // fp32: g of a row relative to 1 - p_label, in [-1, 1], times this
 constexpr long long kPiece = 1ll << 31;
 constexpr int kStatCols = 128;                               // classes per (max, sum) pair
+constexpr int kSlabRows = 128, kSlabCols = 64;               // fp32: what a workgroup turns into g; a class has a scale per kSlabRows rows
+constexpr int kScaleRows = 8192;                             // fp32: rows of dW in one launch, whose classes' scales lie in LDS (8 KB)
 
 struct Ce {
   const char *x, *w, *bias;
@@ -43,9 +46,11 @@ struct Ce {
   int *index, *pos;                                          // live row -> row, row -> live row or -1
   int *label;                                                // of a live row; -1: outside the classes
   float *xmax, *t;                                           // of a live row.  fp32: max |x|.  bf16: w (1 - p_label) / avg
+  float4 *row;                                               // of a live row, fp32: maximum, 1 / sum of the others, w (1 - p_label) / avg, scale of all x / of this
   char *xp, *xwp, *wp;                                       // packed operands (wp may be the caller's W)
   long long ldx, ldw, ldg;                                   // bytes
-  char *g;
+  char *g, *gx;                                              // exponentials, then g (fp32: for dW); fp32: g for dx
+  signed char *ge;                                           // fp32: exponent of a class's scale for dW, [slab][classes]
   float2 *stats;
   float *part;
   double *row_loss;
@@ -77,7 +82,7 @@ __device__ __forceinline__ float unpack_exp(unsigned short v) { return __uint_as
 __device__ __forceinline__ float scale_for(float max) {
   if (!(max > 0.f) || !(max < 3.0e38f)) return 1.f;
   int e = 14 - (ilogbf(max) + 1);
-  e = e > 120 ? 120 : e;
+  e = e > 100 ? 100 : e;
   return ldexpf(1.f, e);
 }
 __device__ __forceinline__ float scale_of(const Ce &c, int slot) { return scale_for(__int_as_float(c.head[slot])); }
@@ -150,7 +155,7 @@ __device__ __forceinline__ void rows_max(const float *const (&p)[kMaxRows], int 
     for (int r = 0; r < kMaxRows; ++r) m[r] = fmaxf(m[r], fabsf(p[r][k]));
 }
 
-// fp32: the largest |x| of each live row and |x w| of all, the largest |W|; four rows a wave, the first `xblocks` workgroups take x, the rest W.
+// fp32: the largest |x| of each live row and of all, the largest |W|; four rows a wave, the first `xblocks` workgroups take x, the rest W.
 // The maximum of positive floats is the maximum of their bits: an integer atomic, whose order does not matter -- one per workgroup, because
 // a thousand of them on one address take 15 us
 __global__ __launch_bounds__(256) void ce_max_kernel(Ce c, int xblocks, int wblocks) {
@@ -162,12 +167,8 @@ __global__ __launch_bounds__(256) void ce_max_kernel(Ce c, int xblocks, int wblo
   if (is_x) {
     const int live = c.head[0];
     for (int j = (blockIdx.x * 4 + wave) * kMaxRows; j < live; j += xblocks * 4 * kMaxRows) {
-      int row[kMaxRows];
 #pragma unroll
-      for (int r = 0; r < kMaxRows; ++r) {
-        row[r] = c.index[j + r < live ? j + r : j];
-        p[r] = (const float *)c.x + row[r] * c.x_stride;
-      }
+      for (int r = 0; r < kMaxRows; ++r) p[r] = (const float *)c.x + c.index[j + r < live ? j + r : j] * c.x_stride;
       rows_max(p, c.hidden, v);
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1)
@@ -177,8 +178,7 @@ __global__ __launch_bounds__(256) void ce_max_kernel(Ce c, int xblocks, int wblo
       for (int r = 0; r < kMaxRows; ++r) {
         if (j + r >= live) break;
         if ((threadIdx.x & 63) == 0) c.xmax[j + r] = v[r];
-        const float w = v[r] * fabsf(c.row_weight ? c.row_weight[row[r]] : 1.f);
-        m = fmaxf(m, w < 3.0e38f ? w : INFINITY);           // a NaN weight counts as infinite: the scale falls back to 1
+        m = fmaxf(m, v[r]);
       }
     }
   } else {
@@ -195,7 +195,7 @@ __global__ __launch_bounds__(256) void ce_max_kernel(Ce c, int xblocks, int wblo
 }
 
 // one stored row of an operand: bf16 copied, fp32 split; zeros behind the last column
-template <bool F32> __device__ __forceinline__ void pack_row(const char *src, char *dst, long long ld, int cols, float scale, float factor) {
+template <bool F32> __device__ __forceinline__ void pack_row(const char *src, char *dst, long long ld, int cols, float scale) {
   if constexpr (F32) {
     const float *s = (const float *)src;
     for (int k = threadIdx.x * 4; k < ld / 4; k += 1024) {
@@ -206,7 +206,7 @@ template <bool F32> __device__ __forceinline__ void pack_row(const char *src, ch
 #pragma unroll
         for (int e = 0; e < 4; ++e) t[e] = k + e < cols ? s[k + e] : 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) split16(t[e] * factor * scale, h[e], l[e]);
+      for (int e = 0; e < 4; ++e) split16(t[e] * scale, h[e], l[e]);
       char *d = dst + (k >> 5) * 128 + (k & 31) * 2;
       *reinterpret_cast<uint2 *>(d) = *reinterpret_cast<uint2 *>(h);
       *reinterpret_cast<uint2 *>(d + 64) = *reinterpret_cast<uint2 *>(l);
@@ -225,17 +225,16 @@ template <bool F32> __device__ __forceinline__ void pack_row(const char *src, ch
 }
 
 template <bool F32>
-__global__ __launch_bounds__(256) void ce_pack_kernel(Ce c, int want_xw) {
+__global__ __launch_bounds__(256) void ce_pack_kernel(Ce c) {
   const int b = blockIdx.x;
   if (b < c.rows) {
     if (b >= c.head[0]) return;
     const int r = c.index[b];
     const char *src = c.x + r * c.x_stride * (F32 ? 4 : 2);
-    pack_row<F32>(src, c.xp + b * c.ldx, c.ldx, c.hidden, F32 ? scale_for(c.xmax[b]) : 1.f, 1.f);
-    if (F32 && want_xw) pack_row<F32>(src, c.xwp + b * c.ldx, c.ldx, c.hidden, scale_of(c, 3), c.row_weight ? c.row_weight[r] : 1.f);
+    pack_row<F32>(src, c.xp + b * c.ldx, c.ldx, c.hidden, F32 ? scale_for(c.xmax[b]) : 1.f);
   } else {
     const int v = b - c.rows;
-    pack_row<F32>(c.w + v * c.w_stride * (F32 ? 4 : 2), c.wp + v * c.ldw, c.ldw, c.hidden, F32 ? scale_of(c, 2) : 1.f, 1.f);
+    pack_row<F32>(c.w + v * c.w_stride * (F32 ? 4 : 2), c.wp + v * c.ldw, c.ldw, c.hidden, F32 ? scale_of(c, 2) : 1.f);
   }
 }
 
@@ -368,7 +367,7 @@ __device__ __forceinline__ void block_sum(double &a, double &b, double (*lds)[4]
   b = lds[1][0] + lds[1][1] + lds[1][2] + lds[1][3];
 }
 
-// one live row: log-sum-exp, loss, and (TRAIN) the exponentials become g.  `wcols`: classes of a (max, sum) pair
+// one live row: log-sum-exp, loss, and (TRAIN) the exponentials become g (fp32: what ce_slab_kernel needs for it).  `wcols`: classes of a (max, sum) pair
 template <bool F32, bool TRAIN>
 __global__ __launch_bounds__(256) void ce_grad_kernel(Ce c, int row0, int wcols, int want_dw) {
   __shared__ double lds[2][4];
@@ -405,36 +404,21 @@ __global__ __launch_bounds__(256) void ce_grad_kernel(Ce c, int row0, int wcols,
   const float w = c.row_weight ? c.row_weight[r] : 1.f;
   if (threadIdx.x == 0) c.row_loss[row0 + j] = ce * (double)w;
   if constexpr (TRAIN) {
-    char *row = c.g + j * c.ldg;
-    // exponentials relative to their pair's maximum -> p, times kSG (fp32); p / (1 - p_label) (bf16)
-    const float l = F32 ? (float)(top + log2(all)) : ms, f = F32 ? kSG : s > 0 ? (float)(1. / s) : (float)(s * 0.), at = F32 ? -(float)rest * kSG : -1.f;
+    // exponentials relative to their pair's maximum -> p / (1 - p_label)
+    const float f = s > 0 ? (float)(1. / s) : (float)(s * 0.), t = (float)(rest * (double)w / (double)((const float *)c.head)[1]);
     if constexpr (F32) {
-      for (long long k = threadIdx.x * 4; k < c.ldg / 4; k += 1024) {
-        float4 p = *reinterpret_cast<const float4 *>(row + k * 4);
-        const float e = __builtin_amdgcn_exp2f(st[k / wcols].x - l) * f;
-        float v[4] = {p.x * e, p.y * e, p.z * e, p.w * e};
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (k + q == label) v[q] = at;
-        _Float16 hi[4], lo[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) split16(v[q], hi[q], lo[q]);
-        // 32 values a group, 8 lanes of one wave: all of its loads have returned before any of its stores leaves
-        char *d = row + (k >> 5) * 128 + (k & 31) * 2;
-        *reinterpret_cast<uint2 *>(d) = *reinterpret_cast<uint2 *>(hi);
-        *reinterpret_cast<uint2 *>(d + 64) = *reinterpret_cast<uint2 *>(lo);
-      }
+      if (threadIdx.x == 0) c.row[row0 + j] = make_float4(ms, f, t, scale_of(c, 3) / scale_for(c.xmax[row0 + j]));
     } else {
+      char *row = c.g + j * c.ldg;
       for (long long k = threadIdx.x * 8; k < c.ldg / 2; k += 2048) {
         unsigned short p[8];
-        bf16 t[8];
+        bf16 v[8];
         *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(row + k * 2);
-        const float e = __builtin_amdgcn_exp2f(st[k / wcols].x - l) * f;
+        const float e = __builtin_amdgcn_exp2f(st[k / wcols].x - ms) * f;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) t[q] = (bf16)(k + q == label ? at : unpack_exp(p[q]) * e);
-        *reinterpret_cast<uint4 *>(row + k * 2) = *reinterpret_cast<uint4 *>(t);
+        for (int q = 0; q < 8; ++q) v[q] = (bf16)(k + q == label ? -1.f : unpack_exp(p[q]) * e);
+        *reinterpret_cast<uint4 *>(row + k * 2) = *reinterpret_cast<uint4 *>(v);
       }
-      const float t = (float)(rest * (double)w / (double)((const float *)c.head)[1]);
       if (threadIdx.x == 0) c.t[row0 + j] = t;
       if (want_dw) {
         const char *from = c.xp + (row0 + j) * c.ldx;
@@ -450,6 +434,99 @@ __global__ __launch_bounds__(256) void ce_grad_kernel(Ce c, int row0, int wcols,
   }
 }
 
+// fp32: the exponentials of kSlabRows rows x kSlabCols classes become g, as the two products and db want it.
+//   dx  g' = p / (1 - p_label), the label's -1: relative to its row, the row's factor t joins at the end
+//   dW  t g' over x's own scale: a class has a scale of its own (a power of two, for these rows, undone where the product's accumulators restart).
+//       Fp16 planes relative to the row would lose the classes that are unlikely in every row: 22 bits end at 2^-17, all of them at 2^-39
+//   db  sums of t g' in fp32
+// Two forms of g are written where both are wanted: 105 us for 2010 rows of 20011 classes (4.6 TB/s).  16 threads a row, 8 rows a thread
+__global__ __launch_bounds__(256) void ce_slab_kernel(Ce c, int row0, int wcols, int want_dx, int want_dw, int want_db) {
+  __shared__ float lmax[16][kSlabCols], lsum[16][kSlabCols];
+  __shared__ float4 rows[kSlabRows];
+  __shared__ int labels[kSlabRows];
+  const int live = min(c.head[0] - row0, c.cap), j0 = blockIdx.y * kSlabRows, i0 = blockIdx.x * kSlabCols, own = i0 + threadIdx.x;
+  const bool column = threadIdx.x < kSlabCols && own < c.classes;
+  if (j0 >= live) {
+    if (want_db && !row0 && column) c.dbpart[(long long)blockIdx.y * c.classes + own] = 0.f;
+    return;
+  }
+  const int cg = (threadIdx.x & 15) * 4, rg = threadIdx.x >> 4, i = i0 + cg;
+  const bool in = i < c.ldg / 4;
+  float v[8][4], m[4], s[4], top[8];
+  const int i_load = in ? i : 0;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {                              // all loads side by side: what lies outside repeats the last row or the first classes
+    const int j = min(j0 + rg + 16 * q, live - 1);
+    *reinterpret_cast<float4 *>(v[q]) = *reinterpret_cast<const float4 *>(c.g + j * c.ldg + i_load * 4);
+    top[q] = c.stats[(long long)j * c.pieces + i_load / wcols].x;
+  }
+  if (threadIdx.x < kSlabRows && j0 + (int)threadIdx.x < live) {
+    rows[threadIdx.x] = c.row[row0 + j0 + threadIdx.x];
+    labels[threadIdx.x] = c.label[row0 + j0 + threadIdx.x];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < 4; ++e) m[e] = s[e] = 0.f;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const int r = rg + 16 * q;
+    if (j0 + r >= live) break;
+    const float4 f = rows[r];
+    const float e2 = __builtin_amdgcn_exp2f(top[q] - f.x) * f.y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[q][e] = i + e == labels[r] ? -1.f : v[q][e] * e2;
+      s[e] += v[q][e] * f.z;
+      m[e] = fmaxf(m[e], fabsf(v[q][e] * (f.z * f.w)));
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    lmax[rg][cg + e] = m[e];
+    lsum[rg][cg + e] = s[e];
+  }
+  __syncthreads();                                           // every load of g has returned too: what follows may be stored in its place
+  float scale[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) t = fmaxf(t, lmax[k][cg + e]);
+    int k = 0;
+    if (t > 0.f && t < 3.0e38f) k = min(max(13 - ilogbf(t), -100), 120);
+    scale[e] = __int_as_float((127 + k) << 23);
+    if (want_dw && rg == 0 && i + e < c.classes) c.ge[(long long)blockIdx.y * c.classes + i + e] = (signed char)k;
+  }
+  if (want_db && column) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) t += lsum[k][threadIdx.x];
+    float *d = c.dbpart + (long long)blockIdx.y * c.classes + own;
+    *d = row0 ? *d + t : t;                                  // pieces one after the other
+  }
+  if (!in) return;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const int r = rg + 16 * q;
+    if (j0 + r >= live) break;
+    const long long at = (j0 + r) * c.ldg + (i >> 5) * 128 + (i & 31) * 2;
+    _Float16 hi[4], lo[4];
+    if (want_dx) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) split16(v[q][e] * kSG, hi[e], lo[e]);
+      *reinterpret_cast<uint2 *>(c.gx + at) = *reinterpret_cast<uint2 *>(hi);
+      *reinterpret_cast<uint2 *>(c.gx + at + 64) = *reinterpret_cast<uint2 *>(lo);
+    }
+    if (want_dw) {
+      const float f = rows[r].z * rows[r].w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) split16(v[q][e] * f * scale[e], hi[e], lo[e]);
+      *reinterpret_cast<uint2 *>(c.g + at) = *reinterpret_cast<uint2 *>(hi);
+      *reinterpret_cast<uint2 *>(c.g + at + 64) = *reinterpret_cast<uint2 *>(lo);
+    }
+  }
+}
+
 // part z of dx: live rows x hidden, summed over the z-th share of the classes
 template <class T> __device__ __forceinline__ void dx_tile(const Ce &c, int row0, int bid, char *lds) {
   const int live = min(c.head[0] - row0, c.cap);
@@ -461,7 +538,7 @@ template <class T> __device__ __forceinline__ void dx_tile(const Ce &c, int row0
   const int total = (c.classes + T::KK - 1) / T::KK;
   const int s0 = (int)((long long)total * zi / c.z), s1 = (int)((long long)total * (zi + 1) / c.z);
   f32x4 acc[T::TI][T::TJ];
-  run<T>(lds, side_ks<T>(c.wp, c.ldw, c.classes, c.ldx, ti * T::BI * (T::SPLIT ? 4 : 2), s0), side_kc<T>(c.g, c.ldg, live, c.ldg, tj * T::BJ, s0),
+  run<T>(lds, side_ks<T>(c.wp, c.ldw, c.classes, c.ldx, ti * T::BI * (T::SPLIT ? 4 : 2), s0), side_kc<T>(T::SPLIT ? c.gx : c.g, c.ldg, live, c.ldg, tj * T::BJ, s0),
          s1 - s0, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave % T::NWI, wj = wave / T::NWI;
   const int hp = (c.hidden + 3) / 4 * 4;
@@ -482,18 +559,17 @@ template <class T> __device__ __forceinline__ void dx_tile(const Ce &c, int row0
 template <bool F32> __device__ __forceinline__ void dx_row(const Ce &c, int row0, int r) {
   const int live = min(c.head[0] - row0, c.cap);
   const int hp = (c.hidden + 3) / 4 * 4;
-  const float avg = ((const float *)c.head)[1], rsw = F32 ? 1.f / scale_of(c, 2) : 1.f;
   const int p = c.pos[r];
   if (p >= 0 && (p < row0 || p >= row0 + live)) return;                       // another piece's row
-  const float f = F32 ? (c.row_weight ? c.row_weight[r] : 1.f) / avg * (rsw / kSG) : p >= 0 ? c.t[p] : 0.f;
+  const float t = p < 0 ? 0.f : F32 ? c.row[p].z : c.t[p], ws = F32 ? 1.f / kSG / scale_of(c, 2) : 1.f;      // one by one: their product may leave fp32's range
   for (int k = threadIdx.x * 4; k < c.hidden; k += 1024) {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (p >= 0) {
       for (int z = 0; z < c.z; ++z) {
-        const float4 t = *reinterpret_cast<const float4 *>(c.part + ((long long)z * c.cap + p - row0) * hp + k);
-        v.x += t.x; v.y += t.y; v.z += t.z; v.w += t.w;
+        const float4 a = *reinterpret_cast<const float4 *>(c.part + ((long long)z * c.cap + p - row0) * hp + k);
+        v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
       }
-      v.x *= f; v.y *= f; v.z *= f; v.w *= f;
+      v.x = v.x * ws * t; v.y = v.y * ws * t; v.z = v.z * ws * t; v.w = v.w * ws * t;
     }
     const float o[4] = {v.x, v.y, v.z, v.w};
     const long long at = (long long)r * c.hidden + k;
@@ -511,20 +587,41 @@ template <bool F32> __device__ __forceinline__ void dx_row(const Ce &c, int row0
   }
 }
 
-// dW tile: classes x hidden, summed over the piece's live rows.  mode 0: store in the caller's type, 1: store to / 2: add to an fp32 accumulator
-template <class T> __device__ __forceinline__ void dw_tile(const Ce &c, int row0, int mode, int bid, char *lds) {
-  const int live = max(min(c.head[0] - row0, c.cap), 0);
-  if (live == 0 && row0) return;
+// what kSlabRows rows add to this lane's classes: their scale undone, from LDS, and that of x
+template <class T> struct ClassScales {
+  const signed char *at;
+  float f;
+  __device__ __forceinline__ float operator()(int slab, int b) const { return f * __int_as_float((127 - at[slab * T::BJ + b * 16]) << 23); }
+};
+
+// dW tile: classes x hidden, summed over the piece's live rows (fp32: kScaleRows of them, from `from` on; a loop over them here costs 25 spilled
+// registers and 15 % of the time).  mode 0: store in the caller's type, 1: store to / 2: add to an fp32 accumulator
+template <class T> __device__ __forceinline__ void dw_tile(const Ce &c, int row0, int mode, int from, int bid, char *lds) {
+  int live = max(min(c.head[0] - row0, c.cap), 0);
+  if (live <= from && row0 + from) return;
   const int nti = (c.hidden + T::BI - 1) / T::BI, ntj = (c.classes + T::BJ - 1) / T::BJ;
   int ti, tj;
   tile_of(bid, nti * ntj, nti, ntj, ti, tj);
   constexpr int E = T::SPLIT ? 4 : 2;
-  f32x4 acc[T::TI][T::TJ];
-  const char *x = c.xwp + row0 * c.ldx;
-  run<T>(lds, side_ks<T>(x, c.ldx, live, c.ldx, ti * T::BI * E, 0), side_ks<T>(c.g, c.ldg, live, c.ldg, (long long)tj * T::BJ * E, 0),
-         (live + T::KK - 1) / T::KK, acc);
+  const char *x = (T::SPLIT ? c.xp : c.xwp) + row0 * c.ldx;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave % T::NWI, wj = wave / T::NWI;
-  const float f = T::SPLIT ? 1.f / (kSG * ((const float *)c.head)[1] * scale_of(c, 3)) : 1.f;
+  f32x4 acc[T::TI][T::TJ];
+  if constexpr (T::SPLIT) {
+    static_assert(T::RESTART * T::KK == kSlabRows, "a part of the sums is a slab");
+    live = min(live, from + kScaleRows);
+    signed char *scales = reinterpret_cast<signed char *>(lds + T::LDS_BYTES);
+    for (int k = threadIdx.x; k < kScaleRows / kSlabRows * T::BJ; k += T::THREADS) {
+      const int j = tj * T::BJ + k % T::BJ, slab = from / kSlabRows + k / T::BJ;
+      scales[k] = j < c.classes && slab * kSlabRows < live ? c.ge[(long long)slab * c.classes + j] : 0;
+    }
+    __syncthreads();
+    const int s = from / T::KK;
+    run<T>(lds, side_ks<T>(x, c.ldx, live, c.ldx, ti * T::BI * E, s), side_ks<T>(c.g, c.ldg, live, c.ldg, (long long)tj * T::BJ * E, s),
+           (live - from + T::KK - 1) / T::KK, acc, ClassScales<T>{scales + wj * T::TJ * 16 + (lane & 15), 1.f / scale_of(c, 3)});
+  } else {
+    run<T>(lds, side_ks<T>(x, c.ldx, live, c.ldx, ti * T::BI * E, 0), side_ks<T>(c.g, c.ldg, live, c.ldg, (long long)tj * T::BJ * E, 0),
+           (live + T::KK - 1) / T::KK, acc);
+  }
 #pragma unroll
   for (int b = 0; b < T::TJ; ++b) {
     const int j = tj * T::BJ + (wj * T::TJ + b) * 16 + (lane & 15);
@@ -532,9 +629,7 @@ template <class T> __device__ __forceinline__ void dw_tile(const Ce &c, int row0
 #pragma unroll
     for (int a = 0; a < T::TI; ++a) {
       const int i = ti * T::BI + (wi * T::TI + a) * 16 + (lane >> 4) * 4;
-      float v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = T::SPLIT ? acc[a][b][e] * f : acc[a][b][e];
+      const f32x4 v = acc[a][b];
       const long long at = (long long)j * c.hidden + i;
       const bool whole = i + 4 <= c.hidden;
       if (T::SPLIT || mode) {
@@ -566,10 +661,10 @@ __global__ __launch_bounds__(256) void ce_dw_round_kernel(const float *__restric
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) dw[i] = (bf16)acc[i];
 }
 
-// db: column sums of g.  A workgroup adds kDbRows rows of 256 columns: 8 columns (16 bytes, split: of each plane) a thread and 8 rows side
+// bf16's db: column sums of g.  A workgroup adds kDbRows rows of 256 columns: 8 columns (16 bytes) a thread and 8 rows side
 // by side, which meet in LDS; the parts are added in order afterwards
 constexpr int kDbRows = 64;
-template <bool F32> __device__ __forceinline__ void db_part(const Ce &c, int row0, int bx, int slice, char *lds) {
+__device__ __forceinline__ void db_part(const Ce &c, int row0, int bx, int slice, char *lds) {
   float (*sum)[256] = reinterpret_cast<float (*)[256]>(lds);
   const int live = min(c.head[0] - row0, c.cap);
   const int j0 = slice * kDbRows, j1 = min(j0 + kDbRows, live);
@@ -580,19 +675,10 @@ template <bool F32> __device__ __forceinline__ void db_part(const Ce &c, int row
   if (i < c.classes) {                                       // whole groups of 8 exist: rows are padded with zeros
 #pragma unroll 4
     for (int j = j0 + sub; j < j1; j += 8) {
-      const char *row = c.g + j * c.ldg;
-      if constexpr (F32) {
-        const char *d = row + (i >> 5) * 128 + (i & 31) * 2;
-        const f16x8 h = *reinterpret_cast<const f16x8 *>(d), l = *reinterpret_cast<const f16x8 *>(d + 64);
-        const float w = c.row_weight ? c.row_weight[c.index[row0 + j]] : 1.f;
+      const bf16x8 v = *reinterpret_cast<const bf16x8 *>(c.g + j * c.ldg + i * 2);
+      const float t = c.t[row0 + j];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] += ((float)h[e] + (float)l[e]) * w;
-      } else {
-        const bf16x8 v = *reinterpret_cast<const bf16x8 *>(row + i * 2);
-        const float t = c.t[row0 + j];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] += (float)v[e] * t;
-      }
+      for (int e = 0; e < 8; ++e) s[e] += (float)v[e] * t;
     }
   }
 #pragma unroll
@@ -603,21 +689,20 @@ template <bool F32> __device__ __forceinline__ void db_part(const Ce &c, int row
   float t = 0.f;
 #pragma unroll
   for (int k = 0; k < 8; ++k) t += sum[k][threadIdx.x];
-  if (F32) t /= kSG * ((const float *)c.head)[1];
   float *d = c.dbpart + (long long)slice * c.classes + o;
   *d = row0 ? *d + t : t;                                    // pieces one after the other
 }
 
-// The gradients' launches.  Tiles of 64 and 128 (one workgroup shape) share one launch with db's sums: each of the three alone leaves CUs idle
-template <class TX, class TW, bool F32>
-__global__ __launch_bounds__(256, 2) void ce_gradients_kernel(Ce c, int row0, int mode, int dx_blocks, int dw_blocks, int db_blocks) {
+// The gradients' launches.  Tiles of 64 and 128 (one workgroup shape) share one launch, bf16 with db's sums: each alone leaves CUs idle
+template <class TX, class TW>
+__global__ __launch_bounds__(256, 2) void ce_gradients_kernel(Ce c, int row0, int mode, int from, int dx_blocks, int dw_blocks, int db_blocks) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   int b = blockIdx.x;
   if (b < dx_blocks) return dx_tile<TX>(c, row0, b, lds);
   b -= dx_blocks;
-  if (b < dw_blocks) return dw_tile<TW>(c, row0, mode, b, lds);
+  if (b < dw_blocks) return dw_tile<TW>(c, row0, mode, from, b, lds);
   b -= dw_blocks;
-  db_part<F32>(c, row0, b % db_blocks, b / db_blocks, lds);
+  if constexpr (!TX::SPLIT) db_part(c, row0, b % db_blocks, b / db_blocks, lds);
 }
 template <class T> __global__ __launch_bounds__(T::THREADS, 2) void ce_dx_kernel(Ce c, int row0) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
@@ -625,11 +710,11 @@ template <class T> __global__ __launch_bounds__(T::THREADS, 2) void ce_dx_kernel
 }
 template <class T> __global__ __launch_bounds__(T::THREADS, 2) void ce_dw_kernel(Ce c, int row0, int mode) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  dw_tile<T>(c, row0, mode, blockIdx.x, lds);
+  dw_tile<T>(c, row0, mode, 0, blockIdx.x, lds);
 }
-template <bool F32> __global__ __launch_bounds__(256) void ce_db_kernel(Ce c, int row0) {
+__global__ __launch_bounds__(256) void ce_db_kernel(Ce c, int row0) {
   __shared__ __attribute__((aligned(16))) char lds[8 * 256 * 4];
-  db_part<F32>(c, row0, blockIdx.x, blockIdx.y, lds);
+  db_part(c, row0, blockIdx.x, blockIdx.y, lds);
 }
 
 // live rows of dx of a piece that is not the last
@@ -700,7 +785,7 @@ int tile_for(bool f32, long long i, long long j, long long z) {
 long long up(long long v, long long a) { return (v + a - 1) / a * a; }
 
 struct Layout {
-  size_t bytes, head, index, pos, label, xmax, xp, xwp, wp, g, stats, part, row_loss, dwacc, dbpart;
+  size_t bytes, head, index, pos, label, xmax, row, xp, xwp, wp, g, gx, ge, stats, part, row_loss, dwacc, dbpart;
   long long ldx, ldw, ldg;
   int cap, chunks, pieces, z, wcols, db_slices;
   int bt_logits, bt_dx, bt_dw;
@@ -729,8 +814,9 @@ int layout_of(const mr3d_linear_ce *a, Layout &l) {
   l.pack_w = f32 || a->hidden % 64 || a->weight_stride % 8 || a->weight_stride > 1 << 21 || ((uintptr_t)a->weight & 15);
   l.ldw = l.pack_w ? l.ldx : a->weight_stride * 2;
   l.chunks = 1;
-  // bytes a row of a piece needs: its exponentials, or only its (max, sum) pairs (one for 32 classes at most)
-  const long long row_bytes = train ? l.ldg : up(a->classes, 64) / 32 * 8;
+  // bytes a row of a piece needs: its exponentials (fp32 with dx and dW: and a second form of g), or only its (max, sum) pairs (one for 32 classes at most)
+  const bool two = f32 && a->want_dx && a->want_dweight;
+  const long long row_bytes = train ? l.ldg * (two ? 2 : 1) : up(a->classes, 64) / 32 * 8;
   long long cap = a->rows;
   if (cap * row_bytes > kPiece) {
     cap = kPiece / row_bytes / 256 * 256;
@@ -748,10 +834,13 @@ int layout_of(const mr3d_linear_ce *a, Layout &l) {
   l.label = take(at, (size_t)a->rows * 4);
   l.xmax = take(at, (size_t)a->rows * 4);
   l.xp = take(at, (size_t)(a->rows * l.ldx));
-  if (a->want_dweight) l.xwp = take(at, (size_t)(a->rows * l.ldx));
+  if (f32 && train) l.row = take(at, (size_t)a->rows * 16);
+  if (!f32 && a->want_dweight) l.xwp = take(at, (size_t)(a->rows * l.ldx));
   if (l.pack_w) l.wp = take(at, (size_t)(a->classes * l.ldx));
   l.stats = take(at, (size_t)cap * l.pieces * 8);
-  if (train) l.g = take(at, (size_t)(cap * l.ldg));
+  if (train) l.g = l.gx = take(at, (size_t)(cap * l.ldg));
+  if (two) l.gx = take(at, (size_t)(cap * l.ldg));
+  if (f32 && a->want_dweight) l.ge = take(at, (size_t)((cap + kSlabRows - 1) / kSlabRows * a->classes));
   if (a->want_dx) {
     // parts over the classes until two workgroups a CU have work; a part keeps 16 k-steps
     const long long steps = l.ldg / 128, most = steps / 16 > 1 ? steps / 16 : 1;
@@ -770,7 +859,7 @@ int layout_of(const mr3d_linear_ce *a, Layout &l) {
   l.bt_dw = tile_for(f32, a->hidden, a->classes, 1);
   if (a->want_dweight && !f32 && l.chunks > 1) l.dwacc = take(at, (size_t)a->classes * a->hidden * 4);
   if (a->want_dbias) {
-    l.db_slices = (int)((cap + kDbRows - 1) / kDbRows);
+    l.db_slices = f32 ? (int)((cap + kSlabRows - 1) / kSlabRows) : (int)((cap + kDbRows - 1) / kDbRows);
     l.dbpart = take(at, (size_t)l.db_slices * a->classes * 4);
   }
   l.bytes = at;
@@ -802,12 +891,18 @@ template <class T> int launch_dw(const Ce &c, int row0, int mode, hipStream_t q)
   ce_dw_kernel<T><<<dw_blocks<T>(c), T::THREADS, T::LDS_BYTES, q>>>(c, row0, mode);
   return MR3D_OK;
 }
-template <class TX, class TW, bool F32> void launch_gradients(const mr3d_linear_ce *a, const Ce &c, int row0, int mode, hipStream_t q) {
-  constexpr int lds = TX::LDS_BYTES > TW::LDS_BYTES ? TX::LDS_BYTES : TW::LDS_BYTES;
-  static_assert(lds <= 65536 && lds >= 8192 && TX::THREADS == 256 && TW::THREADS == 256, "");
-  const int nx = a->want_dx ? dx_blocks<TX>(c) : 0, nw = a->want_dweight ? dw_blocks<TW>(c) : 0, nb = (a->classes + 255) / 256;
-  const int n = nx + nw + (a->want_dbias ? nb * ((c.cap + kDbRows - 1) / kDbRows) : 0);
-  ce_gradients_kernel<TX, TW, F32><<<n, 256, lds, q>>>(c, row0, mode, nx, nw, nb);
+template <class TX, class TW> int launch_gradients(const mr3d_linear_ce *a, const Ce &c, int row0, int mode, hipStream_t q) {
+  constexpr bool F32 = TX::SPLIT;
+  constexpr int ldw = TW::LDS_BYTES + (F32 ? kScaleRows / kSlabRows * TW::BJ : 0), lds = TX::LDS_BYTES > ldw ? TX::LDS_BYTES : ldw;
+  static_assert(lds <= 81920 && lds >= 8192 && TX::THREADS == 256 && TW::THREADS == 256, "two workgroups a CU");
+  const int nw = a->want_dweight ? dw_blocks<TW>(c) : 0, nb = (a->classes + 255) / 256;
+  if (lds > 65536)
+    if (const int e = allow_lds(ce_gradients_kernel<TX, TW>, lds)) return e;
+  for (int from = 0; from == 0 || (F32 && nw && from < c.cap); from += kScaleRows) {
+    const int nx = a->want_dx && !from ? dx_blocks<TX>(c) : 0, n = nx + nw + (!F32 && a->want_dbias ? nb * ((c.cap + kDbRows - 1) / kDbRows) : 0);
+    if (n) ce_gradients_kernel<TX, TW><<<n, 256, lds, q>>>(c, row0, from ? 2 : mode, from, nx, nw, nb);
+  }
+  return MR3D_OK;
 }
 
 template <class TT, class F> int pick(int bt, F f) {
@@ -824,7 +919,7 @@ template <bool F32> int run_ce(const mr3d_linear_ce *a, const Layout &l, Ce &c, 
     const int per = 4 * kMaxRows, xb = a->rows < 128 * per ? (a->rows + per - 1) / per : 128, wb = a->classes < 512 * per ? (a->classes + per - 1) / per : 512;
     ce_max_kernel<<<xb + wb, 256, 0, q>>>(c, xb, wb);
   }
-  ce_pack_kernel<F32><<<a->rows + (l.pack_w ? a->classes : 0), 256, 0, q>>>(c, a->want_dweight);
+  ce_pack_kernel<F32><<<a->rows + (l.pack_w ? a->classes : 0), 256, 0, q>>>(c);
   for (int k = 0; k < l.chunks; ++k) {
     const int row0 = k * l.cap;
     int e = MR3D_OK;
@@ -838,17 +933,21 @@ template <bool F32> int run_ce(const mr3d_linear_ce *a, const Layout &l, Ce &c, 
     if (e) return e;
     const int mode = k ? 2 : (l.chunks > 1 ? 1 : 0);
     if (!train) continue;
-    if ((!a->want_dx || l.bt_dx < 256) && (!a->want_dweight || l.bt_dw < 256)) {
-      if (l.bt_dx == 128 && l.bt_dw == 128) launch_gradients<typename TX::Small, typename TW::Small, F32>(a, c, row0, mode, q);
-      else if (l.bt_dx == 128) launch_gradients<typename TX::Small, typename TW::Tiny, F32>(a, c, row0, mode, q);
-      else if (l.bt_dw == 128) launch_gradients<typename TX::Tiny, typename TW::Small, F32>(a, c, row0, mode, q);
-      else launch_gradients<typename TX::Tiny, typename TW::Tiny, F32>(a, c, row0, mode, q);
-    } else {
+    if (F32)
+      ce_slab_kernel<<<dim3((unsigned)((l.ldg / 4 + kSlabCols - 1) / kSlabCols), (l.cap + kSlabRows - 1) / kSlabRows), 256, 0, q>>>(c, row0, l.wcols, a->want_dx,
+                                                                                                                     a->want_dweight, a->want_dbias);
+    if (F32 || ((!a->want_dx || l.bt_dx < 256) && (!a->want_dweight || l.bt_dw < 256))) {
+      if (l.bt_dx == 128 && l.bt_dw == 128) e = launch_gradients<typename TX::Small, typename TW::Small>(a, c, row0, mode, q);
+      else if (l.bt_dx == 128) e = launch_gradients<typename TX::Small, typename TW::Tiny>(a, c, row0, mode, q);
+      else if (l.bt_dw == 128) e = launch_gradients<typename TX::Tiny, typename TW::Small>(a, c, row0, mode, q);
+      else e = launch_gradients<typename TX::Tiny, typename TW::Tiny>(a, c, row0, mode, q);
+      if (e) return e;
+    } else if constexpr (!F32) {
       if (a->want_dx) e = pick<TX>(l.bt_dx, [&](auto t) { return launch_dx<decltype(t)>(c, row0, q); });
       if (e) return e;
       if (a->want_dweight) e = pick<TW>(l.bt_dw, [&](auto t) { return launch_dw<decltype(t)>(c, row0, mode, q); });
       if (e) return e;
-      if (a->want_dbias) ce_db_kernel<F32><<<dim3((a->classes + 255) / 256, (l.cap + kDbRows - 1) / kDbRows), 256, 0, q>>>(c, row0);
+      if (a->want_dbias) ce_db_kernel<<<dim3((a->classes + 255) / 256, (l.cap + kDbRows - 1) / kDbRows), 256, 0, q>>>(c, row0);
     }
     if (a->want_dx && k + 1 < l.chunks) ce_dx_rows_kernel<F32><<<l.cap, 256, 0, q>>>(c, row0);
   }
@@ -883,10 +982,12 @@ extern "C" int mr3d_linear_cross_entropy(const mr3d_linear_ce *a, void *workspac
   c.head = (int *)(b + l.head); c.index = (int *)(b + l.index); c.pos = (int *)(b + l.pos);
   c.label = (int *)(b + l.label);
   c.xmax = c.t = (float *)(b + l.xmax);
+  c.row = (float4 *)(b + l.row);
   c.xp = b + l.xp; c.xwp = b + l.xwp;
   c.wp = l.pack_w ? b + l.wp : (char *)const_cast<void *>(a->weight);
   c.ldx = l.ldx; c.ldw = l.ldw; c.ldg = l.ldg;
-  c.g = b + l.g; c.stats = (float2 *)(b + l.stats); c.part = (float *)(b + l.part);
+  c.g = b + l.g; c.gx = b + l.gx; c.ge = (signed char *)(b + l.ge);
+  c.stats = (float2 *)(b + l.stats); c.part = (float *)(b + l.part);
   c.row_loss = (double *)(b + l.row_loss);
   c.dwacc = (float *)(b + l.dwacc); c.dbpart = (float *)(b + l.dbpart);
   c.cap = l.cap; c.pieces = l.pieces; c.z = l.z;
