@@ -11,7 +11,8 @@ def linear_cross_entropy(x, weight, label, row_weight=None, bias=None, avg_facto
     x [..., K] and weight [C, K]: both fp32 or both bf16; bias [C] in their type or fp32; label [...] int64; row_weight [...] (None: 1).
     A row counts when its weight is not 0, its label is not ignore_index and it lies before valid_rows (a device int32 scalar: static
     shapes with padding).  The others take no part, whatever they hold, and get zero gradients.  avg_factor: a number, a device scalar, or None for
-    max(number of counted rows with a positive weight, 1), as `weighted_cross_entropy` divides.  A counted label outside [0, C) makes the loss NaN.
+    max(number of counted rows with a positive weight, 1) (`weighted_cross_entropy` counts every positive weight, also of rows behind valid_rows:
+    the same where those rows have weight 0, as the samplers leave them).  A counted label outside [0, C) makes the loss NaN.
     Beside copies of x and weight the memory is bounded (2 GiB of exponentials, rows go through in pieces).  fp32: products carry 22 bits of
     each factor, relative to the largest of its row (x, and g for dx), of its class (g for dW) or of all (weight).  One backward per call;
     under graph capture both are captured (as `torch.cuda.make_graphed_callables` does) or neither."""
