@@ -773,6 +773,29 @@ extern "C" size_t mr3d_orthogonalize_workspace_bytes(const mr3d_matrix *mats_hos
   return plan_list(mats_host, count, nullptr, plan, nullptr, false) == MR3D_OK ? plan.bytes : 0;
 }
 
+extern "C" int mr3d_orthogonalize_tiles(const mr3d_matrix *mats_host, int count, mr3d_ortho_tiles *tiles_host) {
+  if (!tiles_host || !mats_host || count <= 0 || count > 65536) return MR3D_ERR_INVALID_ARG;
+  Mat *table = new (std::nothrow) Mat[count];
+  if (!table) return MR3D_ERR_INVALID_ARG;
+  Plan plan;
+  const int st = plan_list(mats_host, count, nullptr, plan, table, false);
+  if (st == MR3D_OK) {
+    mr3d_ortho_tiles t{{plan.bt_gram, plan.bt_square, plan.bt_apply}, {}, {}, {1, 1, 1}};
+    for (int k = 0; k < count; ++k) {
+      if (table[k].m <= kSmall) continue;
+      const Split s[3] = {table[k].gram, table[k].square, table[k].apply};
+      for (int i = 0; i < 3; ++i) {
+        t.whole[i] += s[i].whole;
+        t.split[i] += s[i].tiles - s[i].whole;
+        if (s[i].tiles > s[i].whole && s[i].z > t.parts[i]) t.parts[i] = s[i].z;
+      }
+    }
+    *tiles_host = t;
+  }
+  delete[] table;
+  return st;
+}
+
 extern "C" int mr3d_orthogonalize(const mr3d_matrix *mats_host, int count, int steps, float ca, float cb, float cc, float eps, void *workspace,
                                   size_t workspace_bytes, mr3d_stream_t s) {
   if (steps < 1 || steps > 100 || !(eps >= 0.f)) return MR3D_ERR_INVALID_ARG;

@@ -583,6 +583,13 @@ typedef struct {
 size_t mr3d_orthogonalize_workspace_bytes(const mr3d_matrix *mats_host, int count);
 int mr3d_orthogonalize(const mr3d_matrix *mats_host, int count, int steps, float a, float b, float c, float eps, void *workspace,
                        size_t workspace_bytes, mr3d_stream_t s);
+/* How the products A = X X^T (0), A A (1) and P X (2) of a list are cut, from its shapes alone (in / out may be NULL, nothing is launched): the width of
+ * their tiles (matrices of more than 64 rows), and over the whole list the tiles that one workgroup computes, those that several share, and the
+ * largest number of workgroups that share one. */
+typedef struct {
+  int width[3], whole[3], split[3], parts[3];
+} mr3d_ortho_tiles;
+int mr3d_orthogonalize_tiles(const mr3d_matrix *mats_host, int count, mr3d_ortho_tiles *tiles_host);
 
 /* ------------------------------------------------------------------------------------------------
  * DeformConv3d (v1) / modulated (v2): the sampling halves of the operator; the GEMM halves are
