@@ -43,10 +43,10 @@ struct Side {
   unsigned ldb;
 };
 
-template <int BI_, int BJ_, int NWI_, int NWJ_, bool IKS_, bool JKS_, bool SPLIT_, int RB_, int STAGES_> struct Tile {
+template <int BI_, int BJ_, int NWI_, int NWJ_, bool IKS_, bool JKS_, bool SPLIT_, int STAGES_> struct Tile {
   static constexpr int BI = BI_, BJ = BJ_, NWI = NWI_, NWJ = NWJ_, NW = NWI * NWJ, THREADS = NW * 64;
   static constexpr bool IKS = IKS_, JKS = JKS_, SPLIT = SPLIT_;
-  static constexpr int RB = RB_, STAGES = STAGES_;                          // bytes of a KC row per k-step, tiles in LDS
+  static constexpr int RB = 128, STAGES = STAGES_;                          // bytes of a KC row per k-step, tiles in LDS
   static constexpr int TI = BI / NWI / 16, TJ = BJ / NWJ / 16;              // 16 x 16 blocks of a wave
   static constexpr int IBYTES = BI * RB, JBYTES = BJ * RB, STAGE = IBYTES + JBYTES, LDS_BYTES = STAGES * STAGE;
   static constexpr int KK = SPLIT ? RB / 4 : RB / 2;                        // k of a k-step
@@ -54,7 +54,6 @@ template <int BI_, int BJ_, int NWI_, int NWJ_, bool IKS_, bool JKS_, bool SPLIT
   static constexpr int RESTART = SPLIT ? 128 / KK : 0;                     // k-steps between two restarts of the accumulators (0: never)
   static_assert(!SPLIT || TI * TJ <= 16, "accumulators and their sums fit the registers");
   static_assert(IBYTES % (1024 * NW) == 0 && JBYTES % (1024 * NW) == 0, "whole 1 KB loads per wave");
-  static_assert(RB == 128 || (RB == 64 && !SPLIT), "a split row's group is 128 bytes");
   static_assert(KK % 32 == 0, "whole matrix instructions");
 };
 
@@ -77,7 +76,7 @@ template <int ROWB> __device__ __forceinline__ int place(int kr, int c) {
   const int u = ROWB >= 256 ? kr & 3 : (kr >> 1) & 1;
   return c ^ (u << 2) ^ (((kr >> 3) & 1) << 1);
 }
-template <int RB> __device__ __forceinline__ int swizzle(int row) { return RB == 128 ? (row >> 1) & 7 : (row >> 2) & 3; }
+__device__ __forceinline__ int swizzle(int row) { return (row >> 1) & 7; }
 
 // source byte offset of this lane in load q of the wave (BT = tile extent, NL loads per wave)
 template <class T, int BT, int NL, bool KS>
@@ -86,7 +85,7 @@ __device__ __forceinline__ unsigned source_offset(int wave, int lane, int q, uns
   if constexpr (!KS) {
     constexpr int CPR = T::RB / 16;
     const int row = pos / CPR;
-    return row * ldb + (((pos % CPR) ^ swizzle<T::RB>(row)) << 4);
+    return row * ldb + (((pos % CPR) ^ swizzle(row)) << 4);
   } else {
     constexpr int ROWB = BT * (T::SPLIT ? 4 : 2), CPR = ROWB / 16;
     const int kr = pos / CPR, c = pos % CPR;
@@ -122,7 +121,7 @@ template <class T, int BT, bool KS>
 __device__ __forceinline__ i16x8 fragment(const char *lds, int b, int ks, int p, int lane) {
   if constexpr (!KS) {
     const int row = b * 16 + (lane & 15), chunk = (T::SPLIT ? p * 4 : 0) + ks * 4 + (lane >> 4);
-    return *reinterpret_cast<const i16x8 *>(lds + row * T::RB + ((chunk ^ swizzle<T::RB>(row)) << 4));
+    return *reinterpret_cast<const i16x8 *>(lds + row * T::RB + ((chunk ^ swizzle(row)) << 4));
   } else {
     constexpr int ROWB = BT * (T::SPLIT ? 4 : 2);
     const int s = lane & 15, kr = ks * 32 + (lane >> 4) * 8 + (s >> 2);

@@ -750,7 +750,8 @@ template <bool F32> __global__ __launch_bounds__(256) void ce_finish_kernel(Ce c
   else ((bf16 *)c.db)[i] = (bf16)(float)s;
 }
 
-// gradients *= *factor, unless the factor is 1 (the usual root of a backward pass): then nothing is read or written
+// gradients *= *factor, unless the factor is 1 (the usual root of a backward pass): then nothing is read or written.  bf16 gradients are rounded here a
+// second time (2^-8 at most; exact for powers of two): kept in fp32 until now they would cost as much memory again as x and W
 struct Spans { mr3d_span s[4]; };
 __global__ __launch_bounds__(256) void ce_scale_kernel(Spans spans, const float *__restrict__ factor) {
   const float f = *factor;
@@ -766,13 +767,13 @@ __global__ __launch_bounds__(256) void ce_scale_kernel(Spans spans, const float 
 // 128 x 128 (4 waves of 64 x 64, two workgroups a CU) below that, and for fp32, whose restarted sums leave no room for the large tile's
 // accumulators.  64 x 64 (three workgroups a CU) where even those would leave CUs without one: 1024^3, fp32: 25 -> 14 us.
 template <bool IKS, bool JKS, bool SPLIT> struct Tiles {
-  typedef Tile<64, 64, 2, 2, IKS, JKS, SPLIT, 128, 3> Tiny;
-  typedef Tile<128, 128, 2, 2, IKS, JKS, SPLIT, 128, 2> Small;
-  typedef Tile<256, 256, 2, 4, IKS, JKS, SPLIT, 128, 2> Large;
+  typedef Tile<64, 64, 2, 2, IKS, JKS, SPLIT, 3> Tiny;
+  typedef Tile<128, 128, 2, 2, IKS, JKS, SPLIT, 2> Small;
+  typedef Tile<256, 256, 2, 4, IKS, JKS, SPLIT, 2> Large;
 };
 template <bool IKS, bool JKS> struct Tiles<IKS, JKS, true> {
-  typedef Tile<64, 64, 2, 2, IKS, JKS, true, 128, 3> Tiny;
-  typedef Tile<128, 128, 2, 2, IKS, JKS, true, 128, 2> Small;
+  typedef Tile<64, 64, 2, 2, IKS, JKS, true, 3> Tiny;
+  typedef Tile<128, 128, 2, 2, IKS, JKS, true, 2> Small;
   typedef Small Large;
 };
 long long tiles_of(long long i, long long j, int bt) { return ((i + bt - 1) / bt) * ((j + bt - 1) / bt); }

@@ -6,8 +6,8 @@
 // once.  Double, because the noise of A is amplified by a^2 a step where singular values are small: fp32 loses 1e-5 .. 1e-4 over five steps.
 // It also gives |G|_F = sqrt(trace A) without overflow.
 //
-// Larger ones: every factor is kept as two fp16 planes (gemm16.h, split storage), scaled by powers of two into fp16's range: 22 bits, three passes
-// of the 16-bit matrix pipe, fp32 accumulators.  Plain bf16 or fp16 factors would lose 2e-2 / 2e-3 of the result over five steps (p's slope at 0
+// Larger ones: every factor is kept as two fp16 planes (gemm16.h, split storage), scaled by powers of two into fp16's range: 22 bits (of X down to
+// steps of 2^-36 |G|_F, of A and P 2^-36 and 2^-34), three passes of the 16-bit matrix pipe, fp32 accumulators.  Plain bf16 or fp16 factors would lose 2e-2 / 2e-3 of the result over five steps (p's slope at 0
 // is a = 3.4: rounding errors of the first steps are amplified a few hundred times).  Symmetric results: only the tiles on and below the diagonal are
 // computed and stored twice.  Iterating on A here too, in rounds of two or three steps between looks at X, was measured: 1.6 to 2.4 times fewer
 // products at n = 9 m, but no less time for the 64 matrices of a detector (the m x m products are short), and A's noise, amplified,
@@ -30,7 +30,7 @@ constexpr int kSmall = 64;                                  // rows of the small
 constexpr int kThreads = 256;
 
 // 128 x 128 with two tiles in LDS, two workgroups a CU, or 64 x 64 with three and as many workgroups
-template <int BT, bool APPLY> struct Pick { typedef Tile<BT, BT, 2, 2, APPLY, false, true, 128, BT == 128 ? 2 : 3> T; };
+template <int BT, bool APPLY> struct Pick { typedef Tile<BT, BT, 2, 2, APPLY, false, true, BT == 128 ? 2 : 3> T; };
 
 enum Stage { kNorm, kPack, kGram, kGramJoin, kSquare, kSquareJoin, kApply, kApplyJoin, kSmallGram, kSmallPoly, kSmallApply, kStages };
 enum Buf { kA, kP, kX0, kX1, kBufs };
