@@ -540,9 +540,10 @@ int mr3d_layer_norm_backward(const void *x, long long x_stride, const void *dy, 
  * fp32 products carry 22 bits of each factor, of x relative to the largest of its row, of weight to the largest of all, of the logits' gradients to the
  * largest of their row (dx) or of their class in 128 rows (dweight): what is 2^17 times smaller has fewer, what is 2^39 times smaller none.  bf16:
  * the logits' gradients but the label's and, for dweight, x times its row's factor are rounded to bf16 before their products.  Sums are fp32 or wider,
- * in a fixed order.  hidden <= 65536, classes <= 2^20, rows <= 2^22.  workspace: 1024-byte aligned device memory of mr3d_linear_cross_entropy_workspace_bytes (0 = refused): x (and, fp32 or unaligned, weight) in packed form, dx in fp32, and at most about
- * 2 GiB of exponentials, as many rows at a time as fit (256 at least).
- * mr3d_scale_by: up to 4 arrays *= *factor_dev in place, in one launch; nothing is touched when the factor is 1.
+ * in a fixed order.  hidden <= 65536, classes <= 2^20, rows <= 2^22.  workspace: 1024-byte aligned device memory
+ * of mr3d_linear_cross_entropy_workspace_bytes (0 = refused): x (and, fp32 or unaligned, weight) in packed form, dx in fp32, and at most about 2 GiB of
+ * exponentials (with dx and dweight in fp32 half of it is a second form of their gradients), as many rows at a time as fit (256 at least).
+ * mr3d_scale_by: up to 4 arrays *= *factor_dev in place, in one launch; nothing is touched when the factor is 1.  bf16 arrays are rounded (again).
  * ---------------------------------------------------------------------------------------------- */
 typedef struct {
   const void *x, *weight, *bias;
@@ -569,7 +570,7 @@ int mr3d_scale_by(const mr3d_span *spans_host, int num_spans, const float *facto
  *   X = G / (|G|_F + eps), transposed when rows > cols;   steps times:  A = X X^T,  X = a X + (b A + c A A) X;   out = X (transposed back)
  * in: element (r, c) at in[r * in_row_stride + c * in_col_stride]; out: packed row-major [rows][cols], of the same dtype (MR3D_DTYPE_F32 / _BF16);
  * out may be in itself (packed), no other overlap.  The whole list runs in one launch per stage.  Products carry 22 bits of each
- * factor with fp32 accumulation; bits do not vary between runs.  1 <= steps <= 100, |a|, |b|, |c| <= 16, rows and cols up to 2^20; singular values that
+ * factor (more than 64 rows and columns: of X down to steps of 2^-36 |G|_F) with fp32 accumulation; bits do not vary between runs.  1 <= steps <= 100, |a|, |b|, |c| <= 16, rows and cols up to 2^20; singular values that
  * the polynomial drives beyond about 4 overflow to infinity or NaN, and an input with NaN or infinity gives NaN in its own matrix.
  * workspace: 256-byte aligned device memory of mr3d_orthogonalize_workspace_bytes(the same list; 0 = the list is refused); mats_host is read
  * before the call returns.
