@@ -15,8 +15,8 @@
 // place of x, db multiplies.  fp32: dW's factor is t g' with a scale per class and 128 rows (ce_slab_kernel).
 // The exponentials of at most kPiece bytes of rows exist at a time; dW accumulates over such pieces in fp32.
 // Measured, 8192 x 2048 x 131072 bf16 (7782 live rows): logits 3.9 ms (1.08 PFLOP/s, exponentials and their 2 GB of stores included), grad 0.93 (4.4 TB/s),
-// dx 3.5, dW 3.5 (1.2): the matrix pipe at the clock its power allows.  3001 x 515 x 20011 fp32 (2010 live): logits 162 us, losses 12, g 105, gradients
-// 305, packing 34.  512 x 1024 x 1204 fp32: nine launches, 64 us in all.  One row, 1024 x 32768 bf16: logits 16 us (W at 4.2 TB/s), 10 in four small launches.
+// dx 3.5, dW 3.5 (1.2).  3001 x 515 x 20011 fp32 (2010 live): logits 162 us, losses 12, g 105, gradients
+// 305, packing 34.  512 x 1024 x 1204 fp32: nine launches, 64 us in all.  One row, 1024 x 32768 bf16: logits 16 us (W at 4.2 TB/s), 13 in four small launches.
 // Recomputing z for the gradient instead (no such buffer at all) costs 2 R V K more: 1.7 ps a logit at 1024 features against 0.8 ps for the
 // buffer's extra trip through memory.
 #include "gemm16.h"

@@ -7,8 +7,8 @@
 // Backward: a workgroup walks rows in a grid-stride loop; the dw / db sums of a lane's own columns stay in registers over all its rows,
 // then meet in LDS and leave as ONE partial row per workgroup; ln_param_kernel adds the partial rows in a fixed order in double
 // (no atomics: run-to-run identical bits).
-// Measured, forward / backward / parameter sums: 655360 x 64 bf16 36 / 55 / 5 us, 10007 x 1531 fp32 25 / 38 / 5 us -- 4.6 to 4.9 TB/s, what a large
-// copy reaches; 512 x 1024 fp32 4.2 / 5.9 / 4.1 us and 1 x 1024 2.4 us are launches.
+// Measured, forward / backward / parameter sums: 655360 x 64 bf16 37 / 55 / 5 us, 10007 x 1531 fp32 27 / 38 / 5 us -- 4.5 to 4.8 TB/s, about what a
+// large copy reaches; 512 x 1024 fp32 4.6 / 5.9 / 4.0 us and 1 x 1024 2.6 us are launches.
 #include "mr3d_common.h"
 #include <hip/hip_bf16.h>
 
