@@ -6,7 +6,7 @@ import pytest
 import torch
 
 
-def _work(seed, dtype):
+def _data(seed, dtype):
     g = torch.Generator().manual_seed(seed)
     x = torch.randn(700, 520, generator=g).to(dtype).cuda()
     lw = (1 + 0.1 * torch.randn(520, generator=g)).to(dtype).cuda()
@@ -35,15 +35,15 @@ def _same(a, b):
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 def test_two_streams(dtype):
-    work = [_work(k, dtype) for k in range(2)]
-    alone = [_step(s) for s in work]
+    data = [_data(k, dtype) for k in range(2)]
+    alone = [_step(s) for s in data]
     torch.cuda.synchronize()
-    streams = [torch.cuda.Stream() for _ in work]
+    streams = [torch.cuda.Stream() for _ in data]
     kept = [[], []]
     for _ in range(4):
         for k, st in enumerate(streams):
             with torch.cuda.stream(st):
-                kept[k].append(_step(work[k]))
+                kept[k].append(_step(data[k]))
     torch.cuda.synchronize()
     assert all(_same(r, alone[k]) for k in range(2) for r in kept[k])
 
@@ -51,8 +51,8 @@ def test_two_streams(dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 def test_two_threads(dtype):
-    work = [_work(k, dtype) for k in range(2)]
-    alone = [_step(s) for s in work]
+    data = [_data(k, dtype) for k in range(2)]
+    alone = [_step(s) for s in data]
     torch.cuda.synchronize()
     out, errors = [[], []], []
 
@@ -60,7 +60,7 @@ def test_two_threads(dtype):
         try:
             with torch.cuda.stream(torch.cuda.Stream()):
                 for _ in range(4):
-                    out[k].append(_step(work[k]))
+                    out[k].append(_step(data[k]))
                 torch.cuda.current_stream().synchronize()
         except Exception as e:                               # shown by the assertion below
             errors.append(e)
@@ -78,22 +78,22 @@ def test_two_threads(dtype):
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 def test_two_graphs_in_turn(dtype):
     """replays of two graphs alternate with each other and with eager calls on changed inputs"""
-    work = [_work(k, dtype) for k in range(2)]
-    for s in work:
+    data = [_data(k, dtype) for k in range(2)]
+    for s in data:
         _step(s)
     torch.cuda.synchronize()
     graphs, held = [], []
-    for s in work:
+    for s in data:
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             held.append(_step(s))
         graphs.append(g)
     for turn in range(3):
         for k in (0, 1) if turn % 2 else (1, 0):
-            fresh = _work(10 * turn + k, dtype)
-            for t, f in zip(work[k], fresh):
+            fresh = _data(10 * turn + k, dtype)
+            for t, f in zip(data[k], fresh):
                 t.copy_(f)
             graphs[k].replay()
         torch.cuda.synchronize()
         for k in range(2):
-            assert _same(held[k], _step(work[k])), (turn, k)
+            assert _same(held[k], _step(data[k])), (turn, k)
