@@ -70,6 +70,9 @@ template <bool F32> __device__ __forceinline__ float elem(const char *p, long lo
   return F32 ? ((const float *)p)[i] : (float)((const bf16 *)p)[i];
 }
 
+// e^v for v <= 0, one instruction behind the product.  The difference comes first: logits of the type's lowest value (a mask) times log2 e would be infinite
+__device__ __forceinline__ float exp_of(float v) { return __builtin_amdgcn_exp2f(v * kLog2e); }
+
 // Two exponentials in [0, 1] as 16 bits each: of an fp32 value the sign and the upper bit of the exponent are 0 there, the next 16 bits are kept
 // (rounded).  2^-10 of the value over fp32's whole range down to 2^-126: fp16 would have 2^-11, but only above 2^-14 of the largest of the 128
 // classes, and nothing below 2^-25, where g in bf16 still has its 8 bits
@@ -252,7 +255,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void ce_logits_kernel(Ce c, int row0
   run<T>(lds, side_kc<T>(c.wp, c.ldw, c.classes, c.ldx, ti * T::BI, 0), side_kc<T>(c.xp + row0 * c.ldx, c.ldx, live, c.ldx, tj * T::BJ, 0),
          (int)(c.ldx / 128), acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave % T::NWI, wj = wave / T::NWI;
-  const float rsw = T::SPLIT ? kLog2e / scale_of(c, 2) : kLog2e;
+  const float rsw = T::SPLIT ? 1.f / scale_of(c, 2) : 1.f;
   const int vpad = (int)(c.ldg / (T::SPLIT ? 4 : 2));
   constexpr int WI = T::TI * 16;
   static_assert(kStatCols % WI == 0, "a wave's classes lie in one pair");
@@ -262,16 +265,15 @@ __global__ __launch_bounds__(T::THREADS, 2) void ce_logits_kernel(Ce c, int row0
     const int jl = (wj * T::TJ + b) * 16 + (lane & 15), j = tj * T::BJ + jl;
     const float rs = T::SPLIT ? rsw / scale_for(j < live ? c.xmax[row0 + j] : 0.f) : rsw;
     const int iw = ti * T::BI + wi * WI + (lane >> 4) * 4;
-    // z log2 e: exponentials and sums are taken to base 2, one instruction each
     if (c.bias) {
 #pragma unroll
       for (int a = 0; a < T::TI; ++a)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int i = min(iw + a * 16 + e, c.classes - 1);
-          acc[a][b][e] = fmaf(acc[a][b][e], rs, kLog2e * (c.bias_f32 ? ((const float *)c.bias)[i] : (float)((const bf16 *)c.bias)[i]));
+          acc[a][b][e] = fmaf(acc[a][b][e], rs, c.bias_f32 ? ((const float *)c.bias)[i] : (float)((const bf16 *)c.bias)[i]);
         }
-    } else {
+    } else if constexpr (T::SPLIT) {
 #pragma unroll
       for (int a = 0; a < T::TI; ++a)
 #pragma unroll
@@ -305,7 +307,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void ce_logits_kernel(Ce c, int row0
     for (int a = 0; a < T::TI; ++a)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float p = __builtin_amdgcn_exp2f(acc[a][b][e] - ms);
+        const float p = exp_of(acc[a][b][e] - ms);
         s += p;
         acc[a][b][e] = p;
       }
@@ -395,12 +397,12 @@ __global__ __launch_bounds__(256) void ce_grad_kernel(Ce c, int row0, int wcols,
   m = block_max(nan ? INFINITY : m, ldm);                    // infinity less infinity: the row's sums become NaN
   const float ms = m == -INFINITY ? 0.f : m;
   double s = 0;
-  for (int k = threadIdx.x; k < c.pieces; k += 256) s += (double)st[k].y * (double)__builtin_amdgcn_exp2f(st[k].x - ms);
+  for (int k = threadIdx.x; k < c.pieces; k += 256) s += (double)st[k].y * (double)exp_of(st[k].x - ms);
   block_sum(s, dot, lds);
-  // the others' sum is s 2^m; with the label's 2^d: lse, 1 - p_label, and lse - z_label without a difference where that is small
-  const double d = label >= 0 ? dot * 1.44269504088896340736 : (double)NAN, top = fmax((double)m, d);
-  const double others = s * exp2((double)m - top), all = others + exp2(d - top), rest = others / all;
-  const double ce = ((double)m < d ? log1p(s * exp2((double)m - d)) : (top + log2(all)) * 0.69314718055994530942 - dot) + (all - all);   // NaN stays
+  // the others' sum is s e^m; with the label's e^d: 1 - p_label, and lse - z_label without a difference of sums where that is small
+  const double d = label >= 0 ? dot : (double)NAN, top = fmax((double)m, d);
+  const double others = s * exp((double)m - top), all = others + exp(d - top), rest = others / all;
+  const double ce = ((double)m < d ? log1p(s * exp((double)m - d)) : (top - d) + log(all)) + (all - all);   // NaN stays
   const float w = c.row_weight ? c.row_weight[r] : 1.f;
   if (threadIdx.x == 0) c.row_loss[row0 + j] = ce * (double)w;
   if constexpr (TRAIN) {
@@ -414,7 +416,7 @@ __global__ __launch_bounds__(256) void ce_grad_kernel(Ce c, int row0, int wcols,
         unsigned short p[8];
         bf16 v[8];
         *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(row + k * 2);
-        const float e = __builtin_amdgcn_exp2f(st[k / wcols].x - ms) * f;
+        const float e = exp_of(st[k / wcols].x - ms) * f;
 #pragma unroll
         for (int q = 0; q < 8; ++q) v[q] = (bf16)(k + q == label ? -1.f : unpack_exp(p[q]) * e);
         *reinterpret_cast<uint4 *>(row + k * 2) = *reinterpret_cast<uint4 *>(v);
@@ -472,7 +474,7 @@ __global__ __launch_bounds__(256) void ce_slab_kernel(Ce c, int row0, int wcols,
     const int r = rg + 16 * q;
     if (j0 + r >= live) break;
     const float4 f = rows[r];
-    const float e2 = __builtin_amdgcn_exp2f(top[q] - f.x) * f.y;
+    const float e2 = exp_of(top[q] - f.x) * f.y;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       v[q][e] = i + e == labels[r] ? -1.f : v[q][e] * e2;
