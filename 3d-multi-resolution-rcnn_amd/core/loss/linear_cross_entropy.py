@@ -14,7 +14,8 @@ def linear_cross_entropy(x, weight, label, row_weight=None, bias=None, avg_facto
     max(number of counted rows with a positive weight, 1) (`weighted_cross_entropy` counts every positive weight, also of rows behind valid_rows:
     the same where those rows have weight 0, as the samplers leave them).  A counted label outside [0, C) makes the loss NaN.
     Beside copies of x and weight the memory is bounded (2 GiB of exponentials, rows go through in pieces).  fp32: products carry 22 bits of
-    each factor, relative to the largest of its row (x, and g for dx), of its class (g for dW) or of all (weight).  bf16 gradients are rounded
+    each factor, relative to the largest of its row (x, and g for dx), of its class (g for dW) or of all (weight, but classes
+    whose bias is -1e30 or less).  bf16 gradients are rounded
     once more when the incoming gradient is no power of two.  One backward per call; under graph capture both are captured (as
     `torch.cuda.make_graphed_callables` does) or neither."""
     on_device = torch.is_tensor(avg_factor)

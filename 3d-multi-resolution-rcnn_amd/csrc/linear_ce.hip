@@ -42,7 +42,7 @@ struct Ce {
   long long x_stride, w_stride, ignore;                      // strides in elements
   int rows, hidden, classes, bias_f32;
   // workspace
-  int *head;                                                 // [0] live rows  [1] avg (float)  [2] max |W|  [3] max |x w| (float bits)
+  int *head;                                                 // [0] live rows  [1] avg (float)  float bits of the largest: [2] |W|  [3] |x|  [4] |W| of masked classes
   int *index, *pos;                                          // live row -> row, row -> live row or -1
   int *label;                                                // of a live row; -1: outside the classes
   float *xmax, *t;                                           // of a live row.  fp32: max |x|.  bf16: w (1 - p_label) / avg
@@ -88,7 +88,12 @@ __device__ __forceinline__ float scale_for(float max) {
   e = e > 100 ? 100 : e;
   return ldexpf(1.f, e);
 }
-__device__ __forceinline__ float scale_of(const Ce &c, int slot) { return scale_for(__int_as_float(c.head[slot])); }
+__device__ __forceinline__ float scale_of_x(const Ce &c) { return scale_for(__int_as_float(c.head[3])); }
+// fp32: a class whose bias masks it may have any (finite) weights: they do not set the scale, and are cut off at fp16's largest value.  Where every
+// class is masked, they all count
+constexpr float kMasked = -1e30f;
+__device__ __forceinline__ bool masked_class(const Ce &c, int v) { return c.bias && ((const float *)c.bias)[v] <= kMasked; }
+__device__ __forceinline__ float scale_of_w(const Ce &c) { return scale_for(__int_as_float(c.head[2] ? c.head[2] : c.head[4])); }
 
 // live rows in order: a prefix sum over 1024 rows at a time by one workgroup
 __global__ __launch_bounds__(1024) void ce_rows_kernel(Ce c) {
@@ -127,7 +132,7 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(Ce c) {
   if (threadIdx.x == 0) {
     c.head[0] = base;
     ((float *)c.head)[1] = c.avg_dev ? *c.avg_dev : (c.avg_host > 0.f ? c.avg_host : (float)max(positive, 1));
-    c.head[2] = c.head[3] = 0;
+    c.head[2] = c.head[3] = c.head[4] = 0;
   }
 }
 
@@ -163,7 +168,7 @@ __device__ __forceinline__ void rows_max(const float *const (&p)[kMaxRows], int 
 // a thousand of them on one address take 15 us
 __global__ __launch_bounds__(256) void ce_max_kernel(Ce c, int xblocks, int wblocks) {
   __shared__ float lds[4];
-  float m = 0.f, v[kMaxRows];
+  float m = 0.f, mm = 0.f, v[kMaxRows];
   const float *p[kMaxRows];
   const int wave = threadIdx.x >> 6;
   const bool is_x = (int)blockIdx.x < xblocks;
@@ -190,15 +195,23 @@ __global__ __launch_bounds__(256) void ce_max_kernel(Ce c, int xblocks, int wblo
       for (int r = 0; r < kMaxRows; ++r) p[r] = (const float *)c.w + (j + r < c.classes ? j + r : j) * c.w_stride;
       rows_max(p, c.hidden, v);
 #pragma unroll
-      for (int r = 0; r < kMaxRows; ++r) m = fmaxf(m, v[r]);
+      for (int r = 0; r < kMaxRows; ++r) {
+        const bool masked = masked_class(c, min(j + r, c.classes - 1));
+        m = fmaxf(m, masked ? 0.f : v[r]);
+        mm = fmaxf(mm, masked ? v[r] : 0.f);
+      }
     }
   }
   m = block_max(m, lds);
   if (threadIdx.x == 0 && m > 0.f) atomicMax(&c.head[is_x ? 3 : 2], __float_as_int(m));
+  if (is_x || !c.bias) return;
+  __syncthreads();
+  mm = block_max(mm, lds);
+  if (threadIdx.x == 0 && mm > 0.f) atomicMax(&c.head[4], __float_as_int(mm));
 }
 
 // one stored row of an operand: bf16 copied, fp32 split; zeros behind the last column
-template <bool F32> __device__ __forceinline__ void pack_row(const char *src, char *dst, long long ld, int cols, float scale) {
+template <bool F32> __device__ __forceinline__ void pack_row(const char *src, char *dst, long long ld, int cols, float scale, float most) {
   if constexpr (F32) {
     const float *s = (const float *)src;
     for (int k = threadIdx.x * 4; k < ld / 4; k += 1024) {
@@ -209,7 +222,10 @@ template <bool F32> __device__ __forceinline__ void pack_row(const char *src, ch
 #pragma unroll
         for (int e = 0; e < 4; ++e) t[e] = k + e < cols ? s[k + e] : 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) split16(t[e] * scale, h[e], l[e]);
+      for (int e = 0; e < 4; ++e) {
+        const float u = t[e] * scale;
+        split16(u > most ? most : u < -most ? -most : u, h[e], l[e]);                         // NaN stays
+      }
       char *d = dst + (k >> 5) * 128 + (k & 31) * 2;
       *reinterpret_cast<uint2 *>(d) = *reinterpret_cast<uint2 *>(h);
       *reinterpret_cast<uint2 *>(d + 64) = *reinterpret_cast<uint2 *>(l);
@@ -234,10 +250,10 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(Ce c) {
     if (b >= c.head[0]) return;
     const int r = c.index[b];
     const char *src = c.x + r * c.x_stride * (F32 ? 4 : 2);
-    pack_row<F32>(src, c.xp + b * c.ldx, c.ldx, c.hidden, F32 ? scale_for(c.xmax[b]) : 1.f);
+    pack_row<F32>(src, c.xp + b * c.ldx, c.ldx, c.hidden, F32 ? scale_for(c.xmax[b]) : 1.f, INFINITY);
   } else {
     const int v = b - c.rows;
-    pack_row<F32>(c.w + v * c.w_stride * (F32 ? 4 : 2), c.wp + v * c.ldw, c.ldw, c.hidden, F32 ? scale_of(c, 2) : 1.f);
+    pack_row<F32>(c.w + v * c.w_stride * (F32 ? 4 : 2), c.wp + v * c.ldw, c.ldw, c.hidden, F32 ? scale_of_w(c) : 1.f, F32 && masked_class(c, v) ? 65504.f : INFINITY);
   }
 }
 
@@ -255,7 +271,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void ce_logits_kernel(Ce c, int row0
   run<T>(lds, side_kc<T>(c.wp, c.ldw, c.classes, c.ldx, ti * T::BI, 0), side_kc<T>(c.xp + row0 * c.ldx, c.ldx, live, c.ldx, tj * T::BJ, 0),
          (int)(c.ldx / 128), acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave % T::NWI, wj = wave / T::NWI;
-  const float rsw = T::SPLIT ? 1.f / scale_of(c, 2) : 1.f;
+  const float rsw = T::SPLIT ? 1.f / scale_of_w(c) : 1.f;
   const int vpad = (int)(c.ldg / (T::SPLIT ? 4 : 2));
   constexpr int WI = T::TI * 16;
   static_assert(kStatCols % WI == 0, "a wave's classes lie in one pair");
@@ -409,7 +425,7 @@ __global__ __launch_bounds__(256) void ce_grad_kernel(Ce c, int row0, int wcols,
     // exponentials relative to their pair's maximum -> p / (1 - p_label)
     const float f = s > 0 ? (float)(1. / s) : (float)(s * 0.), t = (float)(rest * (double)w / (double)((const float *)c.head)[1]);
     if constexpr (F32) {
-      if (threadIdx.x == 0) c.row[row0 + j] = make_float4(ms, f, t, scale_of(c, 3) / scale_for(c.xmax[row0 + j]));
+      if (threadIdx.x == 0) c.row[row0 + j] = make_float4(ms, f, t, scale_of_x(c) / scale_for(c.xmax[row0 + j]));
     } else {
       char *row = c.g + j * c.ldg;
       for (long long k = threadIdx.x * 8; k < c.ldg / 2; k += 2048) {
@@ -563,7 +579,7 @@ template <bool F32> __device__ __forceinline__ void dx_row(const Ce &c, int row0
   const int hp = (c.hidden + 3) / 4 * 4;
   const int p = c.pos[r];
   if (p >= 0 && (p < row0 || p >= row0 + live)) return;                       // another piece's row
-  const float t = p < 0 ? 0.f : F32 ? c.row[p].z : c.t[p], ws = F32 ? 1.f / kSG / scale_of(c, 2) : 1.f;      // one by one: their product may leave fp32's range
+  const float t = p < 0 ? 0.f : F32 ? c.row[p].z : c.t[p], ws = F32 ? 1.f / kSG / scale_of_w(c) : 1.f;      // one by one: their product may leave fp32's range
   for (int k = threadIdx.x * 4; k < c.hidden; k += 1024) {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (p >= 0) {
@@ -619,7 +635,7 @@ template <class T> __device__ __forceinline__ void dw_tile(const Ce &c, int row0
     __syncthreads();
     const int s = from / T::KK;
     run<T>(lds, side_ks<T>(x, c.ldx, live, c.ldx, ti * T::BI * E, s), side_ks<T>(c.g, c.ldg, live, c.ldg, (long long)tj * T::BJ * E, s),
-           (live - from + T::KK - 1) / T::KK, acc, ClassScales<T>{scales + wj * T::TJ * 16 + (lane & 15), 1.f / scale_of(c, 3)});
+           (live - from + T::KK - 1) / T::KK, acc, ClassScales<T>{scales + wj * T::TJ * 16 + (lane & 15), 1.f / scale_of_x(c)});
   } else {
     run<T>(lds, side_ks<T>(x, c.ldx, live, c.ldx, ti * T::BI * E, 0), side_ks<T>(c.g, c.ldg, live, c.ldg, (long long)tj * T::BJ * E, 0),
            (live + T::KK - 1) / T::KK, acc);

@@ -537,8 +537,8 @@ int mr3d_layer_norm_backward(const void *x, long long x_stride, const void *dy, 
  * NULL.  A row counts when its weight is not 0, its label is not ignore_index and it lies before *valid_rows_dev; the others take no part whatever
  * they hold and get zeros in dx.  avg: *avg_factor_dev, else avg_factor when it is > 0, else max(number of counted rows with a positive weight, 1).
  * A counted row whose label is outside [0, classes) makes the loss, its dx row and dweight NaN.  want_*: which gradients are written.
- * fp32 products carry 22 bits of each factor, of x relative to the largest of its row, of weight to the largest of all, of the logits' gradients to the
- * largest of their row (dx) or of their class in 128 rows (dweight): what is 2^17 times smaller has fewer, what is 2^39 times smaller none.  bf16:
+ * fp32 products carry 22 bits of each factor, of x relative to the largest of its row, of weight to the largest of all (of the classes with a bias above
+ * -1e30: what masked ones hold does not count), of the logits' gradients to the largest of their row (dx) or of their class in 128 rows (dweight): what is 2^17 times smaller has fewer, what is 2^39 times smaller none.  bf16:
  * the logits' gradients but the label's and, for dweight, x times its row's factor are rounded to bf16 before their products.  Sums are fp32 or wider,
  * in a fixed order.  hidden <= 65536, classes <= 2^20, rows <= 2^22.  workspace: 1024-byte aligned device memory
  * of mr3d_linear_cross_entropy_workspace_bytes (0 = refused): x (and, fp32 or unaligned, weight) in packed form, dx in fp32, and at most about 2 GiB of

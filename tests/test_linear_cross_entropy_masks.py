@@ -53,3 +53,25 @@ def test_labels_that_are_masked(dtype):
         step = 2.0 ** -16 if dtype == torch.float32 else 2.0 ** -6
         for got, ref in ((dx, g @ w.double()), (dw, g.t() @ x.double()), (db, g.sum(0))):
             assert float((got.double().cpu() - ref).norm()) <= step * float(ref.norm())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('low', [float('-inf'), torch.finfo(torch.float32).min])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_masked_classes_may_have_any_finite_weights(dtype, low):
+    """weights of 1e-30 to 1e30 in classes that the bias takes out: the others' loss and gradients have the bits of the same call with zeros there"""
+    from mr3d_amd.core import linear_cross_entropy
+    x, w, b, label, rw = (t.cuda() for t in _inputs(60, 40, 500, dtype, dead=0.1))
+    keep = torch.ones(500, dtype=torch.bool, device='cuda')
+    keep[::5], keep[256:384] = False, False
+    kept = keep.nonzero().squeeze(1)
+    label = torch.where(label < 0, label, kept[label % len(kept)])
+    b = b.float().masked_fill(~keep, low)
+    out = []
+    for junk in (0.0, 1e-30, 1.0, 1e8, 1e30):
+        wj = torch.where(keep[:, None], w, torch.randn(500, 40, generator=torch.Generator().manual_seed(1)).cuda().to(dtype) * junk)
+        leaves = [t.detach().requires_grad_(True) for t in (x, wj, b)]
+        loss = linear_cross_entropy(leaves[0], leaves[1], label, rw, leaves[2])
+        out.append([loss.detach(), *torch.autograd.grad(loss, leaves)])
+        assert all(bool(torch.isfinite(t).all()) for t in out[-1]) and not out[-1][2][~keep].any(), junk
+        assert all(torch.equal(p, q) for p, q in zip(out[0], out[-1])), junk
