@@ -15,9 +15,8 @@ def linear_cross_entropy(x, weight, label, row_weight=None, bias=None, avg_facto
     the same where those rows have weight 0, as the samplers leave them).  A counted label outside [0, C) makes the loss NaN.
     Beside copies of x and weight the memory is bounded (2 GiB of exponentials, rows go through in pieces).  fp32: products carry 22 bits of
     each factor, relative to the largest of its row (x, and g for dx), of its class (g for dW) or of all (weight, but classes
-    whose bias is -1e30 or less).  bf16 gradients are rounded
-    once more when the incoming gradient is no power of two.  One backward per call; under graph capture both are captured (as
-    `torch.cuda.make_graphed_callables` does) or neither."""
+    whose bias is -1e30 or less).  bf16 gradients are rounded once more when the incoming gradient is no power of two.  One backward per call; under
+    graph capture both are captured (as `torch.cuda.make_graphed_callables` does) or neither."""
     on_device = torch.is_tensor(avg_factor)
     return _hip.train_ops().linear_cross_entropy(x, weight, label, row_weight, bias, avg_factor if on_device else None,
                                                  None if on_device else avg_factor, valid_rows, ignore_index)
